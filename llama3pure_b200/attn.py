@@ -28,7 +28,7 @@ ERRORS = {
     -6: "L3P_E_UNSUPPORTED",
 }
 
-# Every symbol include/llama3pure_attn.h declares.
+# Every symbol include/llama3pure_attn.h and include/llama3pure_paged.h declare.
 EXPORTS = (
     "l3p_attn_create",
     "l3p_attn_destroy",
@@ -74,6 +74,26 @@ EXPORTS = (
     "l3p_attn_wo_allreduce_dev",
     "l3p_attn_decode_noalloc",
     "l3p_attn_noalloc_last_error",
+    "l3p_paged_create",
+    "l3p_paged_destroy",
+    "l3p_paged_last_error",
+    "l3p_paged_check",
+    "l3p_paged_launch_count",
+    "l3p_paged_storage",
+    "l3p_paged_seq_new",
+    "l3p_paged_seq_fork",
+    "l3p_paged_seq_copy",
+    "l3p_paged_seq_truncate",
+    "l3p_paged_seq_free",
+    "l3p_paged_seq_length",
+    "l3p_paged_tables",
+    "l3p_paged_free_pages",
+    "l3p_paged_compact",
+    "l3p_paged_begin",
+    "l3p_paged_set_rope",
+    "l3p_paged_rope_append_dev",
+    "l3p_paged_append_dev",
+    "l3p_paged_attn_dev",
 )
 
 
@@ -111,6 +131,42 @@ class RopeConfig(C.Structure):
     ]
 
 
+class PagedConfig(C.Structure):
+    """Mirror of l3p_paged_config."""
+
+    _fields_ = [(n, C.c_int) for n in ("n_layers", "n_heads", "n_kv_heads", "head_dim", "page_size", "n_pages",
+                                       "max_seqs", "max_tokens", "max_seq_len", "dtype")] + [
+        ("scale", C.c_float),
+        ("is_gemma3", C.c_int),
+        ("swa_window", C.c_int),
+        ("swa_pattern", C.c_int),
+        ("device", C.c_int),
+    ]
+
+
+class PagedRopeConfig(C.Structure):
+    """Mirror of l3p_paged_rope_config."""
+
+    _fields_ = [
+        ("max_pos", C.c_int),
+        ("layout", C.c_int),
+        ("rotary_dim", C.c_int),
+        ("scaling", C.c_int),
+        ("theta", C.c_float),
+        ("theta_swa", C.c_float),
+        ("factor", C.c_float),
+        ("low_freq", C.c_float),
+        ("high_freq", C.c_float),
+        ("beta_fast", C.c_float),
+        ("beta_slow", C.c_float),
+        ("original_len", C.c_int),
+        ("attn_factor", C.c_float),
+        ("rms_norm_eps", C.c_float),
+        ("q_norm", C.c_void_p),
+        ("k_norm", C.c_void_p),
+    ]
+
+
 class AttnError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"{ERRORS.get(code, code)}: {msg}")
@@ -132,7 +188,7 @@ def load_library(path: str = LIB_PATH):
             "(the CUDA path is the only implementation)"
         )
     lib = C.CDLL(path)
-    vp, fp, i = C.c_void_p, C.c_void_p, C.c_int
+    vp, fp, i, ll, ip = C.c_void_p, C.c_void_p, C.c_int, C.c_longlong, C.c_void_p
     sig = {
         "l3p_attn_create": (i, [C.POINTER(AttnConfig), C.POINTER(C.c_void_p)]),
         "l3p_attn_destroy": (None, [vp]),
@@ -178,6 +234,26 @@ def load_library(path: str = LIB_PATH):
         "l3p_attn_wo_allreduce_dev": (i, [vp, i, fp, fp, vp]),
         "l3p_attn_decode_noalloc": (i, [C.POINTER(AttnConfig), i, i, fp, fp, fp, fp, vp]),
         "l3p_attn_noalloc_last_error": (C.c_char_p, []),
+        "l3p_paged_create": (i, [C.POINTER(PagedConfig), C.POINTER(C.c_void_p)]),
+        "l3p_paged_destroy": (None, [vp]),
+        "l3p_paged_last_error": (C.c_char_p, [vp]),
+        "l3p_paged_check": (i, [vp, vp]),
+        "l3p_paged_launch_count": (C.c_longlong, [vp]),
+        "l3p_paged_storage": (i, [vp, C.POINTER(C.c_void_p), C.POINTER(C.c_size_t)]),
+        "l3p_paged_seq_new": (i, [vp, ip]),
+        "l3p_paged_seq_fork": (i, [vp, i, i, i, ip]),
+        "l3p_paged_seq_copy": (i, [vp, i, ip, ip, vp]),
+        "l3p_paged_seq_truncate": (i, [vp, i, i]),
+        "l3p_paged_seq_free": (i, [vp, i, ip]),
+        "l3p_paged_seq_length": (i, [vp, i, ip]),
+        "l3p_paged_tables": (i, [vp, i, ip, i, ip, ip]),
+        "l3p_paged_free_pages": (i, [vp, ip]),
+        "l3p_paged_compact": (i, [vp, ip, vp]),
+        "l3p_paged_begin": (i, [vp, i, ip, ip, vp]),
+        "l3p_paged_set_rope": (i, [vp, C.POINTER(PagedRopeConfig)]),
+        "l3p_paged_rope_append_dev": (i, [vp, i, vp, ll, vp, ll, vp, ll, vp, ll, vp]),
+        "l3p_paged_append_dev": (i, [vp, i, vp, ll, vp, ll, vp]),
+        "l3p_paged_attn_dev": (i, [vp, i, vp, ll, vp, ll, vp]),
     }
     for name, (res, args) in sig.items():
         f = getattr(lib, name)

@@ -1,0 +1,733 @@
+// l3p_paged.cu -- the paged cache: pool, sequences, pages, and the batch
+// description of a step (llama3pure_paged.h).  Books are kept on the host;
+// the device holds the storage and what the current step's kernels read.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstring>
+#include <functional>
+#include <new>
+
+#include "paged.h"
+#include "ptx.cuh"
+
+using namespace l3p;
+using namespace l3p_pg;
+
+namespace {
+
+using Ctx = l3p_paged_ctx;
+
+int pages_for(const Ctx* ctx, int tokens) { return (tokens + ctx->cfg.page_size - 1) >> ctx->shift; }
+
+int take_page(Ctx* ctx) {
+  std::pop_heap(ctx->free_heap.begin(), ctx->free_heap.end(), std::greater<int>());
+  const int p = ctx->free_heap.back();
+  ctx->free_heap.pop_back();
+  ctx->refs[p] = 1;
+  ctx->fill[p] = 0;
+  return p;
+}
+
+void drop_page(Ctx* ctx, int p) {
+  if (--ctx->refs[p] == 0) {
+    ctx->free_heap.push_back(p);
+    std::push_heap(ctx->free_heap.begin(), ctx->free_heap.end(), std::greater<int>());
+  }
+}
+
+int check_seq(Ctx* ctx, int seq) {
+  if (seq < 0 || seq >= (int)ctx->seqs.size() || !ctx->seqs[seq].live)
+    return fail(ctx, L3P_E_RANGE, "there is no sequence %d", seq);
+  return L3P_OK;
+}
+
+// Every id is a live sequence, and no id comes twice.
+int check_seqs(Ctx* ctx, int n, const int* seqs) {
+  std::vector<char> seen(ctx->seqs.size(), 0);
+  for (int i = 0; i < n; ++i) {
+    if (int rc = check_seq(ctx, seqs[i])) return rc;
+    if (seen[seqs[i]]) return fail(ctx, L3P_E_INVAL, "sequence %d is given twice", seqs[i]);
+    seen[seqs[i]] = 1;
+  }
+  return L3P_OK;
+}
+
+int free_seq_count(const Ctx* ctx) {
+  int n = 0;
+  for (const auto& s : ctx->seqs) n += !s.live;
+  return n;
+}
+
+int new_seq(Ctx* ctx) {
+  for (size_t i = 0; i < ctx->seqs.size(); ++i)
+    if (!ctx->seqs[i].live) {
+      ctx->seqs[i].live = true;
+      ctx->seqs[i].len = 0;
+      ctx->seqs[i].pages.clear();
+      return (int)i;
+    }
+  return -1;
+}
+
+// A pinned staging slot of at least `words` words whose last upload is done.
+int take_slot(Ctx* ctx, size_t words, Ctx::Slot** out) {
+  Ctx::Slot& s = ctx->slots[ctx->slot_next++ % Ctx::kSlots];
+  if (s.used) PG_CUDA(ctx, cudaEventSynchronize(s.done));
+  s.used = false;
+  if (s.words < words) {
+    if (s.host) cudaFreeHost(s.host);
+    s.host = nullptr;
+    s.words = 0;
+    const size_t want = std::max(words + words / 2, (size_t)16384);
+    if (cudaHostAlloc(&s.host, want * 4, cudaHostAllocDefault) != cudaSuccess) {
+      cudaGetLastError();
+      return fail(ctx, L3P_E_NOMEM, "pinned staging of %zu bytes failed", want * 4);
+    }
+    s.words = want;
+  }
+  if (!s.done) PG_CUDA(ctx, cudaEventCreateWithFlags(&s.done, cudaEventDisableTiming));
+  *out = &s;
+  return L3P_OK;
+}
+
+int upload(Ctx* ctx, Ctx::Slot* s, int* dev, size_t words, cudaStream_t st) {
+  PG_CUDA(ctx, cudaMemcpyAsync(dev, s->host, words * 4, cudaMemcpyHostToDevice, st));
+  PG_CUDA(ctx, cudaEventRecord(s->done, st));
+  s->used = true;
+  return L3P_OK;
+}
+
+// Enqueues the page copies `jobs` (source, destination, rows, 0).
+int copy_pages(Ctx* ctx, const std::vector<int4>& jobs, cudaStream_t st) {
+  if (jobs.empty()) return L3P_OK;
+  Ctx::Slot* s;
+  if (int rc = take_slot(ctx, jobs.size() * 4, &s)) return rc;
+  memcpy(s->host, jobs.data(), jobs.size() * sizeof(int4));
+  if (int rc = upload(ctx, s, ctx->jobs, jobs.size() * 4, st)) return rc;
+  return launch_page_copy(ctx, (int)jobs.size(), st);
+}
+
+cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
+
+int refuse_capture(Ctx* ctx, cudaStream_t s, const char* what) {
+  if (capturing(s)) return fail(ctx, L3P_E_INVAL, "%s moves host data: not during stream capture", what);
+  return L3P_OK;
+}
+
+// ---- the batch description -----------------------------------------------------
+
+struct BatchSeq {
+  int q_row0, n_new, len, tbl;  // len: with the new tokens
+};
+
+// First key that the token at `pos` attends to.
+int first_key(const Ctx* ctx, bool win, int pos) { return win ? std::max(0, pos - ctx->cfg.swa_window + 1) : 0; }
+
+// Row kernel: the tiles of all units (sequence, KV head, block of 8*nt rows)
+// laid end to end and cut into equal runs, one per CTA, so that every CTA
+// streams the same number of key tiles whatever the lengths are.  A run is a
+// multiple of the CTA's warps, which take its tiles in turn.
+void plan_rows(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, int nt, std::vector<int>* first,
+               std::vector<PgSeg>* segs) {
+  const int limit = row_limit(ctx), rt = 8 * nt, warps = row_warps(ctx), G = ctx->G;
+  std::vector<PgSeg> units;
+  long long total = 0;
+  for (const auto& b : bs) {
+    const long long rows = (long long)b.n_new * G;
+    if (rows == 0 || rows > limit) continue;
+    const int pos0 = b.len - b.n_new;
+    for (int h = 0; h < ctx->cfg.n_kv_heads; ++h)
+      for (int r0 = 0; r0 < rows; r0 += rt) {
+        PgSeg u{};
+        u.tbl = b.tbl;
+        u.q_row0 = b.q_row0;
+        u.pos0 = pos0;
+        u.r0 = r0;
+        u.n_rows = (int)std::min<long long>(rt, rows - r0);
+        u.kvh = h;
+        u.key_lo = first_key(ctx, win, pos0 + r0 / G);
+        u.key_hi = pos0 + (r0 + u.n_rows - 1) / G + 1;
+        u.tile0 = u.key_lo / kPgTile;
+        u.tile1 = (u.key_hi + kPgTile - 1) / kPgTile;
+        total += u.tile1 - u.tile0;
+        units.push_back(u);
+      }
+  }
+  if (units.empty()) return;
+  const long long max_ctas = std::min(ctx->num_sms, kPgMaxCtas);
+  long long run = (total + max_ctas - 1) / max_ctas;
+  run = (run + warps - 1) / warps * warps;
+  const int n_cta = (int)((total + run - 1) / run);
+  long long at = 0;  // tiles laid so far
+  first->assign(1, 0);
+  for (auto& u : units) {
+    const int n = u.tile1 - u.tile0, t_begin = u.tile0, t_end = u.tile1;
+    const int c0 = (int)(at / run), c1 = (int)((at + n - 1) / run);
+    int t = t_begin;
+    for (int c = c0; c <= c1; ++c) {
+      const int end = (int)std::min<long long>(t_end, t_begin + ((long long)(c + 1) * run - at));
+      PgSeg g = u;
+      g.tile0 = t;
+      g.tile1 = end;
+      g.part = c - c0;
+      g.n_parts = c1 - c0 + 1;
+      g.cta0 = c0;
+      while ((int)first->size() <= c) first->push_back((int)segs->size());
+      segs->push_back(g);
+      t = end;
+    }
+    at += n;
+  }
+  while ((int)first->size() <= n_cta) first->push_back((int)segs->size());
+}
+
+// Tensor-core kernels: units (sequence, KV head, block of rows); with too few
+// of them for the GPU (bf16), long key ranges are cut into parts of equal
+// size, merged by the part that ends last.  Longest parts first.
+void plan_tc_bf16(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vector<PgPart>* parts) {
+  const int limit = row_limit(ctx), tile = tc_tile(ctx), rt = tc_rows(ctx), G = ctx->G;
+  std::vector<PgPart> units;
+  long long total = 0;
+  for (const auto& b : bs) {
+    const long long rows = (long long)b.n_new * G;
+    if (rows <= limit) continue;
+    const int pos0 = b.len - b.n_new;
+    for (long long r0 = 0; r0 < rows; r0 += rt)
+      for (int h = 0; h < ctx->cfg.n_kv_heads; ++h) {
+        PgPart u{};
+        u.tbl = b.tbl;
+        u.q_row0 = b.q_row0;
+        u.pos0 = pos0;
+        u.r0 = (int)r0;
+        u.n_rows = (int)std::min<long long>(rt, rows - r0);
+        u.kvh = h;
+        u.key_hi = pos0 + (int)((r0 + u.n_rows - 1) / G) + 1;
+        u.tile0 = first_key(ctx, win, pos0 + (int)(r0 / G)) / tile;
+        u.tile1 = (u.key_hi + tile - 1) / tile;
+        total += u.tile1 - u.tile0;
+        units.push_back(u);
+      }
+  }
+  // no part is shorter than 4 tiles: below that the merge costs more than the split saves
+  const int cap = (int)std::max<long long>(4, (total + ctx->num_sms - 1) / ctx->num_sms);
+  int ticket = 0, slot = 0;
+  for (const auto& u : units) {
+    const int n = u.tile1 - u.tile0, k = (n + cap - 1) / cap;
+    for (int i = 0; i < k; ++i) {
+      PgPart p = u;
+      p.tile0 = u.tile0 + (int)((long long)n * i / k);
+      p.tile1 = u.tile0 + (int)((long long)n * (i + 1) / k);
+      p.part = i;
+      p.n_parts = k;
+      p.ticket = ticket;
+      p.slot = slot;  // of part 0
+      parts->push_back(p);
+    }
+    if (k > 1) {
+      ++ticket;
+      slot += k;
+    }
+  }
+  std::stable_sort(parts->begin(), parts->end(),
+                   [](const PgPart& a, const PgPart& b) { return a.tile1 - a.tile0 > b.tile1 - b.tile0; });
+}
+
+// fp32 pools: units (sequence, 128 query tokens) times the query heads, and the key tiles they read.
+void plan_tc_f32(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vector<PgPart>* parts,
+                 std::vector<PgPrep>* prep) {
+  const int limit = row_limit(ctx);
+  for (const auto& b : bs) {
+    if ((long long)b.n_new * ctx->G <= limit) continue;
+    const int pos0 = b.len - b.n_new;
+    const int t0 = first_key(ctx, win, pos0) / 128, t1 = (b.len + 127) / 128;
+    const int img0 = (int)prep->size() - t0;  // image of the sequence's tile 0
+    for (int t = t0; t < t1; ++t) prep->push_back({b.tbl, t * 128, b.len, img0 + t});
+    for (int r0 = 0; r0 < b.n_new; r0 += 128) {
+      PgPart u{};
+      u.tbl = b.tbl;
+      u.key_hi = b.len;
+      u.q_row0 = b.q_row0;
+      u.pos0 = pos0;
+      u.img = img0;
+      u.qbase = pos0 + r0;
+      u.q_end = b.len;
+      u.tile0 = first_key(ctx, win, u.qbase) / 128;
+      u.tile1 = (std::min(u.qbase + 128, u.q_end) - 1) / 128 + 1;
+      parts->push_back(u);
+    }
+  }
+  std::stable_sort(parts->begin(), parts->end(),
+                   [](const PgPart& a, const PgPart& b) { return a.tile1 - a.tile0 > b.tile1 - b.tile0; });
+}
+
+// Lays the current batch out as the kernels read it.
+void build_batch(const Ctx* ctx, const std::vector<BatchSeq>& bs, const int* seqs, int n_seqs, int n_tokens,
+                 std::vector<int>* words, PgHeader* hdr) {
+  PgHeader h{};
+  h.n_tokens = n_tokens;
+  h.n_seqs = n_seqs;
+  const int limit = row_limit(ctx);
+  int max_rows = 0;
+  for (const auto& b : bs)
+    if ((long long)b.n_new * ctx->G <= limit) max_rows = std::max(max_rows, b.n_new * ctx->G);
+  h.row_nt = std::min(max_rows <= 8 ? 1 : max_rows <= 16 ? 2 : 4, row_max_nt(ctx));
+  auto& w = *words;
+  w.assign(kPgHdrWords, 0);
+  auto add = [&](const void* p, size_t bytes) {
+    while (w.size() % 4) w.push_back(0);  // records are read 16 bytes at a time
+    const size_t at = w.size();
+    w.resize(at + bytes / 4);
+    if (bytes) memcpy(w.data() + at, p, bytes);
+    return (int)at;
+  };
+  for (int v = 0; v < (ctx->swa ? 2 : 1); ++v) {
+    std::vector<int> first;
+    std::vector<PgSeg> segs;
+    std::vector<PgPart> parts;
+    std::vector<PgPrep> prep;
+    plan_rows(ctx, v == 1, bs, h.row_nt, &first, &segs);
+    if (ctx->bf16)
+      plan_tc_bf16(ctx, v == 1, bs, &parts);
+    else if (ctx->hd != 256)
+      plan_tc_f32(ctx, v == 1, bs, &parts, &prep);
+    PgLists& l = h.lists[v];
+    l.row_ctas = first.empty() ? 0 : (int)first.size() - 1;
+    l.row_first = add(first.data(), first.size() * 4);
+    l.row_segs = add(segs.data(), segs.size() * sizeof(PgSeg));
+    l.n_tc = (int)parts.size();
+    l.tc_parts = add(parts.data(), parts.size() * sizeof(PgPart));
+    l.n_prep = (int)prep.size();
+    l.prep = add(prep.data(), prep.size() * sizeof(PgPrep));
+  }
+  std::vector<int2> tok(n_tokens);
+  h.tbl = 0;
+  size_t tbl_words = 0;
+  for (int i = 0; i < n_seqs; ++i) {
+    const auto& s = ctx->seqs[seqs[i]];
+    const auto& b = bs[i];
+    tbl_words += s.pages.size();
+    for (int t = 0; t < b.n_new; ++t) {
+      const int pos = b.len - b.n_new + t;
+      tok[b.q_row0 + t] = make_int2(s.pages[pos >> ctx->shift] * ctx->cfg.page_size + (pos & (ctx->cfg.page_size - 1)), pos);
+    }
+  }
+  h.tok = add(tok.data(), tok.size() * sizeof(int2));
+  h.tbl = add(nullptr, 0);
+  w.reserve(w.size() + tbl_words);
+  for (int i = 0; i < n_seqs; ++i) {
+    const auto& s = ctx->seqs[seqs[i]];
+    w.insert(w.end(), s.pages.begin(), s.pages.end());
+  }
+  memcpy(w.data(), &h, sizeof h);
+  *hdr = h;
+}
+
+// Words of the largest batch block: bounds on what build_batch lays out.
+size_t batch_capacity(const Ctx* ctx) {
+  const auto& c = ctx->cfg;
+  const size_t max_len = c.max_seq_len;
+  // units of either path: blocks of at least 8 rows (row kernel), plus one part or segment per CTA and per unit
+  const size_t units = (size_t)c.n_kv_heads * (((size_t)c.max_tokens * ctx->G + 7) / 8 + c.max_seqs);
+  const size_t lists = (units + 2 * kPgMaxCtas + 8) * 16 + kPgMaxCtas + 8;
+  const size_t tiles = ctx->bf16 ? 0 : (size_t)c.max_seqs * ((max_len + 127) / 128 + 1) * 4;
+  const size_t table = (size_t)c.max_seqs * ((max_len + c.page_size - 1) / c.page_size);
+  return kPgHdrWords + 2 * (lists + lists + tiles) + 2 * (size_t)c.max_tokens + table + 64;
+}
+
+void release(Ctx* ctx) {
+  cudaFree(ctx->storage);
+  cudaFree(ctx->batch);
+  cudaFree(ctx->jobs);
+  for (auto& s : ctx->slots) {
+    if (s.host) cudaFreeHost(s.host);
+    if (s.done) cudaEventDestroy(s.done);
+  }
+  cudaFree(ctx->ws_o);
+  cudaFree(ctx->ws_ml);
+  cudaFree(ctx->tickets);
+  cudaFree(ctx->tc_o);
+  cudaFree(ctx->tc_ml);
+  cudaFree(ctx->tc_tickets);
+  cudaFree(ctx->img);
+  cudaFree(ctx->v_flags);
+  if (ctx->rope_tab_swa != ctx->rope_tab) cudaFree(ctx->rope_tab_swa);
+  cudaFree(ctx->rope_tab);
+  cudaFree(ctx->qk_norm);
+  if (ctx->err_host) cudaFreeHost(ctx->err_host);
+}
+
+// Runs `f`, turning a host allocation failure into L3P_E_NOMEM: no C++
+// exception leaves the C ABI.
+template <typename F>
+int guarded(Ctx* ctx, F f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return fail(ctx, L3P_E_NOMEM, "host memory is exhausted");
+  } catch (...) {
+    return fail(ctx, L3P_E_NOMEM, "host library failure");
+  }
+}
+
+int create(const l3p_paged_config& in, Ctx** out) {
+  l3p_paged_config c = in;
+  if (c.n_layers <= 0 || c.n_heads <= 0 || c.n_kv_heads <= 0 || c.n_heads % c.n_kv_heads != 0) return L3P_E_INVAL;
+  if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return L3P_E_UNSUPPORTED;
+  if (c.page_size != 16 && c.page_size != 32 && c.page_size != 64 && c.page_size != 128) return L3P_E_UNSUPPORTED;
+  if (c.n_pages <= 0 || c.max_seqs <= 0 || c.max_tokens <= 0 || c.max_seq_len < 0) return L3P_E_INVAL;
+  if (c.dtype != L3P_PAGED_F32 && c.dtype != L3P_PAGED_BF16) return L3P_E_INVAL;
+  if (!std::isfinite(c.scale) || c.swa_window < 0 || c.swa_pattern < 0 || c.device < 0) return L3P_E_INVAL;
+  // positions, storage rows and query rows are counted in 32 bits
+  const long long pool_pos = (long long)c.n_pages * c.page_size;
+  if (pool_pos > INT_MAX / 2 || c.max_seqs > 65536) return L3P_E_RANGE;
+  if (c.max_seq_len == 0 || c.max_seq_len > pool_pos) c.max_seq_len = (int)pool_pos;
+  if ((long long)c.max_tokens * c.n_heads > INT_MAX / 2) return L3P_E_RANGE;
+  if (pool_pos * c.n_layers * 2 * c.n_kv_heads > INT_MAX) return L3P_E_RANGE;  // rows of the tensor map
+  Ctx* ctx = new Ctx;
+  ctx->cfg = c;
+  ctx->hd = c.head_dim;
+  ctx->G = c.n_heads / c.n_kv_heads;
+  ctx->bf16 = c.dtype == L3P_PAGED_BF16;
+  ctx->es = ctx->bf16 ? 2 : 4;
+  while ((1 << ctx->shift) < c.page_size) ++ctx->shift;
+  ctx->swa = c.is_gemma3 && c.swa_window > 0 && c.swa_pattern > 0;
+  ctx->scale = c.scale != 0.f ? c.scale : 1.0f / sqrtf((float)c.head_dim);
+  *out = ctx;
+  DeviceScope dev(c.device);
+  ctx->block_bytes = (size_t)c.page_size * c.head_dim * ctx->es;
+  ctx->page_bytes = ctx->block_bytes * c.n_kv_heads * 2 * c.n_layers;
+  cudaDeviceProp prop;
+  PG_CUDA(ctx, cudaGetDeviceProperties(&prop, c.device));
+  ctx->num_sms = prop.multiProcessorCount;
+  ctx->batch_words = batch_capacity(ctx);
+  if (ctx->batch_words > (1u << 29))
+    return fail(ctx, L3P_E_RANGE, "max_seqs, max_tokens and max_seq_len make a batch description of %zu words",
+                ctx->batch_words);
+  const size_t bytes = ctx->page_bytes * c.n_pages;
+  ctx->jobs_cap = (size_t)c.n_pages;
+  if (cudaMalloc(&ctx->storage, bytes) != cudaSuccess || cudaMalloc(&ctx->batch, ctx->batch_words * 4) != cudaSuccess ||
+      cudaMalloc(&ctx->jobs, ctx->jobs_cap * sizeof(int4)) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(ctx, L3P_E_NOMEM, "a pool of %zu bytes does not fit on the device", bytes);
+  }
+  PG_CUDA(ctx, cudaMemset(ctx->storage, 0, bytes));
+  PG_CUDA(ctx, cudaHostAlloc(&ctx->err_host, sizeof(int), cudaHostAllocMapped));
+  *ctx->err_host = 0;
+  PG_CUDA(ctx, cudaHostGetDevicePointer(&ctx->err_dev, ctx->err_host, 0));
+  ctx->seqs.resize(c.max_seqs);
+  ctx->refs.assign(c.n_pages, 0);
+  ctx->fill.assign(c.n_pages, 0);
+  ctx->free_heap.resize(c.n_pages);
+  for (int i = 0; i < c.n_pages; ++i) ctx->free_heap[i] = i;  // ascending: a min-heap already
+  if (int rc = init_rows(ctx)) return rc;
+  if (int rc = ctx->bf16 ? init_tc(ctx) : init_f32(ctx)) return rc;
+  PG_CUDA(ctx, cudaDeviceSynchronize());  // the storage is zero before any stream of the caller's writes it
+  return L3P_OK;
+}
+
+int begin(Ctx* ctx, int n_seqs, const int* ids, const int* n_new, cudaStream_t s) {
+  if (int rc = check_seqs(ctx, n_seqs, ids)) return rc;
+  long long tokens = 0, need = 0;
+  for (int i = 0; i < n_seqs; ++i) {
+    const auto& q = ctx->seqs[ids[i]];
+    if (n_new[i] < 0) return fail(ctx, L3P_E_INVAL, "sequence %d grows by %d tokens", ids[i], n_new[i]);
+    if ((long long)q.len + n_new[i] > ctx->cfg.max_seq_len)
+      return fail(ctx, L3P_E_RANGE, "sequence %d would hold %lld of at most %d positions", ids[i],
+                  (long long)q.len + n_new[i], ctx->cfg.max_seq_len);
+    tokens += n_new[i];
+    need += pages_for(ctx, q.len + n_new[i]) - (int)q.pages.size();
+  }
+  if (tokens > ctx->cfg.max_tokens)
+    return fail(ctx, L3P_E_RANGE, "%lld new tokens, at most %d", tokens, ctx->cfg.max_tokens);
+  // shared last pages that a sequence grows into: the holder that finds others
+  // beside it takes a copy; a page all of whose holders grow stays with the last one
+  std::vector<std::pair<int, int>> cow;  // (index in the batch, page)
+  std::vector<int> left;                 // holders of cow[i].second after the copies before it
+  for (int i = 0; i < n_seqs; ++i) {
+    const auto& q = ctx->seqs[ids[i]];
+    if (n_new[i] == 0 || (q.len & (ctx->cfg.page_size - 1)) == 0) continue;
+    const int p = q.pages.back();
+    if (ctx->refs[p] > 1) cow.push_back({i, p});
+  }
+  {
+    std::vector<std::pair<int, int>> take;
+    std::vector<int> gone;  // pages of the copies taken so far
+    std::vector<int> count(cow.empty() ? 0 : ctx->cfg.n_pages, 0);
+    for (const auto& x : cow)
+      if (ctx->refs[x.second] - count[x.second] > 1) {
+        ++count[x.second];
+        take.push_back(x);
+      }
+    cow.swap(take);
+  }
+  need += (long long)cow.size();
+  if (need > (long long)ctx->free_heap.size())
+    return fail(ctx, L3P_E_NOMEM, "the batch needs %lld pages, %zu are free", need, ctx->free_heap.size());
+  if (int rc = refuse_capture(ctx, s, "begin")) return rc;
+
+  // all checks passed: give out pages.  In batch order, a sequence's copy first.
+  ctx->batch_valid = false;
+  std::vector<int4> jobs;
+  std::vector<BatchSeq> bs(n_seqs);
+  size_t next = 0;
+  int row = 0, tbl = 0;
+  ctx->max_pos_in_batch = 0;
+  for (int i = 0; i < n_seqs; ++i) {
+    auto& q = ctx->seqs[ids[i]];
+    if (next < cow.size() && cow[next].first == i) {
+      const int src = q.pages.back(), dst = take_page(ctx), rows = q.len & (ctx->cfg.page_size - 1);
+      jobs.push_back(make_int4(src, dst, rows, 0));
+      drop_page(ctx, src);
+      ctx->fill[dst] = rows;
+      q.pages.back() = dst;
+      ++next;
+    }
+    const int len = q.len + n_new[i], n_pages = pages_for(ctx, len);
+    while ((int)q.pages.size() < n_pages) q.pages.push_back(take_page(ctx));
+    for (int pos = q.len; pos < len; pos = (pos | (ctx->cfg.page_size - 1)) + 1) {
+      const int p = q.pages[pos >> ctx->shift];
+      ctx->fill[p] = std::max(ctx->fill[p], std::min(ctx->cfg.page_size, len - (pos & ~(ctx->cfg.page_size - 1))));
+    }
+    q.len = len;
+    bs[i] = {row, n_new[i], len, tbl};
+    row += n_new[i];
+    if (n_new[i] > 0) ctx->max_pos_in_batch = std::max(ctx->max_pos_in_batch, len);
+    tbl += (int)q.pages.size();
+  }
+  if (int rc = copy_pages(ctx, jobs, s)) return rc;
+  std::vector<int> words;
+  build_batch(ctx, bs, ids, n_seqs, row, &words, &ctx->hdr);
+  if (words.size() > ctx->batch_words) return fail(ctx, L3P_E_RANGE, "batch description of %zu words", words.size());
+  Ctx::Slot* slot;
+  if (int rc = take_slot(ctx, words.size(), &slot)) return rc;
+  memcpy(slot->host, words.data(), words.size() * 4);
+  if (int rc = upload(ctx, slot, ctx->batch, words.size(), s)) return rc;
+  ctx->batch_valid = true;
+  return L3P_OK;
+}
+
+int copy_seqs(Ctx* ctx, int n, const int* ids, int* children, cudaStream_t s) {
+  for (int i = 0; i < n; ++i)
+    if (int rc = check_seq(ctx, ids[i])) return rc;
+  if (n > free_seq_count(ctx))
+    return fail(ctx, L3P_E_NOMEM, "%d sequences more than max_seqs = %d allows", n, ctx->cfg.max_seqs);
+  long long need = 0;
+  for (int i = 0; i < n; ++i) need += ctx->seqs[ids[i]].pages.size();
+  if (need > (long long)ctx->free_heap.size())
+    return fail(ctx, L3P_E_NOMEM, "the copies need %lld pages, %zu are free", need, ctx->free_heap.size());
+  if (int rc = refuse_capture(ctx, s, "copy")) return rc;
+  std::vector<int4> jobs;
+  jobs.reserve(need);
+  for (int i = 0; i < n; ++i) {
+    const int child = new_seq(ctx);
+    auto& dst = ctx->seqs[child];
+    const auto& src = ctx->seqs[ids[i]];
+    dst.len = src.len;
+    for (size_t k = 0; k < src.pages.size(); ++k) {
+      const int p = take_page(ctx), rows = std::min(ctx->cfg.page_size, src.len - (int)k * ctx->cfg.page_size);
+      ctx->fill[p] = rows;
+      dst.pages.push_back(p);
+      jobs.push_back(make_int4(src.pages[k], p, rows, 0));
+    }
+    children[i] = child;
+  }
+  return copy_pages(ctx, jobs, s);
+}
+
+int compact(Ctx* ctx, int* n_used, cudaStream_t s) {
+  if (int rc = refuse_capture(ctx, s, "compact")) return rc;
+  const int k = ctx->cfg.n_pages - (int)ctx->free_heap.size();
+  std::vector<int4> jobs;
+  std::vector<int> moved(ctx->cfg.n_pages, -1);
+  int dst = 0;
+  for (int p = k; p < ctx->cfg.n_pages; ++p) {
+    if (ctx->refs[p] == 0) continue;
+    while (ctx->refs[dst] != 0) ++dst;  // fewer used pages below k than k, so dst stays below k
+    moved[p] = dst;
+    jobs.push_back(make_int4(p, dst, ctx->fill[p], 0));
+    ++dst;
+  }
+  if (!jobs.empty()) {
+    ctx->batch_valid = false;
+    if (int rc = copy_pages(ctx, jobs, s)) return rc;
+    for (const auto& j : jobs) {
+      ctx->refs[j.y] = ctx->refs[j.x];
+      ctx->fill[j.y] = ctx->fill[j.x];
+      ctx->refs[j.x] = 0;
+    }
+    for (auto& q : ctx->seqs)
+      for (auto& p : q.pages)
+        if (moved[p] >= 0) p = moved[p];
+    ctx->free_heap.clear();
+    for (int p = k; p < ctx->cfg.n_pages; ++p) ctx->free_heap.push_back(p);
+  }
+  if (n_used) *n_used = k;
+  return L3P_OK;
+}
+
+}  // namespace
+
+L3P_API int l3p_paged_create(const l3p_paged_config* cfg, l3p_paged_ctx** out) {
+  if (!cfg || !out) return L3P_E_INVAL;
+  *out = nullptr;
+  Ctx* ctx = nullptr;
+  const int rc = guarded(nullptr, [&] { return create(*cfg, &ctx); });
+  if (rc != L3P_OK) {
+    if (ctx) {
+      DeviceScope dev(ctx->cfg.device);
+      release(ctx);
+      delete ctx;
+    }
+    return rc;
+  }
+  *out = ctx;
+  return L3P_OK;
+}
+
+L3P_API void l3p_paged_destroy(l3p_paged_ctx* ctx) {
+  if (!ctx) return;
+  DeviceScope dev(ctx->cfg.device);
+  cudaDeviceSynchronize();
+  release(ctx);
+  delete ctx;
+}
+
+L3P_API const char* l3p_paged_last_error(const l3p_paged_ctx* ctx) { return ctx ? ctx->last_error.c_str() : ""; }
+
+L3P_API long long l3p_paged_launch_count(const l3p_paged_ctx* ctx) { return ctx ? ctx->launches : L3P_E_INVAL; }
+
+L3P_API int l3p_paged_check(l3p_paged_ctx* ctx, void* stream) {
+  if (!ctx) return L3P_E_INVAL;
+  DeviceScope dev(ctx->cfg.device);
+  PG_CUDA(ctx, cudaStreamSynchronize(as_stream(stream)));
+  const int e = *ctx->err_host;
+  *ctx->err_host = 0;
+  if (e == kErrTimeout) return fail(ctx, L3P_E_TIMEOUT, "a bounded wait in a kernel gave up");
+  if (e != 0) return fail(ctx, L3P_E_INVAL, "a captured launch met a batch that it does not serve");
+  return L3P_OK;
+}
+
+L3P_API int l3p_paged_storage(l3p_paged_ctx* ctx, void** base, size_t* bytes) {
+  if (!ctx || !base || !bytes) return ctx ? fail(ctx, L3P_E_INVAL, "null pointer") : L3P_E_INVAL;
+  *base = ctx->storage;
+  *bytes = ctx->page_bytes * ctx->cfg.n_pages;
+  return L3P_OK;
+}
+
+L3P_API int l3p_paged_seq_new(l3p_paged_ctx* ctx, int* seq) {
+  if (!ctx || !seq) return ctx ? fail(ctx, L3P_E_INVAL, "null pointer") : L3P_E_INVAL;
+  return guarded(ctx, [&] {
+    const int id = new_seq(ctx);
+    if (id < 0) return fail(ctx, L3P_E_NOMEM, "max_seqs = %d sequences exist", ctx->cfg.max_seqs);
+    *seq = id;
+    return (int)L3P_OK;
+  });
+}
+
+L3P_API int l3p_paged_seq_fork(l3p_paged_ctx* ctx, int seq, int n_tokens, int n, int* children) {
+  if (!ctx || !children || n < 0) return ctx ? fail(ctx, L3P_E_INVAL, "bad argument") : L3P_E_INVAL;
+  return guarded(ctx, [&]() -> int {
+    if (int rc = check_seq(ctx, seq)) return rc;
+    const int len = n_tokens < 0 ? ctx->seqs[seq].len : n_tokens;
+    if (len > ctx->seqs[seq].len)
+      return fail(ctx, L3P_E_RANGE, "sequence %d has %d positions, not %d", seq, ctx->seqs[seq].len, len);
+    if (n > free_seq_count(ctx))
+      return fail(ctx, L3P_E_NOMEM, "%d sequences more than max_seqs = %d allows", n, ctx->cfg.max_seqs);
+    const int n_pages = pages_for(ctx, len);
+    const std::vector<int> pages(ctx->seqs[seq].pages.begin(), ctx->seqs[seq].pages.begin() + n_pages);
+    for (int i = 0; i < n; ++i) {
+      const int id = new_seq(ctx);
+      ctx->seqs[id].pages = pages;
+      ctx->seqs[id].len = len;
+      for (int p : pages) ++ctx->refs[p];
+      children[i] = id;
+    }
+    return L3P_OK;
+  });
+}
+
+L3P_API int l3p_paged_seq_copy(l3p_paged_ctx* ctx, int n, const int* seqs, int* children, void* stream) {
+  if (!ctx || n < 0 || (n > 0 && (!seqs || !children))) return ctx ? fail(ctx, L3P_E_INVAL, "bad argument") : L3P_E_INVAL;
+  DeviceScope dev(ctx->cfg.device);
+  return guarded(ctx, [&] { return copy_seqs(ctx, n, seqs, children, as_stream(stream)); });
+}
+
+L3P_API int l3p_paged_seq_truncate(l3p_paged_ctx* ctx, int seq, int n_tokens) {
+  if (!ctx || n_tokens < 0) return ctx ? fail(ctx, L3P_E_INVAL, "bad argument") : L3P_E_INVAL;
+  return guarded(ctx, [&]() -> int {
+    if (int rc = check_seq(ctx, seq)) return rc;
+    auto& q = ctx->seqs[seq];
+    if (n_tokens > q.len) return fail(ctx, L3P_E_RANGE, "sequence %d has %d positions, not %d", seq, q.len, n_tokens);
+    ctx->batch_valid = false;
+    while ((int)q.pages.size() > pages_for(ctx, n_tokens)) {
+      drop_page(ctx, q.pages.back());
+      q.pages.pop_back();
+    }
+    q.len = n_tokens;
+    return L3P_OK;
+  });
+}
+
+L3P_API int l3p_paged_seq_free(l3p_paged_ctx* ctx, int n, const int* seqs) {
+  if (!ctx || n < 0 || (n > 0 && !seqs)) return ctx ? fail(ctx, L3P_E_INVAL, "bad argument") : L3P_E_INVAL;
+  return guarded(ctx, [&]() -> int {
+    if (int rc = check_seqs(ctx, n, seqs)) return rc;
+    if (n > 0) ctx->batch_valid = false;
+    for (int i = 0; i < n; ++i) {
+      auto& q = ctx->seqs[seqs[i]];
+      for (int p : q.pages) drop_page(ctx, p);
+      q.pages.clear();
+      q.len = 0;
+      q.live = false;
+    }
+    return L3P_OK;
+  });
+}
+
+L3P_API int l3p_paged_seq_length(l3p_paged_ctx* ctx, int seq, int* n_tokens) {
+  if (!ctx || !n_tokens) return ctx ? fail(ctx, L3P_E_INVAL, "null pointer") : L3P_E_INVAL;
+  if (int rc = check_seq(ctx, seq)) return rc;
+  *n_tokens = ctx->seqs[seq].len;
+  return L3P_OK;
+}
+
+L3P_API int l3p_paged_tables(l3p_paged_ctx* ctx, int n, const int* seqs, int width, int* table, int* need) {
+  if (!ctx || n < 0 || (n > 0 && !seqs) || width < 0) return ctx ? fail(ctx, L3P_E_INVAL, "bad argument") : L3P_E_INVAL;
+  int widest = 0;
+  for (int i = 0; i < n; ++i) {
+    if (int rc = check_seq(ctx, seqs[i])) return rc;
+    widest = std::max(widest, (int)ctx->seqs[seqs[i]].pages.size());
+  }
+  if (need) *need = widest;
+  if (!table) return L3P_OK;
+  if (width < widest) return fail(ctx, L3P_E_RANGE, "tables of %d pages, rows of %d", widest, width);
+  for (int i = 0; i < n; ++i) {
+    const auto& p = ctx->seqs[seqs[i]].pages;
+    int* row = table + (size_t)i * width;
+    std::copy(p.begin(), p.end(), row);
+    std::fill(row + p.size(), row + width, -1);
+  }
+  return L3P_OK;
+}
+
+L3P_API int l3p_paged_free_pages(l3p_paged_ctx* ctx, int* n_free) {
+  if (!ctx || !n_free) return ctx ? fail(ctx, L3P_E_INVAL, "null pointer") : L3P_E_INVAL;
+  *n_free = (int)ctx->free_heap.size();
+  return L3P_OK;
+}
+
+L3P_API int l3p_paged_compact(l3p_paged_ctx* ctx, int* n_used, void* stream) {
+  if (!ctx) return L3P_E_INVAL;
+  DeviceScope dev(ctx->cfg.device);
+  return guarded(ctx, [&] { return compact(ctx, n_used, as_stream(stream)); });
+}
+
+L3P_API int l3p_paged_begin(l3p_paged_ctx* ctx, int n_seqs, const int* seqs, const int* n_new, void* stream) {
+  if (!ctx || n_seqs < 0 || (n_seqs > 0 && (!seqs || !n_new)))
+    return ctx ? fail(ctx, L3P_E_INVAL, "bad argument") : L3P_E_INVAL;
+  DeviceScope dev(ctx->cfg.device);
+  return guarded(ctx, [&] { return begin(ctx, n_seqs, seqs, n_new, as_stream(stream)); });
+}

@@ -1,0 +1,202 @@
+// paged.h -- the paged cache's context and the batch description that its
+// kernels read (l3p_paged.cu, l3p_paged_kv.cu, l3p_paged_rows.cu,
+// l3p_paged_tc.cu, l3p_paged_f32.cu).  Private: not part of the C ABI.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+#include <string>
+#include <vector>
+
+#include "llama3pure_paged.h"
+
+#define L3P_API extern "C" __attribute__((visibility("default")))
+
+namespace l3p {
+
+// ---- the batch on the device: one block of 32-bit words ----------------------
+// [0, kPgHdrWords) header, then the arrays at the word offsets that the header
+// names.  Everything that depends on the batch is read from here, so that a
+// captured launch serves the batch that is current when it is replayed.
+constexpr int kPgMaxCtas = 160;   // CTAs of the row kernel at most
+constexpr int kPgTile = 16;       // keys of a warp tile of the row kernel
+
+// Lists of one kind of layer: [0] layers that attend to everything, [1] sliding-window layers.
+struct PgLists {
+  int row_ctas;    // CTAs of the row kernel that have segments (0: no sequence takes that path)
+  int row_first;   // word offset: int[row_ctas + 1], first segment of each
+  int row_segs;    // word offset: PgSeg[]
+  int n_tc;        // parts of the tensor-core kernels (0: none)
+  int tc_parts;    // word offset: PgPart[]
+  int n_prep;      // fp32 pools: key tiles to split
+  int prep;        // word offset: PgPrep[]
+  int pad;
+};
+struct PgHeader {
+  int n_tokens, n_seqs, row_nt, tok;  // tok: word offset of int2[n_tokens] (storage row, position)
+  int tbl;                            // word offset: the sequences' page tables, one after the other
+  int pad[3];
+  PgLists lists[2];
+};
+constexpr int kPgHdrWords = 32;
+static_assert(sizeof(PgHeader) <= kPgHdrWords * 4, "batch header");
+
+// Keys [tile0*16, tile1*16) of the rows r0 .. r0+n_rows-1 of one sequence and
+// KV head.  Row r is query head kvh*G + r % G of new token r / G.
+struct __align__(16) PgSeg {
+  int tbl;             // the sequence's table starts here (index into the tables)
+  int key_lo, key_hi;  // keys that any of the rows attends to
+  int tile0, tile1;
+  int q_row0, pos0;    // batch row and position of the sequence's first new token
+  int r0, n_rows, kvh;
+  int part, n_parts;   // split of the rows' key range; the merge's ticket and slots go by
+  int cta0;            //   the CTA that holds part 0
+  int pad[3];
+};
+static_assert(sizeof(PgSeg) == 64, "segment");
+
+// Key tiles [tile0, tile1) of 128 (64 for head_dim 256) keys for the rows
+// r0 .. r0+n_rows-1 on the tensor cores.
+struct __align__(16) PgPart {
+  int tbl, key_hi, tile0, tile1;
+  int q_row0, pos0, r0, n_rows;
+  int kvh, part, n_parts, ticket;
+  int slot, img, qbase, q_end;  // fp32: image tile of tile 0; position of the first query row, end of the chunk
+};
+static_assert(sizeof(PgPart) == 64, "part");
+
+struct PgPrep {
+  int tbl, key0, key_hi, img;  // keys [key0, key0+128) below key_hi, to image tile img
+};
+
+}  // namespace l3p
+
+struct l3p_paged_ctx {
+  l3p_paged_config cfg{};
+  int hd = 0, G = 1, es = 4, shift = 4;  // head size, heads per KV head, bytes of a value, log2(page_size)
+  bool bf16 = false, swa = false;
+  float scale = 1.f;
+  int num_sms = 148;
+  void* storage = nullptr;
+  size_t page_bytes = 0;       // one page: all layers, K and V, all heads
+  size_t block_bytes = 0;      // one head's rows of one layer's K or V in a page
+  int* batch = nullptr;        // device batch block
+  size_t batch_words = 0;
+  int* jobs = nullptr;         // device page-copy jobs (int4 each)
+  size_t jobs_cap = 0;
+  // pinned staging of uploads, used in turn; an event says when a slot's copy is done
+  static constexpr int kSlots = 4;
+  struct Slot {
+    int* host = nullptr;
+    size_t words = 0;
+    cudaEvent_t done = nullptr;
+    bool used = false;
+  } slots[kSlots];
+  unsigned slot_next = 0;
+
+  // books
+  struct Seq {
+    bool live = false;
+    int len = 0;
+    std::vector<int> pages;
+  };
+  std::vector<Seq> seqs;
+  std::vector<int> refs;       // holders of each page
+  std::vector<int> fill;       // rows of each page that any holder has used since it was given out
+  std::vector<int> free_heap;  // free pages, the lowest index on top
+
+  // current batch
+  bool batch_valid = false;
+  l3p::PgHeader hdr{};
+  int max_pos_in_batch = 0;  // one more than the highest position of a new token
+
+  // split workspace: partial rows, (m, l) pairs, tickets (0 between launches)
+  float* ws_o = nullptr;
+  float* ws_ml = nullptr;
+  unsigned* tickets = nullptr;
+  float* tc_o = nullptr;
+  float* tc_ml = nullptr;
+  unsigned* tc_tickets = nullptr;
+  // fp32 pools on the tensor cores: K/V tile images, flags of tiles with values that are not finite
+  float* img = nullptr;
+  size_t img_floats = 0;
+  int* v_flags = nullptr;
+  size_t v_flags_n = 0;
+  alignas(64) unsigned char tmap[128] = {};  // bf16 pools: the storage as rows of head_dim values (CUtensorMap)
+
+  float2* rope_tab = nullptr;      // (cos, sin) [max_pos][rotary_dim/2]
+  float2* rope_tab_swa = nullptr;  // sliding-window layers (the same array without them)
+  float* qk_norm = nullptr;        // [2][n_layers][hd]
+  int rope_max = 0, rope_layout = 0, rotary_dim = 0;
+  float rms_eps = 1e-5f;
+
+  int* err_host = nullptr;
+  int* err_dev = nullptr;
+  long long launches = 0;
+  std::string last_error;
+};
+
+namespace l3p_pg {
+
+inline int fail(l3p_paged_ctx* ctx, int code, const char* fmt, ...) {
+  if (ctx) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    ctx->last_error = buf;
+  }
+  return code;
+}
+
+#define PG_CUDA(ctx, call)                                                                                      \
+  do {                                                                                                          \
+    cudaError_t e_ = (call);                                                                                    \
+    if (e_ != cudaSuccess)                                                                                      \
+      return l3p_pg::fail((ctx), L3P_E_CUDA, "%s: %s (%s:%d)", #call, cudaGetErrorString(e_), __FILE__, __LINE__); \
+  } while (0)
+
+// Makes the context's device current for an entry point and restores the caller's.
+struct DeviceScope {
+  int prev = -1;
+  bool changed = false;
+  explicit DeviceScope(int dev) {
+    if (cudaGetDevice(&prev) == cudaSuccess && prev != dev) changed = cudaSetDevice(dev) == cudaSuccess;
+  }
+  ~DeviceScope() {
+    if (changed) cudaSetDevice(prev);
+  }
+};
+
+inline bool capturing(cudaStream_t s) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  return cudaStreamIsCapturing(s, &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
+}
+
+inline bool windowed(const l3p_paged_ctx* ctx, int layer) {
+  return ctx->swa && layer % ctx->cfg.swa_pattern < ctx->cfg.swa_pattern - 1;
+}
+
+// Rows per KV head up to which a sequence takes the row kernel, and the key
+// tile of the tensor-core kernel (l3p_paged_rows.cu, l3p_paged_tc.cu).
+int row_limit(const l3p_paged_ctx* ctx);
+int row_max_nt(const l3p_paged_ctx* ctx);  // blocks of 8 rows that one CTA takes at most
+int row_warps(const l3p_paged_ctx* ctx);
+int tc_tile(const l3p_paged_ctx* ctx);
+int tc_rows(const l3p_paged_ctx* ctx);  // rows of a part
+
+// Set-up of the kernels at create: shared-memory attributes, tensor map, workspaces.
+int init_rows(l3p_paged_ctx* ctx);
+int init_tc(l3p_paged_ctx* ctx);
+int init_f32(l3p_paged_ctx* ctx);
+
+int launch_rows(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void* out, long long os, cudaStream_t s);
+int launch_tc(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void* out, long long os, cudaStream_t s);
+int launch_f32(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void* out, long long os, cudaStream_t s);
+// Copies rows of pages: jobs (source page, destination page, rows, 0) in device memory.
+int launch_page_copy(l3p_paged_ctx* ctx, int n_jobs, cudaStream_t s);
+
+}  // namespace l3p_pg

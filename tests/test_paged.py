@@ -1,0 +1,64 @@
+"""The paged cache's C ABI without a GPU: bad configurations are refused
+before the device is touched, and null arguments are errors."""
+import ctypes as C
+
+import pytest
+
+from llama3pure_b200 import attn
+
+
+def _cfg(**kw):
+    base = dict(n_layers=2, n_heads=8, n_kv_heads=2, head_dim=128, page_size=16, n_pages=8, max_seqs=4, max_tokens=64,
+                max_seq_len=0, dtype=0, scale=0.0, is_gemma3=0, swa_window=0, swa_pattern=0, device=0)
+    base.update(kw)
+    return attn.PagedConfig(**base)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(n_heads=6, n_kv_heads=4), -1),
+    (dict(n_heads=0), -1),
+    (dict(n_layers=0), -1),
+    (dict(head_dim=96), -6),
+    (dict(page_size=24), -6),
+    (dict(page_size=256), -6),
+    (dict(n_pages=0), -1),
+    (dict(max_seqs=0), -1),
+    (dict(max_tokens=0), -1),
+    (dict(max_seq_len=-1), -1),
+    (dict(dtype=2), -1),
+    (dict(scale=float("nan")), -1),
+    (dict(swa_window=-1), -1),
+    (dict(device=-1), -1),
+    (dict(n_pages=2**30), -2),                                  # positions beyond 32 bits
+    (dict(n_pages=2**20, n_layers=2**10), -2),                  # rows of storage beyond 32 bits
+    (dict(max_tokens=2**30), -2),
+    (dict(max_seqs=2**20), -2),
+])
+def test_create_rejects_bad_config_without_device(lib, kw, code):
+    h = C.c_void_p()
+    assert lib.l3p_paged_create(C.byref(_cfg(**kw)), C.byref(h)) == code
+    assert not h.value
+
+
+def test_null_arguments_are_errors(lib):
+    n = C.c_int()
+    assert lib.l3p_paged_create(None, None) == -1
+    assert lib.l3p_paged_seq_new(None, C.byref(n)) == -1
+    assert lib.l3p_paged_seq_fork(None, 0, -1, 1, C.byref(n)) == -1
+    assert lib.l3p_paged_seq_copy(None, 0, None, None, None) == -1
+    assert lib.l3p_paged_seq_truncate(None, 0, 0) == -1
+    assert lib.l3p_paged_seq_free(None, 0, None) == -1
+    assert lib.l3p_paged_seq_length(None, 0, C.byref(n)) == -1
+    assert lib.l3p_paged_tables(None, 0, None, 0, None, None) == -1
+    assert lib.l3p_paged_free_pages(None, C.byref(n)) == -1
+    assert lib.l3p_paged_compact(None, C.byref(n), None) == -1
+    assert lib.l3p_paged_begin(None, 0, None, None, None) == -1
+    assert lib.l3p_paged_set_rope(None, None) == -1
+    assert lib.l3p_paged_rope_append_dev(None, 0, None, 0, None, 0, None, 0, None, 0, None) == -1
+    assert lib.l3p_paged_append_dev(None, 0, None, 0, None, 0, None) == -1
+    assert lib.l3p_paged_attn_dev(None, 0, None, 0, None, 0, None) == -1
+    assert lib.l3p_paged_check(None, None) == -1
+    assert lib.l3p_paged_storage(None, None, None) == -1
+    assert lib.l3p_paged_launch_count(None) == -1
+    assert lib.l3p_paged_last_error(None) == b""
+    lib.l3p_paged_destroy(None)

@@ -1,0 +1,650 @@
+"""The paged cache on the GPU against a plain implementation in 64 bits.
+
+Tolerances.  Scores of bf16 rows are sums of exact products in fp32; of fp32
+rows, three TF32 products leave at most 2^-20 of each product.  A score that is
+off by ds moves a softmax weight by a factor within 1 +- 2 ds, so an output by
+2 ds sum(p |v|).  With bf16 pages the weights are rounded once (2^-8) ahead of
+the second product and the output once (2^-8).  `ds` counts the accumulation too,
+2^-23 per term of head_dim terms at the sum's size (far above what it is), and
+2^-21 of the score for the scaling and the exponential.
+"""
+import math
+import random
+
+import numpy as np
+import pytest
+
+from llama3pure_b200.attn import AttnError
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+
+    return torch
+
+
+def _cache(**kw):
+    from llama3pure_b200.paged import PagedCache
+
+    base = dict(n_layers=2, n_heads=8, n_kv_heads=2, head_dim=128, page_size=16, n_pages=64, max_seqs=16, max_tokens=512)
+    base.update(kw)
+    return PagedCache(**base)
+
+
+def _type(torch, dtype):
+    return torch.bfloat16 if dtype == "bf16" else torch.float32
+
+
+def _want(torch, q, k, v, past, window=0, scale=None):
+    """Exact outputs of new tokens q [n][H][d] over k, v [past + n][Hkv][d], and their tolerance."""
+    n, H, d = q.shape
+    G = H // k.shape[1]
+    scale = 1 / math.sqrt(d) if scale is None else scale
+    out, tol = torch.empty(n, H, d, dtype=torch.float64, device=q.device), torch.empty(n, H, d, dtype=torch.float64, device=q.device)
+    t = torch.arange(past, past + n, device=q.device)[:, None]
+    j = torch.arange(k.shape[0], device=q.device)[None]
+    seen = (j <= t) & ((j > t - window) if window else True)
+    bf16 = q.dtype == torch.bfloat16
+    for h in range(H):
+        kh, vh, qh = k[:, h // G].double(), v[:, h // G].double(), q[:, h].double()
+        s = (qh @ kh.T * scale).masked_fill(~seen, -math.inf)
+        p = torch.softmax(s, -1)
+        out[:, h] = p @ vh
+        size = (qh.abs() @ kh.abs().T * abs(scale)).masked_fill(~seen, 0).amax(-1, keepdim=True)
+        ds = size * ((0 if bf16 else 2**-20) + d * 2**-23 + 2**-21)
+        pv = p @ vh.abs()
+        tol[:, h] = 2 * ds * pv + 2**-22 * pv
+        if bf16:
+            tol[:, h] += 2**-8 * pv + 2**-8 * out[:, h].abs()
+    return out, tol
+
+
+def _near(got, want, tol, what=""):
+    err = (got.double() - want).abs()
+    assert bool((err <= tol + 1e-30).all()), f"{what}: {float((err / (tol + 1e-30)).max()):.3g} times the tolerance"
+
+
+class Books:
+    """What the cache should hold: every sequence's rows as lists of tensors, one per layer."""
+
+    def __init__(self, torch, cache, seed=0):
+        self.torch, self.c, self.rows = torch, cache, {}
+        self.g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def randn(self, *shape):
+        return self.torch.randn(*shape, generator=self.g, device="cuda").to(self.c.dtype)
+
+    def new(self):
+        s = self.c.new_seq()
+        self.rows[s] = [self.randn(0, 2, self.c.n_kv_heads, self.c.head_dim) for _ in range(self.c.n_layers)]
+        return s
+
+    def step(self, seqs, n_new, attend=True, window=lambda layer: 0, scale=None, stream=None):
+        """One step over all layers: q, k, v lie in one tensor, as a projection leaves them."""
+        torch, c = self.torch, self.c
+        c.begin(seqs, n_new, stream)
+        n, H, K, d = sum(n_new), c.n_heads, c.n_kv_heads, c.head_dim
+        for layer in range(c.n_layers):
+            qkv = self.randn(n, H + 2 * K, d)
+            q, k, v = qkv[:, :H], qkv[:, H:H + K], qkv[:, H + K:]
+            out = torch.full((n + 3, H, d), 7.0, device="cuda", dtype=c.dtype)
+            if stream is not None:
+                torch.cuda.synchronize()
+            c.append_dev(layer, k, v, stream)
+            if attend:
+                c.attn_dev(layer, q, out, stream)
+            c.check(stream)
+            assert bool((out[n:] == 7.0).all()), "rows behind the last token"
+            at = 0
+            for s, m in zip(seqs, n_new):
+                old = self.rows[s][layer]
+                new = torch.stack([k[at:at + m], v[at:at + m]], 1)
+                self.rows[s][layer] = torch.cat([old, new])
+                if attend and m:
+                    kv = self.rows[s][layer]
+                    want, tol = _want(torch, q[at:at + m], kv[:, 0], kv[:, 1], len(old), window(layer), scale)
+                    _near(out[at:at + m], want, tol, f"sequence {s}, {m} tokens on {len(old)}, layer {layer}")
+                at += m
+
+    def verify(self):
+        """Lengths, tables and every row of every sequence."""
+        c, st, seen = self.c, self.c.storage(), set()
+        for s, rows in self.rows.items():
+            n = len(rows[0])
+            assert c.length(s) == n
+            table = c.tables([s])[0]
+            assert len(table) == -(-n // c.cfg.page_size) and len(set(table.tolist())) == len(table)
+            seen |= set(table.tolist())
+            if n:
+                idx = self.torch.from_numpy(table).cuda().long()
+                for layer in range(c.n_layers):
+                    got = st[idx, layer].permute(0, 3, 1, 2, 4).reshape(-1, 2, c.n_kv_heads, c.head_dim)[:n]
+                    assert bool((got == rows[layer]).all()), f"rows of sequence {s}"
+        assert c.free_pages() == c.cfg.n_pages - len(seen)
+
+
+SHAPES = [  # heads, KV heads, head_dim
+    (32, 8, 64), (4, 4, 64), (8, 2, 128), (6, 2, 128), (5, 1, 128), (8, 8, 128), (16, 2, 128), (8, 1, 256), (6, 3, 256),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim", SHAPES)
+def test_single_tokens_ragged(torch, dtype, heads, kv, dim):
+    """Lengths around tile and page ends, single tokens of every sequence and of some."""
+    with _cache(n_heads=heads, n_kv_heads=kv, head_dim=dim, dtype=dtype, n_pages=160, n_layers=1) as c:
+        b = Books(torch, c, heads)
+        lengths = [0, 1, 14, 15, 16, 17, 31, 32, 100, 255, 256, 300]
+        seqs = [b.new() for _ in lengths]
+        for at in range(0, 300, 150):
+            new = [max(0, min(n - at, 150)) for n in lengths]
+            for i in range(0, len(seqs), 3):
+                b.step(seqs[i:i + 3], new[i:i + 3], attend=False)
+        b.step(seqs, [1] * len(seqs))
+        b.step(seqs[::2], [1] * len(seqs[::2]))
+        b.step(seqs, [i % 2 for i in range(len(seqs))])
+        b.verify()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim", SHAPES)
+@pytest.mark.parametrize("page", [16, 128])
+def test_chunks(torch, dtype, heads, kv, dim, page):
+    """Chunks of every path: a few tokens, whole tiles, ragged ones, beside single tokens and none."""
+    with _cache(n_heads=heads, n_kv_heads=kv, head_dim=dim, dtype=dtype, page_size=page, n_pages=2048 // page, n_layers=1,
+                max_tokens=1024) as c:
+        b = Books(torch, c, dim + page)
+        seqs = [b.new() for _ in range(5)]
+        b.step(seqs, [3, 0, 129, 1, 40])
+        b.step(seqs, [257, 1, 2, 5, 0])
+        b.step(seqs, [1, 8, 130, 64, 300])
+        b.step(seqs[::-1], [7, 1, 1, 33, 63])
+        b.verify()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("window", [1, 16, 50, 1000])
+def test_sliding_window_layers(torch, dtype, dim, window):
+    """Layers 0 and 1 of pattern 3 look back `window` positions, layer 2 sees everything."""
+    with _cache(n_heads=4, n_kv_heads=1, head_dim=dim, dtype=dtype, n_layers=3, is_gemma3=1, swa_window=window, swa_pattern=3,
+                n_pages=200, max_tokens=600) as c:
+        b = Books(torch, c, window)
+        seqs = [b.new() for _ in range(3)]
+        win = lambda layer: window if layer % 3 < 2 else 0  # noqa: E731
+        b.step(seqs, [390, 17, 0], window=win)
+        b.step(seqs, [1, 1, 1], window=win)
+        b.step(seqs, [150, 5, 260], window=win)
+        b.step(seqs, [1, 4, 1], window=win)
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim,lengths", [
+    ("f32", 32, 8, 128, [9000, 3]), ("bf16", 32, 8, 128, [20000]), ("bf16", 8, 1, 64, [33000]), ("f32", 8, 1, 256, [5000, 1]),
+    ("bf16", 8, 1, 256, [7000]), ("bf16", 16, 8, 128, [40, 6000, 1, 2500, 777]),
+])
+def test_long_sequences_are_split_and_joined(torch, dtype, heads, kv, dim, lengths):
+    with _cache(n_heads=heads, n_kv_heads=kv, head_dim=dim, dtype=dtype, n_layers=1, n_pages=sum(lengths) // 64 + 20, page_size=64,
+                max_tokens=max(lengths)) as c:
+        b = Books(torch, c, dim)
+        seqs = []
+        for n in lengths:
+            seqs.append(b.new())
+            b.step(seqs[-1:], [n], attend=False)
+        b.step(seqs, [1] * len(seqs))
+        b.step(seqs, [3] * len(seqs))
+        b.step(seqs[:1], [70])
+        for _ in range(3):  # tickets return to zero
+            b.step(seqs, [1] * len(seqs))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_scale(torch, dtype):
+    with _cache(dtype=dtype, scale=0.3, n_layers=1) as c:
+        b = Books(torch, c)
+        s = b.new()
+        b.step([s], [60], scale=0.3)
+        b.step([s], [1], scale=0.3)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_values_that_are_not_attended_never_matter(torch, dtype, dim, bad):
+    """Pages full of `bad` behind and before the rows in use, and `bad` in K and V of later tokens of a chunk."""
+    with _cache(n_heads=4, n_kv_heads=1, head_dim=dim, dtype=dtype, n_layers=2, is_gemma3=1, swa_window=40, swa_pattern=2, n_pages=64,
+                max_tokens=700) as c:
+        c.storage().fill_(bad)
+        b = Books(torch, c)
+        seqs = [b.new(), b.new()]
+        win = lambda layer: 40 if layer == 0 else 0  # noqa: E731
+        b.step(seqs, [201, 3], window=win)
+        b.step(seqs, [1, 1], window=win)
+        b.step(seqs, [4, 1], window=win)
+        # the last three of 160 and of 5 new tokens are bad: the rows before them do not see it
+        for n in (160, 5):
+            past = len(b.rows[seqs[0]][1])
+            c.begin(seqs[:1], [n])
+            q, k, v = b.randn(n, 4, dim), b.randn(n, 1, dim), b.randn(n, 1, dim)
+            k[-3:] = bad
+            v[-3:, :, 5:9] = bad
+            for layer in (0, 1):
+                out = torch.empty_like(q)
+                c.append_dev(layer, k, v)
+                c.attn_dev(layer, q, out)
+                c.check()
+                rows = torch.cat([b.rows[seqs[0]][layer], torch.stack([k, v], 1)])[:past + n - 3]
+                want, tol = _want(torch, q[:-3], rows[:, 0], rows[:, 1], past, win(layer))
+                _near(out[:-3], want, tol, f"{n} tokens, layer {layer}")
+            c.truncate(seqs[0], past)
+        # V alone: rows that attend to it have it in its columns and nowhere else
+        for n in (160, 5):
+            past = len(b.rows[seqs[0]][1])
+            c.begin(seqs[:1], [n])
+            q, k, v = b.randn(n, 4, dim), b.randn(n, 1, dim), b.randn(n, 1, dim)
+            v[-3, :, 5:9] = bad
+            c.append_dev(1, k, v)
+            out = torch.empty_like(q)
+            c.attn_dev(1, q, out)
+            c.check()
+            rows = torch.cat([b.rows[seqs[0]][1], torch.stack([k, v], 1)])
+            clean = rows.clone()
+            clean[-3, 1, :, 5:9] = 0
+            want, tol = _want(torch, q, clean[:, 0], clean[:, 1], past)
+            assert bool(out[-3:, :, 5:9].float().isfinite().logical_not().all())
+            keep = torch.ones(n, 1, dim, dtype=torch.bool, device="cuda").expand(n, 4, dim).clone()
+            keep[-3:, :, 5:9] = False
+            _near(out[keep], want[keep], tol[keep], f"columns beside, {n} tokens")
+            c.truncate(seqs[0], past)
+
+
+def test_empty_batches(torch):
+    with _cache(n_layers=1) as c:
+        b = Books(torch, c)
+        c.begin([], [])
+        e = torch.empty(0, 8, 128, device="cuda")
+        kv = torch.empty(0, 2, 128, device="cuda")
+        n0 = c.launch_count()
+        c.append_dev(0, kv, kv)
+        c.attn_dev(0, e, e)
+        s = b.new()
+        b.step([s], [0])
+        assert c.launch_count() == n0
+        b.step([s], [1])
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_pages_under_random_use(torch, seed):
+    """Forks, copies, cuts, frees, compaction and steps in any order: every sequence keeps its rows."""
+    rng = random.Random(seed)
+    dtype = rng.choice(["f32", "bf16"])
+    with _cache(n_heads=4, n_kv_heads=2, head_dim=64, n_pages=90, max_seqs=12, max_tokens=200, dtype=dtype, page_size=rng.choice([16, 32])) as c:
+        b = Books(torch, c, seed)
+        for i in range(60):
+            live = sorted(b.rows)
+            do = rng.choice(["new", "fork", "copy", "cut", "free", "compact", "step", "step", "step"])
+            try:
+                if do == "new" or not live:
+                    b.new()
+                elif do == "fork":
+                    s = rng.choice(live)
+                    n = rng.choice([-1, rng.randint(0, c.length(s))])
+                    for ch in c.fork(s, rng.randint(1, 3), n):
+                        b.rows[ch] = [r[:len(r) if n < 0 else n] for r in b.rows[s]]
+                elif do == "copy":
+                    some = rng.sample(live, rng.randint(1, len(live)))
+                    for s, ch in zip(some, c.copy(some)):
+                        b.rows[ch] = list(b.rows[s])
+                elif do == "cut":
+                    s = rng.choice(live)
+                    n = rng.randint(0, c.length(s))
+                    c.truncate(s, n)
+                    b.rows[s] = [r[:n] for r in b.rows[s]]
+                elif do == "free":
+                    gone = rng.sample(live, rng.randint(1, max(1, len(live) // 2)))
+                    c.free(gone)
+                    for s in gone:
+                        del b.rows[s]
+                elif do == "compact":
+                    used = c.compact()
+                    assert used == c.cfg.n_pages - c.free_pages()
+                    if b.rows:
+                        assert int(c.tables(sorted(b.rows)).max(initial=-1)) < used
+                else:
+                    some = rng.sample(live, rng.randint(1, len(live)))
+                    b.step(some, [rng.choice([0, 1, 1, 5, 30]) for _ in some], attend=i % 2 == 0)
+            except AttnError as e:
+                assert e.code == -4  # the pool or the sequence ids are used up: nothing has changed
+            b.verify()
+
+
+def test_last_holder_of_a_shared_page_keeps_it(torch):
+    with _cache(n_layers=1, n_pages=20) as c:
+        b = Books(torch, c)
+        s = b.new()
+        b.step([s], [20], attend=False)
+        children = c.fork(s, 2)
+        for ch in children:
+            b.rows[ch] = list(b.rows[s])
+        t = c.tables([s])[0].tolist()
+        b.step([s] + children, [1, 2, 1])
+        tables = c.tables([s] + children)
+        assert tables[:, 0].tolist() == [t[0]] * 3
+        assert sorted(tables[:, 1].tolist()) == [t[1], 2, 3] and tables[2, 1] == t[1]
+        b.verify()
+
+
+ROPES = [
+    dict(layout="interleaved"), dict(layout="half"), dict(layout="half", rotary=32), dict(layout="interleaved", rotary=20),
+    dict(layout="half", rotary=6, norm=True), dict(layout="interleaved", scaling="linear", factor=4.0), dict(layout="half", scaling="bands", factor=8.0, norm=True),
+    dict(layout="half", scaling="yarn", factor=16.0, rotary=64), dict(layout="interleaved", scaling="yarn", factor=4.0, attn=1.25),
+]
+
+
+def _turned(torch, x, pos, dim, layout, rotary, scaling, factor, attn, theta, original, w=None):
+    """Exact rotation of rows x [n][heads][dim]."""
+    x = x.double()
+    if w is not None:
+        x = x / torch.sqrt(x.pow(2).mean(-1, keepdim=True) + 1e-5) * w.double()
+    r = rotary or dim
+    f, mult = [theta ** (-2 * i / r) for i in range(r // 2)], 1.0
+    if scaling == "linear":
+        f = [v / factor for v in f]
+    elif scaling == "bands":
+        g = []
+        for v in f:
+            wave = 2 * math.pi / v
+            if wave < original / 4.0:
+                g.append(v)
+            elif wave > original / 1.0:
+                g.append(v / factor)
+            else:
+                mix = (original / wave - 1.0) / 3.0
+                g.append((1 - mix) * v / factor + mix * v)
+        f = g
+    elif scaling == "yarn":
+        at = lambda n: r * math.log(original / (n * 2 * math.pi)) / (2 * math.log(theta))  # noqa: E731
+        lo, hi = max(math.floor(at(32)), 0), min(math.ceil(at(1)), r - 1)
+        ramp = [min(1.0, max(0.0, (i - lo) / ((hi - lo) or 0.001))) for i in range(r // 2)]
+        f = [v * (1 - m) + v / factor * m for v, m in zip(f, ramp)]
+        mult = attn or 0.1 * math.log(factor) + 1
+    ang = pos[:, None].double() * torch.tensor(f, dtype=torch.float64, device=x.device)
+    c, s = torch.cos(ang)[:, None] * mult, torch.sin(ang)[:, None] * mult
+    y = x.clone()
+    if layout == "half":
+        a, b = x[..., :r // 2], x[..., r // 2:r]
+        y[..., :r // 2], y[..., r // 2:r] = a * c - b * s, a * s + b * c
+    else:
+        a, b = x[..., 0:r:2], x[..., 1:r:2]
+        y[..., 0:r:2], y[..., 1:r:2] = a * c - b * s, a * s + b * c
+    return y
+
+
+def _rope_near(torch, got, want, dtype, what):
+    # fp32: cosine and sine rounded (2^-24 each), two products and a sum, and with a norm a mean over the row, a square root, a
+    # division and two products: within 2^-20 of a pair's size, which the row's largest value bounds.  bf16: and one rounding, 2^-8.
+    size = want.abs().amax(-1, keepdim=True) * 2
+    tol = size * 2**-20 + (want.abs() * 2**-8 if dtype == "bf16" else 0)
+    _near(got, want, tol, what)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("kw", ROPES, ids=lambda k: "-".join(str(v) for v in k.values()))
+def test_rotary_and_append(torch, dtype, dim, kw):
+    kw = dict(rotary=0, scaling="none", factor=1.0, attn=0.0, norm=False) | kw
+    original = 512
+    with _cache(n_heads=6, n_kv_heads=2, head_dim=dim, dtype=dtype, n_layers=2, n_pages=400, max_tokens=3000) as c:
+        b = Books(torch, c, dim)
+        rng = np.random.default_rng(5)
+        wq, wk = (1 + 0.1 * rng.standard_normal((2, dim))).astype(np.float32), (1 + 0.1 * rng.standard_normal((2, dim))).astype(np.float32)
+        norm = dict(q_norm=wq, k_norm=wk) if kw["norm"] else {}
+        c.set_rope(max_pos=4000, layout=kw["layout"], rotary_dim=kw["rotary"], scaling=kw["scaling"], factor=kw["factor"], theta=10000.0,
+                   original_len=original, attn_factor=kw["attn"], **norm)
+        seqs = [b.new() for _ in range(3)]
+        c.begin(seqs, [2900, 0, 17])
+        for new in ([5, 1, 0], [1, 1, 1], [700, 100, 30]):
+            past = [c.length(s) for s in seqs]
+            c.begin(seqs, new)
+            n = sum(new)
+            pos = torch.cat([torch.arange(p, p + m, device="cuda") for p, m in zip(past, new)])
+            for layer in (0, 1):
+                qkv = b.randn(n, 10, dim)
+                q, k, v = qkv[:, :6], qkv[:, 6:8], qkv[:, 8:]
+                args = (pos, dim, kw["layout"], kw["rotary"], kw["scaling"], kw["factor"], kw["attn"], 10000.0, original)
+                w = [torch.from_numpy(x[layer]).cuda() if kw["norm"] else None for x in (wq, wk)]
+                want_q, want_k = _turned(torch, q, *args, w=w[0]), _turned(torch, k, *args, w=w[1])
+                want_v = v.clone()
+                out = torch.empty(n, 6, dim, device="cuda", dtype=c.dtype)
+                c.rope_append_dev(layer, q, k, v, out)
+                c.check()
+                _rope_near(torch, out, want_q, dtype, "q")
+                c.rope_append_dev(layer, q, k, v, q)  # in place
+                c.check()
+                assert bool((q == out).all())
+                st, at = c.storage(), 0
+                for s, p, m in zip(seqs, past, new):
+                    if m:
+                        t = torch.from_numpy(c.tables([s])[0]).cuda().long()
+                        rows = st[t, layer].permute(0, 3, 1, 2, 4).reshape(-1, 2, 2, dim)[p:p + m]
+                        _rope_near(torch, rows[:, 0], want_k[at:at + m], dtype, "k")
+                        assert bool((rows[:, 1] == want_v[at:at + m]).all())
+                    at += m
+
+
+def test_rotary_far_positions_and_window_layers(torch):
+    """Angles of far positions keep their precision; sliding-window layers use their own, unscaled table."""
+    with _cache(n_heads=4, n_kv_heads=1, head_dim=64, n_layers=2, is_gemma3=1, swa_window=8, swa_pattern=2, page_size=128, n_pages=4100,
+                max_tokens=600000) as c:
+        b = Books(torch, c)
+        c.set_rope(max_pos=524288, layout="half", scaling="linear", factor=8.0, theta=1e6, theta_swa=1e4)
+        s = b.new()
+        c.begin([s], [524280])
+        c.begin([s], [8])
+        pos = torch.arange(524280, 524288, device="cuda")
+        for layer in (0, 1):
+            q, k, v = b.randn(8, 4, 64), b.randn(8, 1, 64), b.randn(8, 1, 64)
+            out = torch.empty_like(q)
+            c.rope_append_dev(layer, q, k, v, out)
+            c.check()
+            args = ("none", 1.0, 0.0, 1e4) if layer == 0 else ("linear", 8.0, 0.0, 1e6)
+            _rope_near(torch, out, _turned(torch, q, pos, 64, "half", 0, *args, 0), "f32", f"layer {layer}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_serving_loop_on_another_stream(torch, dtype):
+    """Prompts in chunks beside decoding sequences, forks of a prompt, frees and compaction, on a stream of the caller's: every
+    output equals attention over the whole rotated history."""
+    heads, kv, dim = 8, 2, 128
+    s = torch.cuda.Stream()
+    with _cache(n_heads=heads, n_kv_heads=kv, head_dim=dim, dtype=dtype, n_layers=2, n_pages=80, max_tokens=256) as c, torch.cuda.stream(s):
+        c.set_rope(max_pos=1000, layout="interleaved", scaling="bands", factor=8.0, original_len=256)
+        g = torch.Generator(device="cuda").manual_seed(1)
+        hist = {}
+
+        def step(seqs, new):
+            c.begin(seqs, new)
+            n = sum(new)
+            for layer in range(2):
+                qkv = torch.randn(n, heads + 2 * kv, dim, generator=g, device="cuda").to(c.dtype)
+                q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv], qkv[:, heads + kv:]
+                qr, out = torch.empty(n, heads, dim, device="cuda", dtype=c.dtype), torch.empty(n, heads, dim, device="cuda", dtype=c.dtype)
+                c.rope_append_dev(layer, q, k, v, qr)
+                c.attn_dev(layer, qr, out)
+                c.check()
+                at = 0
+                for x, m in zip(seqs, new):
+                    past = len(hist[x][layer])
+                    pos = torch.arange(past, past + m, device="cuda")
+                    kr = _turned(torch, k[at:at + m], pos, dim, "interleaved", 0, "bands", 8.0, 0.0, 500000.0, 256)
+                    # the rounded row that the page holds: the table's cosines are the oracle's within 2^-24, so take the page's own
+                    t = torch.from_numpy(c.tables([x])[0]).cuda().long()
+                    row = c.storage()[t, layer].permute(0, 3, 1, 2, 4).reshape(-1, 2, kv, dim)[past:past + m]
+                    _rope_near(torch, row[:, 0], kr, dtype, "k")
+                    hist[x][layer] = torch.cat([hist[x][layer], row.clone()])
+                    if m:
+                        h = hist[x][layer]
+                        want, tol = _want(torch, qr[at:at + m], h[:, 0], h[:, 1], past)
+                        _near(out[at:at + m], want, tol, f"sequence {x}")
+                    at += m
+
+        def new():
+            x = c.new_seq()
+            hist[x] = [torch.empty(0, 2, kv, dim, device="cuda", dtype=c.dtype) for _ in range(2)]
+            return x
+
+        a, b = new(), new()
+        step([a, b], [100, 7])
+        step([a, b], [1, 90])
+        kids = c.fork(a, 3)
+        for x in kids:
+            hist[x] = list(hist[a])
+        step([a, b] + kids, [1, 1, 1, 1, 4])
+        step([b] + kids, [130, 1, 1, 1])
+        c.free([a, kids[0]])
+        c.compact()
+        step([b] + kids[1:], [1, 60, 1])
+        d = c.copy([b])[0]
+        hist[d] = list(hist[b])
+        c.truncate(b, 50)
+        hist[b] = [x[:50] for x in hist[b]]
+        step([b, d], [20, 1])
+
+
+def test_captured_step_serves_later_batches(torch):
+    """One graph of a decoding step, replayed on other sequences and lengths; a batch that it cannot serve is reported."""
+    with _cache(n_heads=8, n_kv_heads=2, head_dim=64, dtype="bf16", n_layers=2, n_pages=600, max_tokens=4096, page_size=16) as c:
+        b = Books(torch, c)
+        c.set_rope(max_pos=6000, layout="half")
+        seqs = [b.new() for _ in range(6)]
+        for x, n in zip(seqs, [5, 900, 17, 64, 333, 2000]):
+            c.begin([x], [n])
+            for layer in range(2):
+                k, v = b.randn(n, 2, 64), b.randn(n, 2, 64)
+                c.append_dev(layer, k, v)
+        c.begin(seqs, [1] * 6)
+        q, k, v = b.randn(6, 8, 64), b.randn(6, 2, 64), b.randn(6, 2, 64)
+        qr, outs = torch.empty_like(q), [torch.empty_like(q) for _ in range(2)]
+
+        def layers():
+            for layer in range(2):
+                c.rope_append_dev(layer, q, k, v, qr)
+                c.attn_dev(layer, qr, outs[layer])
+
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            layers()
+            c.check()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                layers()
+            for some in (seqs, seqs[:2], seqs[::-1], seqs[5:], seqs[1:5]):
+                c.begin(some, [1] * len(some))
+                for t in (q, k, v):
+                    t.copy_(b.randn(*t.shape))
+                layers()
+                want = [o.clone() for o in outs]
+                for o in outs:
+                    o.fill_(3.0)
+                graph.replay()
+                c.check()
+                for o, w in zip(outs, want):
+                    assert bool((o[:len(some)] == w[:len(some)]).all())
+                    assert bool((o[len(some):] == 3.0).all())
+            for some, new in ((seqs, [2, 1, 1, 1, 1, 1]), (seqs[:1], [200]), (seqs[:2], [4, 1])):
+                c.begin(some, new)
+                graph.replay()
+                with pytest.raises(AttnError) as e:
+                    c.check()
+                assert e.value.code == -1
+            c.begin(seqs, [1] * 6)
+            graph.replay()
+            c.check()
+            del graph
+
+
+def test_calls_during_capture_are_refused(torch):
+    with _cache(n_layers=1) as c:
+        b = Books(torch, c)
+        s = b.new()
+        b.step([s], [20], attend=False)
+        stream = torch.cuda.Stream()
+        graph = torch.cuda.CUDAGraph()
+        codes = []
+        with torch.cuda.graph(graph, stream=stream):
+            for call in (lambda: c.begin([s], [1]), lambda: c.copy([s]), lambda: c.compact()):
+                with pytest.raises(AttnError) as e:
+                    call()
+                codes.append(e.value.code)
+            torch.zeros(4, device="cuda")
+        assert codes == [-1] * 3
+        b.verify()
+        b.step([s], [1])
+
+
+def test_refusals_change_nothing(torch):
+    with _cache(n_layers=1, n_pages=4, max_seqs=3, max_tokens=60, max_seq_len=50) as c:
+        b = Books(torch, c)
+        s, t = b.new(), b.new()
+        q, kv = b.randn(8, 8, 128), b.randn(8, 2, 128)
+
+        def code(f, *a, **k):
+            with pytest.raises(AttnError) as e:
+                f(*a, **k)
+            return e.value.code
+
+        assert code(c.attn_dev, 0, q, q) == -1  # no batch yet
+        assert code(c.append_dev, 0, kv, kv) == -1
+        assert code(c.begin, [s, s], [1, 1]) == -1
+        assert code(c.begin, [s, 2], [1, 1]) == -2
+        assert code(c.begin, [-1], [1]) == -2
+        assert code(c.begin, [s], [-1]) == -1
+        assert code(c.begin, [s], [51]) == -2       # max_seq_len
+        assert code(c.begin, [s, t], [40, 21]) == -2  # max_tokens
+        assert code(c.begin, [s, t], [33, 17]) == -4  # 3 + 2 pages of 4
+        assert code(c.truncate, s, 1) == -2
+        assert code(c.truncate, 2, 0) == -2
+        assert code(c.fork, s, 1, 1) == -2
+        assert code(c.fork, s, 2) == -4             # sequence ids
+        assert code(c.free, [s, s]) == -1
+        assert code(c.free, [7]) == -2
+        assert code(c.copy, [s, s]) == -4
+        assert code(c.copy, [2]) == -2
+        assert code(c.length, 2) == -2
+        b.verify()
+        b.step([s], [8], attend=False)
+        assert code(c.append_dev, 1, kv, kv) == -2
+        assert code(c.attn_dev, -1, q, q) == -2
+        assert code(c.rope_append_dev, 0, q, kv, kv, q) == -1  # no tables
+        for bad in (dict(max_pos=0), dict(max_pos=9, rotary_dim=3), dict(max_pos=9, rotary_dim=130), dict(max_pos=9, theta=0.5),
+                    dict(max_pos=9, scaling="linear", factor=0.5), dict(max_pos=9, scaling="bands", factor=2.0),
+                    dict(max_pos=9, scaling="yarn", factor=2.0), dict(max_pos=9, scaling="bands", factor=2.0, original_len=9, low_freq=4.0, high_freq=2.0),
+                    dict(max_pos=9, scaling="yarn", factor=float("nan"), original_len=9), dict(max_pos=9, q_norm=np.ones((1, 128), np.float32))):
+            assert code(c.set_rope, **bad) == -1
+        c.set_rope(max_pos=7)
+        assert code(c.rope_append_dev, 0, q, kv, kv, q) == -2  # position 7
+        lib, h = c.lib, c.h
+        p = q.data_ptr()
+        assert lib.l3p_paged_attn_dev(h, 0, p, 0, None, 0, None) == -1
+        assert lib.l3p_paged_attn_dev(h, 0, p + 4, 0, p, 0, None) == -1      # alignment
+        assert lib.l3p_paged_attn_dev(h, 0, p, 8 * 128 - 4, p, 0, None) == -1  # a stride below the row
+        assert lib.l3p_paged_attn_dev(h, 0, p, 8 * 128 + 2, p, 0, None) == -1  # a stride off 16 bytes
+        assert lib.l3p_paged_tables(h, 1, (np.array([s], np.int32)).ctypes.data, 0, np.zeros(1, np.int32).ctypes.data, None) == -2
+        for bad in (q.half(), q.cpu(), q[:7], q[:, :4], q.transpose(0, 1), q[:1].expand(8, 8, 128)):
+            with pytest.raises((TypeError, ValueError)):
+                c.attn_dev(0, bad, q)
+        with pytest.raises(ValueError):
+            c.begin([s], [1, 1])
+        b.verify()
+        c.truncate(s, 8)
+        assert code(c.attn_dev, 0, q, q) == -1  # the batch has ended
+        b.step([s], [1])
+
+
+def test_create_without_memory(torch):
+    with pytest.raises(AttnError) as e:
+        _cache(n_layers=64, n_heads=8, n_kv_heads=8, head_dim=256, page_size=128, n_pages=16000)  # 537 GB
+    assert e.value.code == -4
+    assert torch.zeros(4, device="cuda").sum().item() == 0
