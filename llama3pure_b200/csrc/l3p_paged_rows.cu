@@ -12,6 +12,7 @@ namespace l3p_pg {
 // Sequences with more query rows per KV head take the tensor-core kernels.
 // fp32 with head_dim 256 has none: Q and O alone would fill tensor memory.
 int row_limit(const l3p_paged_ctx* ctx) {
+  if (ctx->bf16) return ctx->hd == 256 ? 16 : 32;
   return INT_MAX;
 }
 

@@ -25,7 +25,11 @@
 // registers with ldmatrix and nothing waits for tensor memory.
 //   bf16: m16n8k16, fp32 accumulators; P is rounded to bf16 for the second
 //         product (at most 2^-8 of each weight), l sums the unrounded P.
-//   fp32: 3xTF32 m16n8k8 (x = hi + lo; hi*hi + hi*lo + lo*hi), ~2^-21 of a product.
+//   fp32: 3xTF32 m16n8k8 (x = hi + lo; hi*hi + hi*lo + lo*hi).  The matrix
+//         instruction cuts its sums off instead of rounding them, a bias that
+//         grows with every instruction in a chain (1.4e-5 of the output at
+//         128K keys), so at most six instructions share an accumulator and
+//         what they leave is added to the running fp32 sums by ordinary adds.
 #pragma once
 #include <cuda_bf16.h>
 
@@ -96,9 +100,11 @@ __device__ __forceinline__ void pg_mma_tf32(float (&c)[4], const uint32_t (&a)[4
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo: hi has tf32's 11 significant bits, lo = x - hi is exact in fp32.
+// x = hi + lo: hi is x rounded to tf32's 11 significant bits, lo = x - hi is
+// exact in fp32.  Rounding hi to nearest leaves lo 12 bits of either sign, so
+// the bit that tf32 drops of it has no bias.
 __device__ __forceinline__ void pg_split(float x, uint32_t& hi, uint32_t& lo) {
-  hi = __float_as_uint(x) & 0xFFFFE000u;
+  hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
   lo = __float_as_uint(x - __uint_as_float(hi));
 }
 __device__ __forceinline__ uint32_t pg_pack_bf16(float lo, float hi) {
@@ -279,11 +285,13 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
           pg_split(y.x, hi[1], lo[1]);
           pg_split(x.y, hi[2], lo[2]);
           pg_split(y.y, hi[3], lo[3]);
+          float c0[NT][4], c1[NT][4];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            pg_mma_tf32(sc[n], lo, qa[n][k][0], qa[n][k][1]);
-            pg_mma_tf32(sc[n], hi, qb[n][k][0], qb[n][k][1]);
-            pg_mma_tf32(sc[n], hi, qa[n][k][0], qa[n][k][1]);
+            c0[n][0] = c0[n][1] = c0[n][2] = c0[n][3] = 0.f;
+            pg_mma_tf32(c0[n], lo, qa[n][k][0], qa[n][k][1]);
+            pg_mma_tf32(c0[n], hi, qb[n][k][0], qb[n][k][1]);
+            pg_mma_tf32(c0[n], hi, qa[n][k][0], qa[n][k][1]);
           }
           pg_split(x.z, hi[0], lo[0]);
           pg_split(y.z, hi[1], lo[1]);
@@ -291,9 +299,15 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
           pg_split(y.w, hi[3], lo[3]);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            pg_mma_tf32(sd[n], lo, qa[n][k][2], qa[n][k][3]);
-            pg_mma_tf32(sd[n], hi, qb[n][k][2], qb[n][k][3]);
-            pg_mma_tf32(sd[n], hi, qa[n][k][2], qa[n][k][3]);
+            c1[n][0] = c1[n][1] = c1[n][2] = c1[n][3] = 0.f;
+            pg_mma_tf32(c1[n], lo, qa[n][k][2], qa[n][k][3]);
+            pg_mma_tf32(c1[n], hi, qb[n][k][2], qb[n][k][3]);
+            pg_mma_tf32(c1[n], hi, qa[n][k][2], qa[n][k][3]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              sc[n][i] += c0[n][i];
+              sd[n][i] += c1[n][i];
+            }
           }
         }
       }
@@ -327,7 +341,7 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
           lsum[n][j] = lsum[n][j] * alpha[n][j] + (sc[n][j] + sc[n][2 + j]);
         }
       }
-      if (__any_sync(0xffffffffu, grew)) {
+      if (kB && __any_sync(0xffffffffu, grew)) {  // fp32 scales where it adds
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -372,9 +386,9 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
           for (int n = 0; n < NT; ++n) pg_mma_bf16(o[n][i], va, pb[n][0], pb[n][1]);
         }
       } else {
+        uint32_t bh[2][NT][2], bl[2][NT][2];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          uint32_t bh[NT][2], bl[NT][2];
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -383,10 +397,17 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
               const int src = 4 * (4 * j + t4) + (g >> 1);
               const float p0 = __shfl_sync(0xffffffffu, sc[n][2 * kb], src);
               const float p1 = __shfl_sync(0xffffffffu, sc[n][2 * kb + 1], src);
-              pg_split(g & 1 ? p1 : p0, bh[n][j], bl[n][j]);
+              pg_split(g & 1 ? p1 : p0, bh[kb][n][j], bl[kb][n][j]);
             }
 #pragma unroll
-          for (int i = 0; i < MT; i += 2) {
+        for (int i = 0; i < MT; i += 2) {
+          float c0[NT][4], c1[NT][4];
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c0[n][e] = c1[n][e] = 0.f;
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
             float4 x, y;  // values 16 i + 4 g .. + 3 of keys 8 kb + t4 and 8 kb + 4 + t4
             const uint32_t ax = vs + pg_piece<T, HD>(8 * kb + t4, 4 * i + g), ay = vs + pg_piece<T, HD>(8 * kb + 4 + t4, 4 * i + g);
             asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(ax));
@@ -398,9 +419,9 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
             pg_split(y.y, hi[3], lo[3]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              pg_mma_tf32(o[n][i], lo, bh[n][0], bh[n][1]);
-              pg_mma_tf32(o[n][i], hi, bl[n][0], bl[n][1]);
-              pg_mma_tf32(o[n][i], hi, bh[n][0], bh[n][1]);
+              pg_mma_tf32(c0[n], lo, bh[kb][n][0], bh[kb][n][1]);
+              pg_mma_tf32(c0[n], hi, bl[kb][n][0], bl[kb][n][1]);
+              pg_mma_tf32(c0[n], hi, bh[kb][n][0], bh[kb][n][1]);
             }
             pg_split(x.z, hi[0], lo[0]);
             pg_split(x.w, hi[1], lo[1]);
@@ -408,11 +429,18 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
             pg_split(y.w, hi[3], lo[3]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              pg_mma_tf32(o[n][i + 1], lo, bh[n][0], bh[n][1]);
-              pg_mma_tf32(o[n][i + 1], hi, bl[n][0], bl[n][1]);
-              pg_mma_tf32(o[n][i + 1], hi, bh[n][0], bh[n][1]);
+              pg_mma_tf32(c1[n], lo, bh[kb][n][0], bh[kb][n][1]);
+              pg_mma_tf32(c1[n], hi, bl[kb][n][0], bl[kb][n][1]);
+              pg_mma_tf32(c1[n], hi, bh[kb][n][0], bh[kb][n][1]);
             }
           }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              o[n][i][e] = o[n][i][e] * alpha[n][e & 1] + c0[n][e];
+              o[n][i + 1][e] = o[n][i + 1][e] * alpha[n][e & 1] + c1[n][e];
+            }
         }
       }
       if (patch) {

@@ -1,0 +1,515 @@
+// paged_tc.cuh -- attention of many query rows per KV head over paged bf16
+// keys and values on the tcgen05 tensor cores (sm_100a): chunks of prompts.
+//
+// Rows.  The query heads of a KV head's group and the chunk's tokens are one
+// axis of rows (row r: token r / G, head r % G of the group), so a 128-row MMA
+// is full for any group size, and every K/V tile serves the whole group.  One
+// CTA takes 256 rows (two Q tiles; one of 128 for head_dim 256) and a run of
+// key tiles of 128 (64) keys.
+//
+// S = Q K^T and O += P V accumulate in tensor memory in fp32.  Softmax is
+// online, in fp32, thread = row; P is rounded to bf16 for the second product
+// (at most 2^-8 of each weight; l sums the unrounded P) and takes the place of
+// the S it came from.  O is rescaled only when a row's maximum grew by more
+// than 2^8 since its reference was set; the reference is exact, so this
+// changes no result but by rounding.
+//
+// What bounds it: for head_dim 128 the MMAs of a tile pair take 2048 cycles and
+// so do its 32K exponentials at 16 a cycle.  Two Q tiles in turn keep the tensor
+// core on one while the other's softmax runs.
+//
+// Tiles come from the pages by TMA, one box per page (or 128-key tile) and 64
+// columns, into a ring in consumption order K0 V0 K1 V1 ..., 128-byte swizzled:
+// K is the K-major B operand of S, V the MN-major B operand of O.
+//
+// Roles: warp 0 loads; warp 1 issues MMAs; warp 2 checks V tiles that some row
+// does not attend to entirely (masked weights are 0, and 0 times a value that
+// is not finite is NaN: rows outside every window become 0, such values are
+// taken out and added in the epilogue to the rows that attend to them); warps
+// 4-7 and 8-11 are the softmax of Q tile 0 and 1.
+//
+// Long key ranges with few rows are cut into parts (plan_tc_bf16); the part that
+// ends last merges them in part order.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include "paged_rows.cuh"
+#include "tc.cuh"
+
+namespace l3p {
+
+template <int HD>
+struct PgTcCfg {
+  static constexpr int kNQ = HD == 256 ? 1 : 2;     // Q tiles of 128 rows
+  static constexpr int kTN = HD == 256 ? 64 : 128;  // keys of a tile
+  static constexpr int kQBytes = kNQ * 128 * HD * 2;
+  static constexpr int kStage = kTN * HD * 2;
+  static constexpr int kStages = HD == 64 ? 8 : 5;
+  static constexpr int kSmem = kQBytes + kStages * kStage + 1024;
+  static constexpr int kThreads = 128 + kNQ * 128;
+  // tensor memory columns: S (and P in its place), then O
+  static constexpr int kS = HD == 256 ? 64 : 128;
+  static constexpr int kO = 256;
+  static_assert(kSmem <= 232448 - 512, "shared memory");
+};
+
+struct PgTcArgs {
+  const int* batch;
+  const void* q;
+  void* out;
+  long long q_stride, out_stride;
+  const __nv_bfloat16* storage;  // page 0
+  long long page_elems;
+  int row_k;       // storage row of (page 0, layer, K, head 0, slot 0)
+  int page_rows;   // storage rows of a page
+  int n_kv, shift, G, win, window;
+  int n_tokens, with_rows;
+  float scale_log2;
+  float* ws_o;     // [slot][kNQ * 128][HD]
+  float* ws_ml;    // [slot][kNQ * 128][2]
+  unsigned* tickets;
+  int* err;
+};
+
+// mbar_wait_bounded with a limit of about a second: no wait inside one GPU
+// takes longer than the kernel's own milliseconds.
+__device__ __forceinline__ bool pg_wait(uint64_t* bar, uint32_t parity, int* err) {
+  for (uint32_t i = 0; i < (1u << 18); ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  *reinterpret_cast<volatile int*>(err) = kErrTimeout;
+  return false;
+}
+
+__host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, bool b_mn_major) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void mma_bf16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      : "memory");
+}
+__device__ __forceinline__ void pg_tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
+      "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
+      "r"(v[31])
+      : "memory");
+}
+
+// Merge of a split unit's rows by one warp: out row = sum_p w_p o_p / sum_p w_p l_p
+// with w_p = 2^(m_p - max m), in part order.  Lane holds HD/32 values.
+template <int HD, typename Store>
+__device__ __forceinline__ void pg_merge_row(const float* ws_o, const float* ws_ml, long long slot0, int rows, int row,
+                                             int n_parts, int lane, Store store) {
+  constexpr int N = HD / 32;
+  float M = -INFINITY;
+  for (int p = lane; p < n_parts; p += 32) M = fmaxf(M, __ldcg(ws_ml + ((slot0 + p) * rows + row) * 2));
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+  float acc[N], L = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+#pragma unroll 4
+  for (int p = 0; p < n_parts; ++p) {
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(ws_ml + ((slot0 + p) * rows + row) * 2));
+    const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
+    L += w * ml.y;
+    const float* o = ws_o + ((slot0 + p) * rows + row) * HD + lane * N;
+    if constexpr (N == 2) {
+      const float2 t = __ldcg(reinterpret_cast<const float2*>(o));
+      acc[0] += w * t.x, acc[1] += w * t.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) {
+        const float4 t = __ldcg(reinterpret_cast<const float4*>(o + i));
+        acc[i] += w * t.x, acc[i + 1] += w * t.y, acc[i + 2] += w * t.z, acc[i + 3] += w * t.w;
+      }
+    }
+  }
+  const float inv = 1.f / L;
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] *= inv;
+  store(acc);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
+    paged_tc_kernel(const PgTcArgs a, const __grid_constant__ CUtensorMap tmap) {
+  using C = PgTcCfg<HD>;
+  constexpr int S = C::kStages, TN = C::kTN, NQ = C::kNQ;
+  extern __shared__ unsigned char tc_smem_raw[];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_bad, s_last[2];
+  __shared__ __align__(8) uint64_t kv_full[S], kv_empty[S], v_ok[S];
+  __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_done[2], q_ready[2], mma_idle;
+
+  const PgHeader* h = reinterpret_cast<const PgHeader*>(a.batch);
+  const PgLists l = h->lists[a.win];
+  if (h->n_tokens > a.n_tokens || l.n_tc > (int)gridDim.x || (l.row_ctas != 0) != (a.with_rows != 0)) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
+    return;
+  }
+  if ((int)blockIdx.x >= l.n_tc) return;
+  const PgPart u = reinterpret_cast<const PgPart*>(a.batch + l.tc_parts)[blockIdx.x];
+  const int* table = a.batch + h->tbl + u.tbl;
+  unsigned char* sq = (unsigned char*)(((uintptr_t)tc_smem_raw + 1023) & ~(uintptr_t)1023);
+  unsigned char* ring = sq + C::kQBytes;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int nq = u.n_rows > 128 ? NQ : 1;
+  const int nt = u.tile1 - u.tile0;
+  const int first_pos = u.pos0 + u.r0 / a.G, last_pos = u.pos0 + (u.r0 + u.n_rows - 1) / a.G;
+  const int lo_first = a.win ? max(0, first_pos - a.window + 1) : 0;  // keys below: no row attends to them
+  const int lo_last = a.win ? max(0, last_pos - a.window + 1) : 0;    // keys from here to first_pos: every row does
+
+  if (warp == 0) {
+    tc::tmem_alloc(&s_tmem, 512);
+    tc::tmem_relinquish();
+  }
+  if (tid == 32) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+      mbar_init(&v_ok[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&s_full[b], 1);
+      mbar_init(&p_full[b], 4);
+      mbar_init(&o_done[b], 1);
+      mbar_init(&q_ready[b], 4);
+    }
+    mbar_init(&mma_idle, 1);
+    s_bad = 0;
+    fence_mbar_init();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tm = s_tmem;
+
+  if (warp == 0) {
+    // ---------------- loads ----------------
+    const int box = min(1 << a.shift, TN), n_box = TN / box;  // keys of a box, boxes down a tile
+    const int i = lane % n_box, c = lane / n_box;             // this lane's box and column block
+    const bool mine = c < HD / 64;
+    bool ok = true;
+    int n_used = 0;
+    for (int t = 0; ok && t < 2 * nt; ++t) {  // K and V of a tile in turn
+      const int s = t % S, use = t / S;
+      if (use > 0) ok = __all_sync(0xffffffffu, pg_wait(&kv_empty[s], (uint32_t)((use - 1) & 1), a.err));
+      if (!ok) break;
+      const int key = (u.tile0 + t / 2) * TN + i * box;
+      const bool load = mine && key < u.key_hi;
+      const int n = __popc(__ballot_sync(0xffffffffu, load));
+      if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], (uint32_t)(n * box * 128));
+      __syncwarp();
+      if (load) {
+        const int page = table[key >> a.shift];
+        const int row = page * a.page_rows + a.row_k + (((t & 1) * a.n_kv + u.kvh) << a.shift) + (key & ((1 << a.shift) - 1));
+        pg_tma_2d(smem_addr(ring + s * C::kStage + c * (TN * 128) + i * (box * 128)), &tmap, c * 64, row, &kv_full[s]);
+      }
+      n_used = t + 1;
+    }
+    // no copy may still be landing when the CTA ends
+    for (int t = max(0, n_used - S); t < n_used; ++t) pg_wait(&kv_full[t % S], (uint32_t)((t / S) & 1), a.err);
+  } else if (warp == 1) {
+    // ---------------- MMA issue ----------------
+    if (lane == 0) {
+      constexpr uint32_t id_s = idesc_bf16(128, TN, false), id_o = idesc_bf16(128, HD, true);
+      const uint64_t q_d = tc::sdesc_sw128(smem_addr(sq), 16, 1024);
+      const uint64_t k_d = tc::sdesc_sw128(smem_addr(ring), 16, 1024);
+      const uint64_t v_d = tc::sdesc_sw128(smem_addr(ring), TN * 128, 1024);
+      auto add = [](uint64_t d, uint32_t bytes) { return d + (bytes >> 4); };
+      auto qk = [&](int b, int slot, int stage) {  // S[slot] = Q[b] K^T
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+          mma_bf16_ss(tm + slot * C::kS, add(q_d, b * (128 * HD * 2) + (k / 4) * 16384 + (k % 4) * 32),
+                      add(k_d, stage * C::kStage + (k / 4) * (TN * 128) + (k % 4) * 32), id_s, k > 0);
+      };
+      auto pv = [&](int b, int slot, int stage, bool acc) {  // O[b] += P[slot] V
+#pragma unroll
+        for (int k = 0; k < TN / 16; ++k)
+          mma_bf16_ts(tm + C::kO + b * HD, tm + slot * C::kS + k * 8, add(v_d, stage * C::kStage + k * 2048), id_o, acc || k > 0);
+      };
+      auto wait = [&](uint64_t* bar, int phase) {
+        const bool r = pg_wait(bar, (uint32_t)(phase & 1), a.err);
+        tc::fence_after_sync();
+        return r;
+      };
+      bool ok = true;
+      if constexpr (NQ == 2) {
+        // S of both tiles, then per key tile and Q tile: O += P V, S of the next key tile.  MMAs run in the order of
+        // issue, so S may overwrite the P that the product before it reads.
+        ok = wait(&kv_full[0], 0);
+        for (int b = 0; ok && b < nq; ++b) {
+          if (!(ok = wait(&q_ready[b], 0))) break;
+          qk(b, b, 0);
+          tc::commit(&s_full[b]);
+        }
+        tc::commit(&kv_empty[0]);
+        for (int j = 0; ok && j < nt; ++j) {
+          const int tv = 2 * j + 1, tk = 2 * j + 2, sv = tv % S, sk = tk % S;
+          for (int b = 0; ok && b < nq; ++b) {
+            if (b == 0 && !(ok = wait(&v_ok[j % S], j / S))) break;
+            if (!(ok = wait(&p_full[b], j))) break;
+            pv(b, b, sv, j > 0);
+            if (b == nq - 1) tc::commit(&kv_empty[sv]);
+            tc::commit(&o_done[b]);
+            if (j + 1 < nt) {
+              if (b == 0 && !(ok = wait(&kv_full[sk], tk / S))) break;
+              qk(b, b, sk);
+              tc::commit(&s_full[b]);
+              if (b == nq - 1) tc::commit(&kv_empty[sk]);
+            }
+          }
+        }
+      } else {
+        // one Q tile, S in two places: S of the next key tile is issued ahead of this tile's O += P V
+        ok = wait(&kv_full[0], 0) && wait(&q_ready[0], 0);
+        if (ok) {
+          qk(0, 0, 0);
+          tc::commit(&s_full[0]);
+          tc::commit(&kv_empty[0]);
+        }
+        for (int j = 0; ok && j < nt; ++j) {
+          const int tv = 2 * j + 1, tk = 2 * j + 2, sv = tv % S, sk = tk % S;
+          if (j + 1 < nt) {
+            if (!(ok = wait(&kv_full[sk], tk / S))) break;
+            qk(0, (j + 1) & 1, sk);
+            tc::commit(&s_full[(j + 1) & 1]);
+            tc::commit(&kv_empty[sk]);
+          }
+          if (!(ok = wait(&v_ok[j % S], j / S) && wait(&p_full[j & 1], j >> 1))) break;
+          pv(0, j & 1, sv, j > 0);
+          tc::commit(&kv_empty[sv]);
+          tc::commit(&o_done[0]);
+        }
+      }
+      // every MMA has ended before tensor memory is released
+      tc::commit(&mma_idle);
+      pg_wait(&mma_idle, 0, a.err);
+    }
+  } else if (warp == 2) {
+    // ---------------- V tiles that are not attended to entirely ----------------
+    bool ok = true;
+    for (int j = 0; ok && j < nt; ++j) {
+      const int t = 2 * j + 1, s = t % S;
+      ok = __all_sync(0xffffffffu, pg_wait(&kv_full[s], (uint32_t)((t / S) & 1), a.err));
+      if (!ok) break;
+      const int key0 = (u.tile0 + j) * TN;
+      if (key0 + TN - 1 > first_pos || key0 < lo_last) {
+        unsigned char* v = ring + s * C::kStage;
+        bool bad = false;
+#pragma unroll 4
+        for (int x = lane; x < TN * HD / 8; x += 32) {  // 16-byte pieces: column block, key, piece
+          const int key = key0 + (x / 8) % TN;
+          uint4* p = reinterpret_cast<uint4*>(v + x * 16);
+          if (key >= u.key_hi || key < lo_first) {
+            *p = make_uint4(0u, 0u, 0u, 0u);
+          } else {
+            uint4 w = *p;
+            if (pg_clean<__nv_bfloat16>(w)) {
+              *p = w;
+              bad = true;
+            }
+          }
+        }
+        if (bad) *reinterpret_cast<volatile int*>(&s_bad) = 1;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      }
+      if (lane == 0) mbar_arrive(&v_ok[j % S]);  // by V tile: a stage holds K tiles in between
+    }
+  } else if (warp >= 4 && (warp - 4) / 4 < nq) {
+    // ---------------- softmax: thread = row ----------------
+    const int b = (warp - 4) / 4;
+    const int row = (warp & 3) * 32 + lane;  // of this Q tile
+    const uint32_t lb = (uint32_t)((warp & 3) * 32) << 16;
+    const int rr = b * 128 + row;            // of the part
+    const bool valid = rr < u.n_rows;
+    const int r = u.r0 + min(rr, u.n_rows - 1);
+    const int tok = r / a.G, head = u.kvh * a.G + r % a.G;
+    const int qpos = u.pos0 + tok;
+    const int kmin = a.win ? max(0, qpos - a.window + 1) : 0;
+    {
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) +
+                                                        (long long)(u.q_row0 + tok) * a.q_stride + (long long)head * HD);
+      unsigned char* dst = sq + b * (128 * HD * 2) + row * 128;
+#pragma unroll 8
+      for (int i = 0; i < HD / 8; ++i)
+        *reinterpret_cast<uint4*>(dst + (i / 8) * 16384 + (((i % 8) ^ (row & 7)) << 4)) = valid ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_ready[b]);
+    }
+    float m = -INFINITY, lsum = 0.f;  // m: largest score before scaling (of -score for a negative scale)
+    bool ok = true;
+    const float sl = a.scale_log2, asl = fabsf(sl);
+    const uint32_t T_O = tm + C::kO + b * HD + lb;
+    for (int j = 0; j < nt; ++j) {
+      const int slot = NQ == 2 ? b : j & 1;
+      ok = __all_sync(0xffffffffu, pg_wait(&s_full[slot], (uint32_t)((NQ == 2 ? j : j >> 1) & 1), a.err));
+      // With S in two places softmax may be two tiles ahead of O; a barrier's parity tells only neighbouring phases apart,
+      // so every phase of o_done is waited for in turn.
+      if (NQ == 1 && ok && j > 1) ok = __all_sync(0xffffffffu, pg_wait(&o_done[b], (uint32_t)(j & 1), a.err));
+      if (!ok) break;
+      tc::fence_after_sync();
+      const uint32_t T_S = tm + slot * C::kS + lb;
+      float sv[TN];
+#pragma unroll
+      for (int c = 0; c < TN / 32; ++c) {
+        float t[32];
+        tc::ld32(T_S + c * 32, t);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) sv[c * 32 + i] = t[i];
+      }
+      tc::wait_ld();
+      const int key0 = (u.tile0 + j) * TN;
+      if (!__all_sync(0xffffffffu, key0 >= kmin && key0 + TN - 1 <= qpos)) {
+#pragma unroll
+        for (int c = 0; c < TN; ++c)
+          if (key0 + c > qpos || key0 + c < kmin) sv[c] = sl >= 0.f ? -INFINITY : INFINITY;
+      }
+      // the row's largest scaled score: the largest raw score for a positive scale, the smallest for a negative one
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (sl >= 0.f) {
+#pragma unroll
+        for (int c = 0; c < TN; ++c) mx[c & 3] = fmaxf(mx[c & 3], sv[c]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < TN; ++c) mx[c & 3] = fmaxf(mx[c & 3], -sv[c]);
+      }
+      const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+      const bool grow = m == -INFINITY ? m_new != -INFINITY : (m_new - m) * asl > 8.f;
+      float alpha = 1.f;
+      if (grow) {
+        alpha = m == -INFINITY ? 0.f : fast_exp2((m - m_new) * asl);
+        lsum *= alpha;
+        m = m_new;
+      }
+      if (j > 0 && __any_sync(0xffffffffu, grow)) {
+        ok = __all_sync(0xffffffffu, pg_wait(&o_done[b], (uint32_t)((j - 1) & 1), a.err));
+        if (!ok) break;
+        tc::fence_after_sync();
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          float ov[32];
+          tc::ld32(T_O + c * 32, ov);
+          tc::wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) ov[i] *= alpha;
+          tc::st32(T_O + c * 32, ov);
+        }
+      }
+      const float neg = m == -INFINITY ? 0.f : -m * asl;
+      float ls[2] = {0.f, 0.f};
+#pragma unroll
+      for (int hf = 0; hf < TN / 64; ++hf) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float p0 = fast_exp2(fmaf(sv[hf * 64 + 2 * c], sl, neg)), p1 = fast_exp2(fmaf(sv[hf * 64 + 2 * c + 1], sl, neg));
+          ls[0] += p0;
+          ls[1] += p1;
+          pk[c] = pg_pack_bf16(p0, p1);
+        }
+        tmem_st32u(T_S + hf * 32, pk);
+      }
+      lsum += ls[0] + ls[1];
+      tc::wait_st();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[slot]);
+    }
+    if (NQ == 1 && ok && nt > 1) ok = __all_sync(0xffffffffu, pg_wait(&o_done[b], (uint32_t)(nt & 1), a.err));
+    if (ok) ok = __all_sync(0xffffffffu, pg_wait(&o_done[b], (uint32_t)((nt - 1) & 1), a.err));
+    if (ok) {
+      tc::fence_after_sync();
+      const bool split = u.n_parts > 1;
+      const float inv = split ? 1.f : 1.f / lsum;
+      const bool bad = *reinterpret_cast<volatile int*>(&s_bad) != 0;
+      const long long ws_row = (long long)(u.slot + u.part) * (NQ * 128) + rr;
+      __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(a.out) + (long long)(u.q_row0 + tok) * a.out_stride + (long long)head * HD;
+      const __nv_bfloat16* vbase = a.storage + ((long long)a.row_k + ((long long)(a.n_kv + u.kvh) << a.shift)) * HD;
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        float ov[32];
+        tc::ld32(T_O + c * 32, ov);
+        tc::wait_ld();
+        if (bad && valid) {
+          for (int key = max(kmin, u.tile0 * TN); key <= min(qpos, u.tile1 * TN - 1); ++key) {
+            const int key0 = key / TN * TN;
+            if (!(key0 + TN - 1 > first_pos || key0 < lo_last)) continue;  // not taken out of this tile
+            const __nv_bfloat16* v = vbase + (long long)table[key >> a.shift] * a.page_elems + (long long)(key & ((1 << a.shift) - 1)) * HD + c * 32;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float x = __bfloat162float(v[i]);
+              if (!pg_finite(x)) ov[i] += x;
+            }
+          }
+        }
+        if (valid) {
+          if (split) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(a.ws_o + ws_row * HD + c * 32 + i) = make_float4(ov[i], ov[i + 1], ov[i + 2], ov[i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint4 w;
+              w.x = pg_pack_bf16(ov[i] * inv, ov[i + 1] * inv);
+              w.y = pg_pack_bf16(ov[i + 2] * inv, ov[i + 3] * inv);
+              w.z = pg_pack_bf16(ov[i + 4] * inv, ov[i + 5] * inv);
+              w.w = pg_pack_bf16(ov[i + 6] * inv, ov[i + 7] * inv);
+              *reinterpret_cast<uint4*>(orow + c * 32 + i) = w;
+            }
+          }
+        }
+      }
+      if (split) {
+        if (valid) *reinterpret_cast<float2*>(a.ws_ml + ws_row * 2) = make_float2(m == -INFINITY ? m : m * asl, lsum);
+        __threadfence();
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + b) : "memory");
+        if ((tid & 127) == 0) s_last[b] = atomicAdd(a.tickets + u.ticket * 2 + b, 1u) == (unsigned)u.n_parts - 1;
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + b) : "memory");
+        if (s_last[b]) {
+          __threadfence();
+          if ((tid & 127) == 0) a.tickets[u.ticket * 2 + b] = 0;
+          for (int x = (warp & 3); x < 128 && b * 128 + x < u.n_rows; x += 4) {
+            const int q = u.r0 + b * 128 + x;
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (long long)(u.q_row0 + q / a.G) * a.out_stride +
+                                 (long long)(u.kvh * a.G + q % a.G) * HD + lane * (HD / 32);
+            pg_merge_row<HD>(a.ws_o, a.ws_ml, u.slot, NQ * 128, b * 128 + x, u.n_parts, lane, [&](const float (&acc)[HD / 32]) {
+#pragma unroll
+              for (int i = 0; i < HD / 32; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pg_pack_bf16(acc[i], acc[i + 1]);
+            });
+          }
+        }
+      }
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 0) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tm, 512);
+  }
+}
+
+}  // namespace l3p

@@ -102,12 +102,13 @@ class PagedCache:
 
     def storage(self):
         """The pool as a tensor [n_pages][n_layers][2: K, V][n_kv_heads][page_size][head_dim] that shares its
-        memory; valid while the cache is open."""
+        memory and keeps the cache alive; valid until close()."""
         base, size = C.c_void_p(), C.c_size_t()
         self._ok(self.lib.l3p_paged_storage(self.h, C.byref(base), C.byref(size)), "storage")
         c = self.cfg
 
         class _Memory:  # bfloat16 has no array-interface type: 16-bit integers, viewed below
+            owner = self  # the tensor holds this object, and so the cache
             __cuda_array_interface__ = {
                 "shape": (c.n_pages, c.n_layers, 2, c.n_kv_heads, c.page_size, c.head_dim),
                 "typestr": "<f4" if c.dtype == 0 else "<i2", "data": (base.value, False), "version": 3, "stream": None,

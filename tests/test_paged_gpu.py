@@ -643,6 +643,23 @@ def test_refusals_change_nothing(torch):
         b.step([s], [1])
 
 
+def test_storage_keeps_the_cache(torch):
+    import gc
+    import weakref
+
+    c = _cache(n_layers=1)
+    gone = weakref.ref(c)
+    st = c.storage()
+    view = st[1:2]
+    del c, st
+    gc.collect()
+    assert gone() is not None  # ahead of any use of the view
+    assert not bool(view.any())
+    del view
+    gc.collect()
+    assert gone() is None
+
+
 def test_create_without_memory(torch):
     with pytest.raises(AttnError) as e:
         _cache(n_layers=64, n_heads=8, n_kv_heads=8, head_dim=256, page_size=128, n_pages=16000)  # 537 GB
