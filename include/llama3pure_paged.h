@@ -141,7 +141,9 @@ typedef struct l3p_paged_rope_config {
     const float* q_norm; /* HOST [n_layers][head_dim] weights of an RMS norm of every q / k head ahead of the */
     const float* k_norm; /*   rotation (c:3150-3165), both or neither; NULL: none */
 } l3p_paged_rope_config;
-/* Builds the cosine and sine tables, angles in double precision.  Calling it again replaces them. */
+/* Builds the cosine and sine tables, angles in double precision.  Calling it
+ * again replaces them; graphs captured before keep the ones they were captured
+ * with.  Waits for the device. */
 int l3p_paged_set_rope(l3p_paged_ctx* ctx, const l3p_paged_rope_config* rope);
 /* Norm (when configured) and rotation of the batch's q and k rows; q goes to
  * q_out (which may be q), k and v into the pages.  One launch. */

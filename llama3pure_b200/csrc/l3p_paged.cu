@@ -185,16 +185,27 @@ void plan_rows(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, int nt
 }
 
 // Tensor-core kernels: units (sequence, KV head, block of rows); with too few
-// of them for the GPU (bf16), long key ranges are cut into parts of equal
-// size, merged by the part that ends last.  Longest parts first.
-void plan_tc_bf16(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vector<PgPart>* parts) {
-  const int limit = row_limit(ctx), tile = tc_tile(ctx), rt = tc_rows(ctx), G = ctx->G;
+// of them for the GPU, long key ranges are cut into parts of equal size, merged
+// by the part that ends last.  Longest parts first.  fp32 pools: also the list
+// of the key tiles that the units read.
+void plan_tc(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vector<PgPart>* parts,
+             std::vector<PgPrep>* prep) {
+  const int limit = row_limit(ctx), tile = ctx->bf16 ? tc_tile(ctx) : 128, G = ctx->G;
+  const int rt = ctx->bf16 ? tc_rows(ctx) : f32_rows(ctx);
+  // CTAs (or CTA pairs) that run at once
+  const int wide = !ctx->bf16 && rt == 256 ? ctx->num_sms / 2 : ctx->num_sms;
   std::vector<PgPart> units;
   long long total = 0;
   for (const auto& b : bs) {
     const long long rows = (long long)b.n_new * G;
     if (rows <= limit) continue;
     const int pos0 = b.len - b.n_new;
+    int img0 = 0;
+    if (!ctx->bf16) {
+      const int t0 = first_key(ctx, win, pos0) / tile, t1 = (b.len + tile - 1) / tile;
+      img0 = (int)prep->size() - t0;
+      for (int t = t0; t < t1; ++t) prep->push_back({b.tbl, t * tile, b.len, img0 + t});
+    }
     for (long long r0 = 0; r0 < rows; r0 += rt)
       for (int h = 0; h < ctx->cfg.n_kv_heads; ++h) {
         PgPart u{};
@@ -207,12 +218,13 @@ void plan_tc_bf16(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std
         u.key_hi = pos0 + (int)((r0 + u.n_rows - 1) / G) + 1;
         u.tile0 = first_key(ctx, win, pos0 + (int)(r0 / G)) / tile;
         u.tile1 = (u.key_hi + tile - 1) / tile;
+        u.img = img0;
         total += u.tile1 - u.tile0;
         units.push_back(u);
       }
   }
   // no part is shorter than 4 tiles: below that the merge costs more than the split saves
-  const int cap = (int)std::max<long long>(4, (total + ctx->num_sms - 1) / ctx->num_sms);
+  const int cap = (int)std::max<long long>(4, (total + wide - 1) / wide);
   int ticket = 0, slot = 0;
   for (const auto& u : units) {
     const int n = u.tile1 - u.tile0, k = (n + cap - 1) / cap;
@@ -229,34 +241,6 @@ void plan_tc_bf16(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std
     if (k > 1) {
       ++ticket;
       slot += k;
-    }
-  }
-  std::stable_sort(parts->begin(), parts->end(),
-                   [](const PgPart& a, const PgPart& b) { return a.tile1 - a.tile0 > b.tile1 - b.tile0; });
-}
-
-// fp32 pools: units (sequence, 128 query tokens) times the query heads, and the key tiles they read.
-void plan_tc_f32(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vector<PgPart>* parts,
-                 std::vector<PgPrep>* prep) {
-  const int limit = row_limit(ctx);
-  for (const auto& b : bs) {
-    if ((long long)b.n_new * ctx->G <= limit) continue;
-    const int pos0 = b.len - b.n_new;
-    const int t0 = first_key(ctx, win, pos0) / 128, t1 = (b.len + 127) / 128;
-    const int img0 = (int)prep->size() - t0;  // image of the sequence's tile 0
-    for (int t = t0; t < t1; ++t) prep->push_back({b.tbl, t * 128, b.len, img0 + t});
-    for (int r0 = 0; r0 < b.n_new; r0 += 128) {
-      PgPart u{};
-      u.tbl = b.tbl;
-      u.key_hi = b.len;
-      u.q_row0 = b.q_row0;
-      u.pos0 = pos0;
-      u.img = img0;
-      u.qbase = pos0 + r0;
-      u.q_end = b.len;
-      u.tile0 = first_key(ctx, win, u.qbase) / 128;
-      u.tile1 = (std::min(u.qbase + 128, u.q_end) - 1) / 128 + 1;
-      parts->push_back(u);
     }
   }
   std::stable_sort(parts->begin(), parts->end(),
@@ -289,10 +273,7 @@ void build_batch(const Ctx* ctx, const std::vector<BatchSeq>& bs, const int* seq
     std::vector<PgPart> parts;
     std::vector<PgPrep> prep;
     plan_rows(ctx, v == 1, bs, h.row_nt, &first, &segs);
-    if (ctx->bf16)
-      plan_tc_bf16(ctx, v == 1, bs, &parts);
-    else if (ctx->hd != 256)
-      plan_tc_f32(ctx, v == 1, bs, &parts, &prep);
+    plan_tc(ctx, v == 1, bs, &parts, &prep);
     PgLists& l = h.lists[v];
     l.row_ctas = first.empty() ? 0 : (int)first.size() - 1;
     l.row_first = add(first.data(), first.size() * 4);
@@ -356,6 +337,7 @@ void release(Ctx* ctx) {
   if (ctx->rope_tab_swa != ctx->rope_tab) cudaFree(ctx->rope_tab_swa);
   cudaFree(ctx->rope_tab);
   cudaFree(ctx->qk_norm);
+  for (void* p : ctx->retired) cudaFree(p);
   if (ctx->err_host) cudaFreeHost(ctx->err_host);
 }
 

@@ -1,5 +1,119 @@
-#include "paged.h"
+// l3p_paged_f32.cu -- launcher of the fp32 tensor-core kernels (paged_f32.cuh).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "paged_f32.cuh"
+
+using namespace l3p;
+
 namespace l3p_pg {
-int init_f32(l3p_paged_ctx*) { return L3P_OK; }
-int launch_f32(l3p_paged_ctx* ctx, int, const void*, long long, void*, long long, cudaStream_t) { return L3P_E_UNSUPPORTED; }
+
+// Images of more than this are made for some KV heads at a time.
+static constexpr size_t kImageBytes = 1ull << 30;
+
+int f32_rows(const l3p_paged_ctx* ctx) { return ctx->hd == 64 ? 128 : 256; }
+
+int init_f32(l3p_paged_ctx* ctx) {
+  if (ctx->hd == 256) return L3P_OK;  // rows of 256 values take the row kernel
+  if (ctx->hd == 64)
+    PG_CUDA(ctx, cudaFuncSetAttribute(paged_f32_kernel<1, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, PgF32Cfg<1, 64>::kSmem));
+  else
+    PG_CUDA(ctx, cudaFuncSetAttribute(paged_f32_kernel<2, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, PgF32Cfg<2, 128>::kSmem));
+  const size_t rows = 2 * (size_t)ctx->num_sms * f32_rows(ctx);  // as in init_tc
+  if (cudaMalloc(&ctx->tc_o, rows * ctx->hd * sizeof(float)) != cudaSuccess ||
+      cudaMalloc(&ctx->tc_ml, rows * 2 * sizeof(float)) != cudaSuccess ||
+      cudaMalloc(&ctx->tc_tickets, 2 * (size_t)ctx->num_sms * sizeof(unsigned)) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(ctx, L3P_E_NOMEM, "the split workspace does not fit on the device");
+  }
+  PG_CUDA(ctx, cudaMemset(ctx->tc_tickets, 0, 2 * (size_t)ctx->num_sms * sizeof(unsigned)));
+  return L3P_OK;
 }
+
+// Makes the image buffer hold `floats` and the flags `n`.
+static int ensure_images(l3p_paged_ctx* ctx, size_t floats, size_t n, cudaStream_t s) {
+  if (floats <= ctx->img_floats && n <= ctx->v_flags_n) return L3P_OK;
+  if (capturing(s))
+    return fail(ctx, L3P_E_INVAL, "the fp32 chunk's workspace must grow to %zu bytes, which cannot happen during stream capture: "
+                "make one call of this size before capturing", floats * sizeof(float));
+  PG_CUDA(ctx, cudaStreamSynchronize(s));
+  retire(ctx, ctx->img, ctx->img_captured);
+  retire(ctx, ctx->v_flags, ctx->img_captured);
+  ctx->img_captured = false;
+  ctx->img = nullptr;
+  ctx->v_flags = nullptr;
+  ctx->img_floats = ctx->v_flags_n = 0;
+  if (cudaMalloc(&ctx->img, floats * sizeof(float)) != cudaSuccess || cudaMalloc(&ctx->v_flags, n * sizeof(int)) != cudaSuccess) {
+    cudaGetLastError();
+    cudaFree(ctx->img);
+    ctx->img = nullptr;
+    return fail(ctx, L3P_E_NOMEM, "the fp32 chunk's workspace of %zu bytes does not fit on the device", floats * sizeof(float));
+  }
+  ctx->img_floats = floats;
+  ctx->v_flags_n = n;
+  return L3P_OK;
+}
+
+template <int CG, int HD>
+static int launch(l3p_paged_ctx* ctx, PgF32Args a, const PgLists& l, cudaStream_t s) {
+  const size_t tile = PfGeom<HD>::kTileFloats;
+  const int n_kv = ctx->cfg.n_kv_heads;
+  const size_t fit = std::max<size_t>(1, kImageBytes / (tile * sizeof(float) * l.n_prep));
+  const int group = (int)std::min<size_t>(fit, n_kv);
+  if (int rc = ensure_images(ctx, tile * l.n_prep * group, (size_t)l.n_prep * group, s)) return rc;
+  ctx->img_captured |= capturing(s);
+  a.img = ctx->img;
+  a.flags = ctx->v_flags;
+  for (int h = 0; h < n_kv; h += group) {
+    a.kvh0 = h;
+    a.n_kvh = std::min(group, n_kv - h);
+    paged_prep_kernel<CG, HD><<<dim3(l.n_prep, a.n_kvh), 256, 0, s>>>(a);
+    ++ctx->launches;
+    PG_CUDA(ctx, cudaGetLastError());
+    cudaLaunchConfig_t lc{};
+    lc.gridDim = dim3(l.n_tc * CG, 1, 1);
+    lc.blockDim = dim3(384, 1, 1);
+    lc.dynamicSmemBytes = PgF32Cfg<CG, HD>::kSmem;
+    lc.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    lc.attrs = attr;
+    lc.numAttrs = CG == 2 ? 1 : 0;
+    PG_CUDA(ctx, cudaLaunchKernelEx(&lc, paged_f32_kernel<CG, HD>, a));
+    ++ctx->launches;
+  }
+  return L3P_OK;
+}
+
+int launch_f32(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void* out, long long os, cudaStream_t s) {
+  const bool win = windowed(ctx, layer);
+  const PgLists& l = ctx->hdr.lists[win ? 1 : 0];
+  PgF32Args a{};
+  a.batch = ctx->batch;
+  a.q = static_cast<const float*>(q);
+  a.out = static_cast<float*>(out);
+  a.q_stride = qs;
+  a.out_stride = os;
+  a.storage = reinterpret_cast<const float*>(static_cast<char*>(ctx->storage) + (size_t)layer * 2 * ctx->cfg.n_kv_heads * ctx->block_bytes);
+  a.page_elems = (long long)(ctx->page_bytes / ctx->es);
+  a.v_off = (long long)(ctx->block_bytes / ctx->es) * ctx->cfg.n_kv_heads;
+  a.shift = ctx->shift;
+  a.G = ctx->G;
+  a.win = win ? 1 : 0;
+  a.window = ctx->cfg.swa_window;
+  a.n_tokens = ctx->hdr.n_tokens;
+  a.with_rows = l.row_ctas > 0;
+  a.n_prep = l.n_prep;
+  a.scale_log2 = ctx->scale * kLog2e;
+  a.ws_o = ctx->tc_o;
+  a.ws_ml = ctx->tc_ml;
+  a.tickets = ctx->tc_tickets;
+  a.err = ctx->err_dev;
+  return ctx->hd == 64 ? launch<1, 64>(ctx, a, l, s) : launch<2, 128>(ctx, a, l, s);
+}
+
+}  // namespace l3p_pg

@@ -183,9 +183,10 @@ int set_rope(l3p_paged_ctx* ctx, const l3p_paged_rope_config& in) {
     return fail(ctx, L3P_E_CUDA, "rotary tables: %s", cudaGetErrorString(e));
   }
   cudaFree(dfreq);
-  if (ctx->rope_tab_swa != ctx->rope_tab) cudaFree(ctx->rope_tab_swa);
-  cudaFree(ctx->rope_tab);
-  cudaFree(ctx->qk_norm);
+  if (ctx->rope_tab_swa != ctx->rope_tab) retire(ctx, ctx->rope_tab_swa, ctx->rope_captured);
+  retire(ctx, ctx->rope_tab, ctx->rope_captured);
+  retire(ctx, ctx->qk_norm, ctx->rope_captured);
+  ctx->rope_captured = false;
   ctx->rope_tab = tab;
   ctx->rope_tab_swa = ctx->swa ? tab_swa : tab;
   ctx->qk_norm = norm;
@@ -227,6 +228,7 @@ L3P_API int l3p_paged_rope_append_dev(l3p_paged_ctx* ctx, int layer, const void*
   a.q = q, a.k = k, a.v = v, a.q_out = q_out;
   a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.q_out_stride = q_out_stride;
   const bool win = windowed(ctx, layer);
+  ctx->rope_captured |= capturing(static_cast<cudaStream_t>(stream));
   a.tab = win ? ctx->rope_tab_swa : ctx->rope_tab;
   if (ctx->qk_norm) {
     a.q_norm = ctx->qk_norm + (size_t)layer * ctx->hd;

@@ -13,7 +13,7 @@ namespace l3p_pg {
 // fp32 with head_dim 256 has none: Q and O alone would fill tensor memory.
 int row_limit(const l3p_paged_ctx* ctx) {
   if (ctx->bf16) return ctx->hd == 256 ? 16 : 32;
-  return INT_MAX;
+  return ctx->hd == 256 ? INT_MAX : 16;
 }
 
 // Blocks of 8 rows whose Q and O fit a thread's registers.

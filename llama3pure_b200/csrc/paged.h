@@ -63,7 +63,7 @@ struct __align__(16) PgPart {
   int tbl, key_hi, tile0, tile1;
   int q_row0, pos0, r0, n_rows;
   int kvh, part, n_parts, ticket;
-  int slot, img, qbase, q_end;  // fp32: image tile of tile 0; position of the first query row, end of the chunk
+  int slot, img, pad[2];  // workspace slot of part 0; fp32 pools: image of tile 0
 };
 static_assert(sizeof(PgPart) == 64, "part");
 
@@ -132,6 +132,10 @@ struct l3p_paged_ctx {
   int rope_max = 0, rope_layout = 0, rotary_dim = 0;
   float rms_eps = 1e-5f;
 
+  // buffers that captured launches name: kept until the context ends when they are replaced
+  bool img_captured = false, rope_captured = false;
+  std::vector<void*> retired;
+
   int* err_host = nullptr;
   int* err_dev = nullptr;
   long long launches = 0;
@@ -139,6 +143,15 @@ struct l3p_paged_ctx {
 };
 
 namespace l3p_pg {
+
+// Lets a replaced device buffer go: at once, or with the context when a captured launch names it.
+inline void retire(l3p_paged_ctx* ctx, void* p, bool captured) {
+  if (!p) return;
+  if (captured)
+    ctx->retired.push_back(p);
+  else
+    cudaFree(p);
+}
 
 inline int fail(l3p_paged_ctx* ctx, int code, const char* fmt, ...) {
   if (ctx) {
@@ -186,7 +199,8 @@ int row_limit(const l3p_paged_ctx* ctx);
 int row_max_nt(const l3p_paged_ctx* ctx);  // blocks of 8 rows that one CTA takes at most
 int row_warps(const l3p_paged_ctx* ctx);
 int tc_tile(const l3p_paged_ctx* ctx);
-int tc_rows(const l3p_paged_ctx* ctx);  // rows of a part
+int tc_rows(const l3p_paged_ctx* ctx);  // rows of a part, bf16 pools
+int f32_rows(const l3p_paged_ctx* ctx);  // rows of a part, fp32 pools
 
 // Set-up of the kernels at create: shared-memory attributes, tensor map, workspaces.
 int init_rows(l3p_paged_ctx* ctx);

@@ -1,0 +1,512 @@
+// paged_f32.cuh -- attention of many query rows per KV head over paged fp32
+// keys and values on the tcgen05 tensor cores in 3xTF32 (sm_100a), head_dim 64
+// or 128: chunks of prompts.
+//
+// Rows are (token, head of the group) pairs of one KV head as in paged_tc.cuh.
+// The key tiles that the batch reads are first gathered from the pages and split
+// into tf32 hi and lo images in the tensor cores' shared-memory layout
+// (paged_prep_kernel; the layout is that of prefill_tc.cuh), once for all rows.
+//
+// Precision.  x = hi + lo with hi = x rounded to tf32; products are hi*hi +
+// hi*lo + lo*hi (2^-22 of a product is dropped).  The tensor core cuts its
+// accumulations off instead of rounding them: a chain of n MMAs loses about
+// n/2 * 2^-24 of the sum, always towards zero (1.6e-5 of the last rows of a 2K
+// prompt when O stays in one accumulator for all keys).  Therefore
+//   * the small products (hi*lo, lo*hi) of S go in before the hi*hi ones, so
+//     that only the latter meet a large accumulator;
+//   * O is accumulated in registers: the MMAs of 64 keys form a partial sum in
+//     tensor memory that an own warpgroup adds, in fp32 and rounded, to its row.
+// That warpgroup also applies the running maximum's factors, so O is never
+// rescaled in tensor memory.
+//
+// What bounds it: 2 x 3072 tensor-core cycles per 128 rows x 128 keys.
+//
+// CG = 2 (head_dim 128): the CTAs of a pair take 128 rows each of the same KV
+// head; every MMA is cta_group::2 with M = 256, and each CTA stages half of
+// every chunk.  CG = 1 for head_dim 64.
+// Roles (384 threads per CTA): warps 0, 2 load chunks in turn (1-D bulk copies);
+// warp 1 issues S (the odd CTA's relays landed chunks), warp 3 issues P V; warps
+// 4-7 softmax, thread = row; warps 8-11 hold O, thread = row.
+#pragma once
+#include "paged_tc.cuh"
+#include "prefill_tc.cuh"
+
+namespace l3p {
+
+// Ring of the chunk kernel: one stage less than PfCfg has, for the statically
+// allocated shared memory.  At least one tile's K chunks are held at once.
+template <int CG, int HD>
+struct PgF32Cfg {
+  static constexpr int kStages = PfCfg<CG, HD>::kStages - 1;
+  static constexpr int kSmem = PfGeom<HD>::kQloBytes + kStages * PfCfg<CG, HD>::kStageBytes + 1024;
+  static_assert(kStages >= PfGeom<HD>::kKChunks + 1 && kSmem <= 232448 - 3072, "shared memory");
+};
+
+struct PgF32Args {
+  const int* batch;
+  const float* q;
+  float* out;
+  long long q_stride, out_stride;
+  const float* storage;   // the layer's K block of page 0, head 0
+  long long page_elems, v_off;
+  float* img;             // [head of the group of heads][n_prep] tile images
+  int* flags;             // [head][n_prep]: the tile's V holds values that are not finite (0 in the image)
+  int kvh0, n_kvh;        // group of KV heads of this launch
+  int shift, G, win, window;
+  int n_tokens, with_rows, n_prep;
+  float scale_log2;
+  float* ws_o;            // [slot][CG * 128][HD]
+  float* ws_ml;
+  unsigned* tickets;
+  int* err;
+};
+
+__device__ __forceinline__ float pg_tf32(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xFFFFE000u); }
+
+// Tile images of the keys that the batch's chunks attend to.  grid (tiles, KV heads of the group), 256 threads.
+template <int CG, int HD>
+__global__ void paged_prep_kernel(const PgF32Args a) {
+  using C = PfCfg<CG, HD>;
+  using Gm = PfGeom<HD>;
+  const PgHeader* h = reinterpret_cast<const PgHeader*>(a.batch);
+  const PgLists l = h->lists[a.win];
+  if ((int)blockIdx.x >= l.n_prep) return;
+  const PgPrep p = reinterpret_cast<const PgPrep*>(a.batch + l.prep)[blockIdx.x];
+  const int* table = a.batch + h->tbl + p.tbl;
+  const long long slot = (long long)blockIdx.y * a.n_prep + p.img;
+  unsigned char* base = reinterpret_cast<unsigned char*>(a.img) + slot * Gm::kTileBytes;
+  const long long head = (long long)(a.kvh0 + blockIdx.y) * ((long long)HD << a.shift);
+  constexpr int kVRows = HD / CG;
+  constexpr int kVBase = Gm::kKChunks * C::kKBytes;
+  int bad = 0;
+#pragma unroll 4
+  for (int idx = threadIdx.x; idx < kPfBN * HD / 4; idx += 256) {
+    const int key = idx / (HD / 4), c16 = idx % (HD / 4);
+    const int pos = p.key0 + key;
+    float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+    if (pos < p.key_hi) {
+      const float* src = a.storage + (long long)table[pos >> a.shift] * a.page_elems + head +
+                         (long long)(pos & ((1 << a.shift) - 1)) * HD + 4 * c16;
+      k = *reinterpret_cast<const float4*>(src);
+      v = *reinterpret_cast<const float4*>(src + a.v_off);
+      uint4 w = *reinterpret_cast<const uint4*>(&v);
+      if (pg_clean<float>(w)) {
+        bad = 1;
+        v = *reinterpret_cast<const float4*>(&w);
+      }
+    }
+    const float4 kh = make_float4(pg_tf32(k.x), pg_tf32(k.y), pg_tf32(k.z), pg_tf32(k.w));
+    const float4 kl = make_float4(k.x - kh.x, k.y - kh.y, k.z - kh.z, k.w - kh.w);
+    const float4 vh = make_float4(pg_tf32(v.x), pg_tf32(v.y), pg_tf32(v.z), pg_tf32(v.w));
+    const float4 vl = make_float4(v.x - vh.x, v.y - vh.y, v.z - vh.z, v.w - vh.w);
+    const int part = c16 & 7;
+    const int kr = key / C::kRows, kk = key % C::kRows;
+    const int kb = kr * C::kHalfTile + (c16 >> 3) * C::kKBytes + kk * 128 + ((part ^ (kk & 7)) << 4);
+    *reinterpret_cast<float4*>(base + kb) = kh;
+    *reinterpret_cast<float4*>(base + kb + C::kKBytes / 2) = kl;
+    const int dim = 4 * c16, vr = dim / kVRows, atom = (dim % kVRows) >> 5;
+    const int kv = key & 31, byte = part * 16;
+    const int vb = vr * C::kHalfTile + kVBase + (key >> 5) * C::kVBytes + atom * 4096 + (kv >> 2) * 512 + (kv & 3) * 128 +
+                   ((((byte >> 5) ^ (kv & 3)) << 5) | (byte & 31));
+    *reinterpret_cast<float4*>(base + vb) = vh;
+    *reinterpret_cast<float4*>(base + vb + C::kVBytes / 2) = vl;
+  }
+  bad = __syncthreads_or(bad);
+  if (threadIdx.x == 0) a.flags[slot] = bad;
+}
+
+template <int CG, int HD>
+__global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
+  using C = PfCfg<CG, HD>;
+  using Gm = PfGeom<HD>;
+  constexpr int S = PgF32Cfg<CG, HD>::kStages;
+  extern __shared__ unsigned char f32_smem_raw[];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_last;
+  __shared__ float s_alpha[2][128], s_m[128], s_l[128];
+  __shared__ __align__(8) uint64_t bar_kv_full[S], bar_kv_empty[S], bar_kv_peer[S];
+  __shared__ __align__(8) uint64_t bar_s_full, bar_s_free, bar_p_full[2], bar_p_free[2];
+  __shared__ __align__(8) uint64_t bar_o_full, bar_o_free, bar_q_ready, bar_sm_done, bar_mma_idle[2];
+
+  const PgHeader* hd = reinterpret_cast<const PgHeader*>(a.batch);
+  const PgLists l = hd->lists[a.win];
+  if (hd->n_tokens > a.n_tokens || l.n_tc * CG > (int)gridDim.x || l.n_prep != a.n_prep || (l.row_ctas != 0) != (a.with_rows != 0)) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
+    return;
+  }
+  if ((int)blockIdx.x / CG >= l.n_tc) return;
+  const PgPart u = reinterpret_cast<const PgPart*>(a.batch + l.tc_parts)[blockIdx.x / CG];
+  if (u.kvh < a.kvh0 || u.kvh >= a.kvh0 + a.n_kvh) return;  // both CTAs of a pair
+  const int* table = a.batch + hd->tbl + u.tbl;
+  unsigned char* qlo = (unsigned char*)(((uintptr_t)f32_smem_raw + 1023) & ~(uintptr_t)1023);
+  unsigned char* ring = qlo + Gm::kQloBytes;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
+  const int nt = u.tile1 - u.tile0;
+  const long long img_slot = (long long)(u.kvh - a.kvh0) * a.n_prep + u.img + u.tile0;
+
+  if (warp == 0) {
+    tc::tmem_alloc_g<CG>(&s_tmem, 512);
+    tc::tmem_relinquish_g<CG>();
+  }
+  if (tid == 32) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&bar_kv_full[s], 1);
+      mbar_init(&bar_kv_empty[s], 1);
+      mbar_init(&bar_kv_peer[s], 1);
+    }
+    mbar_init(&bar_s_full, 1);
+    mbar_init(&bar_s_free, 4 * CG);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bar_p_full[b], 4 * CG);
+      mbar_init(&bar_p_free[b], 1);
+      mbar_init(&bar_mma_idle[b], 1);
+    }
+    mbar_init(&bar_o_full, 1);
+    mbar_init(&bar_o_free, 4 * CG);
+    mbar_init(&bar_q_ready, 4 * CG);
+    mbar_init(&bar_sm_done, 4);
+    fence_mbar_init();
+  }
+  tc::fence_before_sync();
+  if constexpr (CG == 2)
+    cluster_sync_all();
+  else
+    __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tm = s_tmem;
+  const uint32_t T_QHI = tm + 0, T_O = tm + HD, T_S = tm + 2 * HD, T_P = tm + 2 * HD + kPfBN;
+
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    for (uint32_t i = 0; i < (1u << 18); ++i)
+      if (CG == 2 ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
+    *reinterpret_cast<volatile int*>(a.err) = kErrTimeout;
+    return false;
+  };
+  auto arrive_issuer = [&](uint64_t* bar) {
+    if constexpr (CG == 2)
+      mbar_arrive_cluster(mapa_shared(smem_addr(bar), 0));
+    else
+      mbar_arrive(bar);
+  };
+  auto commit_all = [&](uint64_t* bar) {
+    tc::commit_g<CG>(smem_addr(bar));
+    if constexpr (CG == 2) tc::commit_g<CG>(mapa_shared(smem_addr(bar), 1));
+  };
+  // row of this thread (softmax and O warpgroups); rows behind the last one compute what it computes
+  const int row = (warp & 3) * 32 + lane;
+  const int rr = (int)rank * 128 + row;
+  const bool valid = rr < u.n_rows;
+  const int r = u.r0 + min(rr, u.n_rows - 1);
+  const int tok = r / a.G, head = u.kvh * a.G + r % a.G;
+  const int qpos = u.pos0 + tok;
+  const int kmin = a.win ? max(0, qpos - a.window + 1) : 0;
+  const uint32_t lb = (uint32_t)((warp & 3) * 32) << 16;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0 || warp == 2) {
+      // ---------------- producers, chunks in turn ----------------
+      if (lane == 0) {
+        const int me = warp >> 1;
+        const unsigned char* img = reinterpret_cast<const unsigned char*>(a.img) + img_slot * Gm::kTileBytes + rank * C::kHalfTile;
+        int c = 0;
+        bool ok = true;
+        for (int n = 0; ok && n <= nt; ++n) {
+          for (int part = 0; ok && part < 2; ++part) {
+            const int t = n - part;
+            if (t < 0 || t >= nt) continue;
+            const int n_ch = part == 0 ? Gm::kKChunks : Gm::kVChunks;
+            for (int ch = 0; ch < n_ch; ++ch, ++c) {
+              if (c % kProducers != me) continue;
+              const int s = c % S, use = c / S;
+              if (use >= 1 && !wait(&bar_kv_empty[s], (uint32_t)((use - 1) & 1))) {
+                ok = false;
+                break;
+              }
+              const uint32_t bytes = part == 0 ? C::kKBytes : C::kVBytes;
+              const long long off = part == 0 ? (long long)ch * C::kKBytes
+                                              : (long long)Gm::kKChunks * C::kKBytes + (long long)ch * C::kVBytes;
+              mbar_arrive_expect_tx(&bar_kv_full[s], bytes);
+              asm volatile(
+                  "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                      smem_addr(ring + s * C::kStageBytes)),
+                  "l"(img + (long long)t * Gm::kTileBytes + off), "r"(bytes), "r"(smem_addr(&bar_kv_full[s]))
+                  : "memory");
+            }
+          }
+        }
+        // no copy of this thread may still be landing when the CTA ends
+        for (int i = c > S ? c - S : 0; i < c; ++i)
+          if (i % kProducers == me) wait(&bar_kv_full[i % S], (uint32_t)((i / S) & 1));
+      }
+    } else if (warp == 1 && rank == 1) {
+      if (lane == 0)  // relay: chunk landed here -> issuers
+        for (int c = 0; c < Gm::kChunks * nt; ++c) {
+          if (!wait(&bar_kv_full[c % S], (uint32_t)((c / S) & 1))) break;
+          mbar_arrive_cluster(mapa_shared(smem_addr(&bar_kv_peer[c % S]), 0));
+        }
+    } else if (rank == 0 && lane == 0) {
+      // ---------------- MMA issuers: warp 1 S, warp 3 O ----------------
+      constexpr int nK = Gm::kKChunks, nKV = Gm::kChunks;
+      auto k_chunk0 = [&](int t) { return t == 0 ? 0 : nK + (t - 1) * nKV; };
+      auto v_chunk0 = [&](int t) { return t + 1 < nt ? 2 * nK + t * nKV : nK + t * nKV; };
+      auto chunk_ready = [&](int c, uint32_t& off) -> bool {
+        const int s = c % S, use = c / S;
+        off = (uint32_t)(s * C::kStageBytes);
+        if (!wait(&bar_kv_full[s], (uint32_t)(use & 1))) return false;
+        if (CG == 2 && !wait(&bar_kv_peer[s], (uint32_t)(use & 1))) return false;
+        tc::fence_after_sync();
+        return true;
+      };
+      bool ok = true;
+      if (warp == 1) {
+        constexpr uint32_t id_s = tc::idesc_tf32(kPfBM * CG, kPfBN, false);
+        const uint64_t qlo_d = tc::sdesc_sw128(smem_addr(qlo), 16, 1024);
+        const uint64_t k_d = tc::sdesc_sw128(smem_addr(ring), 16, 1024);
+        ok = wait(&bar_q_ready, 0);
+        tc::fence_after_sync();
+        for (int t = 0; ok && t < nt; ++t) {
+          if (t >= 1) {
+            if (!(ok = wait(&bar_s_free, (uint32_t)((t - 1) & 1)))) break;
+            tc::fence_after_sync();
+          }
+          uint32_t off[nK];
+#pragma unroll
+          for (int ch = 0; ch < nK; ++ch) {  // the small products
+            if (!(ok = chunk_ready(k_chunk0(t) + ch, off[ch]))) break;
+            const uint64_t kh = desc_add(k_d, off[ch]), kl = desc_add(k_d, off[ch] + C::kStageBytes / 2);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+              tc::mma_tf32_ts_g<CG>(T_S, T_QHI + ch * 32 + kk * 8, desc_add(kl, kk * 32), id_s, ch > 0 || kk > 0);
+              tc::mma_tf32_ss_g<CG>(T_S, desc_add(qlo_d, ch * 16384 + kk * 32), desc_add(kh, kk * 32), id_s, true);
+            }
+          }
+          if (!ok) break;
+#pragma unroll
+          for (int ch = 0; ch < nK; ++ch) {  // hi * hi
+            const uint64_t kh = desc_add(k_d, off[ch]);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              tc::mma_tf32_ts_g<CG>(T_S, T_QHI + ch * 32 + kk * 8, desc_add(kh, kk * 32), id_s, true);
+            commit_all(&bar_kv_empty[(k_chunk0(t) + ch) % S]);
+          }
+          commit_all(&bar_s_full);
+        }
+        tc::commit_g<CG>(smem_addr(&bar_mma_idle[0]));
+        wait(&bar_mma_idle[0], 0);
+      } else {
+        constexpr uint32_t id_o = tc::idesc_tf32(kPfBM * CG, HD, true);
+        const uint64_t v_d = sdesc_mn_sw128_32b(smem_addr(ring));
+        for (int t = 0; ok && t < nt; ++t) {
+#pragma unroll 1
+          for (int qq = 0; ok && qq < Gm::kVChunks; ++qq) {
+            const int c = v_chunk0(t) + qq, slot = qq & 1;
+            uint32_t off;
+            if (!(ok = chunk_ready(c, off))) break;
+            if (!(ok = wait(&bar_p_full[slot], (uint32_t)((qq >> 1) & 1)))) break;
+            // a new partial sum every 64 keys: the one before has been taken
+            const int half = 2 * t + (qq >> 1);
+            if (slot == 0 && half >= 1 && !(ok = wait(&bar_o_free, (uint32_t)((half - 1) & 1)))) break;
+            tc::fence_after_sync();
+            const uint64_t vh = desc_add(v_d, off), vl = desc_add(v_d, off + C::kVBytes / 2);
+            const uint32_t p_hi = T_P + slot * 64, p_lo = p_hi + 32;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+              tc::mma_tf32_ts_g<CG>(T_O, p_hi + ks * 8, desc_add(vl, ks * 1024), id_o, slot > 0 || ks > 0);
+              tc::mma_tf32_ts_g<CG>(T_O, p_lo + ks * 8, desc_add(vh, ks * 1024), id_o, true);
+            }
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) tc::mma_tf32_ts_g<CG>(T_O, p_hi + ks * 8, desc_add(vh, ks * 1024), id_o, true);
+            commit_all(&bar_kv_empty[c % S]);
+            commit_all(&bar_p_free[slot]);
+            if (slot == 1) commit_all(&bar_o_full);
+          }
+        }
+        tc::commit_g<CG>(smem_addr(&bar_mma_idle[1]));
+        wait(&bar_mma_idle[1], 0);
+      }
+    }
+  } else if (warp < 8) {
+    // ---------------- softmax: thread = row ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    {
+      const float4* src = reinterpret_cast<const float4*>(a.q + (long long)(u.q_row0 + tok) * a.q_stride + (long long)head * HD);
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        float hi[32], lo[32];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 t = src[c * 8 + i];
+          hi[4 * i] = pg_tf32(t.x), lo[4 * i] = t.x - hi[4 * i];
+          hi[4 * i + 1] = pg_tf32(t.y), lo[4 * i + 1] = t.y - hi[4 * i + 1];
+          hi[4 * i + 2] = pg_tf32(t.z), lo[4 * i + 2] = t.z - hi[4 * i + 2];
+          hi[4 * i + 3] = pg_tf32(t.w), lo[4 * i + 3] = t.w - hi[4 * i + 3];
+        }
+        tc::st32(T_QHI + lb + c * 32, hi);
+        unsigned char* rp = qlo + c * 16384 + row * 128;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<float4*>(rp + ((i ^ (row & 7)) << 4)) = make_float4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+      }
+      tc::wait_st();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) arrive_issuer(&bar_q_ready);
+    }
+    float m = -INFINITY, lsum = 0.f;
+    bool ok = true;
+    for (int j = 0; j < nt; ++j) {
+      ok = __all_sync(0xffffffffu, wait(&bar_s_full, (uint32_t)(j & 1)));
+      if (!ok) break;
+      tc::fence_after_sync();
+      float sv[kPfBN];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float t[32];
+        tc::ld32(T_S + lb + c * 32, t);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) sv[c * 32 + i] = t[i];
+      }
+      tc::wait_ld();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) arrive_issuer(&bar_s_free);
+      const int key0 = (u.tile0 + j) * kPfBN;
+      const bool full = __all_sync(0xffffffffu, key0 >= kmin && key0 + kPfBN - 1 <= qpos);
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < kPfBN; ++c) {
+        sv[c] *= a.scale_log2;
+        if (!full && (key0 + c > qpos || key0 + c < kmin)) sv[c] = -INFINITY;
+        mx[c & 3] = fmaxf(mx[c & 3], sv[c]);
+      }
+      const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+      const float base = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = fast_exp2(m - base);
+      m = m_new;
+      s_alpha[j & 1][row] = alpha;
+      lsum *= alpha;
+#pragma unroll
+      for (int qq = 0; qq < 4; ++qq) {
+        const int slot = qq & 1;
+        if (j >= 1 || qq >= 2) {
+          // the slot's quarter before has been multiplied: p_free[slot] number 2 j + qq / 2 - 1
+          ok = __all_sync(0xffffffffu, wait(&bar_p_free[slot], (uint32_t)((qq >> 1) ^ 1)));
+          if (!ok) break;
+          tc::fence_after_sync();
+        }
+        float ph[32], pl[32], ls = 0.f;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float p = fast_exp2(sv[qq * 32 + c] - base);
+          ls += p;
+          ph[c] = pg_tf32(p);
+          pl[c] = p - ph[c];
+        }
+        lsum += ls;
+        tc::st32(T_P + lb + slot * 64, ph);
+        tc::st32(T_P + lb + slot * 64 + 32, pl);
+        tc::wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) arrive_issuer(&bar_p_full[slot]);
+      }
+      if (!ok) break;
+    }
+    s_m[row] = m;
+    s_l[row] = lsum;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bar_sm_done);
+  } else {
+    // ---------------- O: thread = row ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    float acc[HD];
+#pragma unroll
+    for (int i = 0; i < HD; ++i) acc[i] = 0.f;
+    bool ok = true;
+    for (int x = 0; ok && x < 2 * nt; ++x) {
+      ok = __all_sync(0xffffffffu, wait(&bar_o_full, (uint32_t)(x & 1)));
+      if (!ok) break;
+      tc::fence_after_sync();
+      const float f = x & 1 ? 1.f : s_alpha[(x >> 1) & 1][row];
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        float ov[32];
+        tc::ld32(T_O + lb + c * 32, ov);
+        tc::wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(acc[c * 32 + i], f, ov[i]);
+      }
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) arrive_issuer(&bar_o_free);
+    }
+    if (ok) ok = __all_sync(0xffffffffu, wait(&bar_sm_done, 0));
+    if (ok) {
+      // values of V that are not finite, to the rows that attend to them
+      const int* flags = a.flags + img_slot;
+      for (int t = 0; t < nt; ++t) {
+        if (flags[t] == 0) continue;
+        const int key0 = (u.tile0 + t) * kPfBN;
+        for (int key = max(kmin, key0); key <= min(qpos, key0 + kPfBN - 1); ++key) {
+          const float* v = a.storage + a.v_off + (long long)table[key >> a.shift] * a.page_elems +
+                           ((long long)u.kvh << a.shift) * HD + (long long)(key & ((1 << a.shift) - 1)) * HD;
+#pragma unroll
+          for (int i = 0; i < HD; ++i) {
+            const float y = v[i];
+            if (!pg_finite(y)) acc[i] += y;
+          }
+        }
+      }
+      const float lsum = s_l[row];
+      const bool split = u.n_parts > 1;
+      if (!split) {
+        const float inv = 1.f / lsum;
+        float* dst = a.out + (long long)(u.q_row0 + tok) * a.out_stride + (long long)head * HD;
+        if (valid)
+#pragma unroll
+          for (int i = 0; i < HD; i += 4)
+            *reinterpret_cast<float4*>(dst + i) = make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
+      } else {
+        const long long ws_row = (long long)(u.slot + u.part) * (CG * 128) + rr;
+        if (valid) {
+#pragma unroll
+          for (int i = 0; i < HD; i += 4)
+            *reinterpret_cast<float4*>(a.ws_o + ws_row * HD + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+          *reinterpret_cast<float2*>(a.ws_ml + ws_row * 2) = make_float2(s_m[row], lsum);
+        }
+        __threadfence();
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if ((tid & 127) == 0) s_last = atomicAdd(a.tickets + u.ticket * 2 + rank, 1u) == (unsigned)u.n_parts - 1;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (s_last) {
+          __threadfence();
+          if ((tid & 127) == 0) a.tickets[u.ticket * 2 + rank] = 0;
+          for (int x = (warp & 3); x < 128 && (int)rank * 128 + x < u.n_rows; x += 4) {
+            const int q = u.r0 + (int)rank * 128 + x;
+            float* dst = a.out + (long long)(u.q_row0 + q / a.G) * a.out_stride + (long long)(u.kvh * a.G + q % a.G) * HD +
+                         lane * (HD / 32);
+            pg_merge_row<HD>(a.ws_o, a.ws_ml, u.slot, CG * 128, (int)rank * 128 + x, u.n_parts, lane,
+                             [&](const float (&o)[HD / 32]) {
+#pragma unroll
+                               for (int i = 0; i < HD / 32; i += 2) *reinterpret_cast<float2*>(dst + i) = make_float2(o[i], o[i + 1]);
+                             });
+          }
+        }
+      }
+    }
+  }
+  tc::fence_before_sync();
+  if constexpr (CG == 2)
+    cluster_sync_all();
+  else
+    __syncthreads();
+  if (warp == 0) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc_g<CG>(tm, 512);
+  }
+}
+
+}  // namespace l3p

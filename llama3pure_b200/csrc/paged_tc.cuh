@@ -28,7 +28,7 @@
 // taken out and added in the epilogue to the rows that attend to them); warps
 // 4-7 and 8-11 are the softmax of Q tile 0 and 1.
 //
-// Long key ranges with few rows are cut into parts (plan_tc_bf16); the part that
+// Long key ranges with few rows are cut into parts (plan_tc); the part that
 // ends last merges them in part order.
 #pragma once
 #include <cuda.h>
