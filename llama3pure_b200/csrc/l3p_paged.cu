@@ -126,15 +126,23 @@ struct BatchSeq {
 // First key that the token at `pos` attends to.
 int first_key(const Ctx* ctx, bool win, int pos) { return win ? std::max(0, pos - ctx->cfg.swa_window + 1) : 0; }
 
-// Row kernel: the tiles of all units (sequence, KV head, block of 8*nt rows)
-// laid end to end and cut into equal runs, one per CTA, so that every CTA
-// streams the same number of key tiles whatever the lengths are.  A run is a
-// multiple of the CTA's warps, which take its tiles in turn.
+// Row kernel: units are (sequence, KV head, block of 8*nt rows), their cost the
+// 16-key tiles they read.  Two ways to share them out:
+//   laid end to end and cut into equal runs, one per CTA: every SM streams the
+//     same number of tiles, but a CTA may begin, end and merge several units;
+//   every unit cut into equal parts on CTAs of its own (with no more units than
+//     CTAs): one segment per CTA, the longest part sets the time.
+// A run or part is a multiple of the CTA's warps, which take its tiles in turn,
+// so both are counted in rounds of one tile per warp.  A further segment of a CTA
+// costs about kSegRounds rounds that its prefetched tiles do not hide (16
+// sequences x 2 tokens x 3000 keys, 8B heads: 46.8 us end to end, 39.5 us by units).
+constexpr double kSegRounds = 1.5;
 void plan_rows(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, int nt, std::vector<int>* first,
                std::vector<PgSeg>* segs) {
   const int limit = row_limit(ctx), rt = 8 * nt, warps = row_warps(ctx), G = ctx->G;
   std::vector<PgSeg> units;
   long long total = 0;
+  int longest = 0;
   for (const auto& b : bs) {
     const long long rows = (long long)b.n_new * G;
     if (rows == 0 || rows > limit) continue;
@@ -153,16 +161,54 @@ void plan_rows(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, int nt
         u.tile0 = u.key_lo / kPgTile;
         u.tile1 = (u.key_hi + kPgTile - 1) / kPgTile;
         total += u.tile1 - u.tile0;
+        longest = std::max(longest, u.tile1 - u.tile0);
         units.push_back(u);
       }
   }
   if (units.empty()) return;
-  const long long max_ctas = std::min(ctx->num_sms, kPgMaxCtas);
-  long long run = (total + max_ctas - 1) / max_ctas;
-  run = (run + warps - 1) / warps * warps;
+  const int max_ctas = std::min(ctx->num_sms, kPgMaxCtas);
+  auto rounds = [&](long long tiles) { return (tiles + warps - 1) / warps; };
+  const long long run = rounds((total + max_ctas - 1) / max_ctas) * warps;
+  long long part = 0;  // tiles of a part at most, when every CTA has one
+  if ((int)units.size() <= max_ctas) {
+    auto ctas = [&](long long r) {
+      long long n = 0;
+      for (const auto& u : units) n += (u.tile1 - u.tile0 + r * warps - 1) / (r * warps);
+      return n;
+    };
+    long long lo = std::max<long long>(1, run / warps), hi = rounds(longest);  // rounds; ctas(hi) is the number of units
+    while (lo < hi) {
+      const long long mid = (lo + hi) / 2;
+      if (ctas(mid) <= max_ctas)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    const double more = std::ceil((double)units.size() * run / total);  // segments of a CTA behind its first, end to end
+    if (hi <= run / warps + kSegRounds * more) part = hi * warps;
+  }
+  first->assign(1, 0);
+  if (part > 0) {
+    int cta = 0;
+    for (const auto& u : units) {
+      const int n = u.tile1 - u.tile0, k = (int)((n + part - 1) / part);
+      const long long each = rounds((n + k - 1) / k) * warps;
+      for (int i = 0; i < k; ++i) {
+        PgSeg g = u;
+        g.tile0 = (int)std::min<long long>(u.tile1, u.tile0 + i * each);
+        g.tile1 = (int)std::min<long long>(u.tile1, g.tile0 + each);
+        g.part = i;
+        g.n_parts = k;
+        g.cta0 = cta;
+        segs->push_back(g);
+        first->push_back((int)segs->size());
+      }
+      cta += k;
+    }
+    return;
+  }
   const int n_cta = (int)((total + run - 1) / run);
   long long at = 0;  // tiles laid so far
-  first->assign(1, 0);
   for (auto& u : units) {
     const int n = u.tile1 - u.tile0, t_begin = u.tile0, t_end = u.tile1;
     const int c0 = (int)(at / run), c1 = (int)((at + n - 1) / run);
@@ -185,11 +231,11 @@ void plan_rows(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, int nt
 }
 
 // Tensor-core kernels: units (sequence, KV head, block of rows); with too few
-// of them for the GPU, long key ranges are cut into parts of equal size, merged
-// by the part that ends last.  Longest parts first.  fp32 pools: also the list
-// of the key tiles that the units read.
+// of them for the GPU, long key ranges are cut into parts of equal size, which a
+// second kernel merges.  Longest parts first.  fp32 pools: also the list of the
+// key tiles that the units read.
 void plan_tc(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vector<PgPart>* parts,
-             std::vector<PgPrep>* prep) {
+             std::vector<PgPart>* merges, std::vector<PgPrep>* prep) {
   const int limit = row_limit(ctx), tile = ctx->bf16 ? tc_tile(ctx) : 128, G = ctx->G;
   const int rt = ctx->bf16 ? tc_rows(ctx) : f32_rows(ctx);
   // CTAs (or CTA pairs) that run at once
@@ -223,9 +269,9 @@ void plan_tc(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vec
         units.push_back(u);
       }
   }
-  // no part is shorter than 4 tiles: below that the merge costs more than the split saves
-  const int cap = (int)std::max<long long>(4, (total + wide - 1) / wide);
-  int ticket = 0, slot = 0;
+  // no part is shorter than 8 tiles: below that the merge's launch costs more than the split saves
+  const int cap = (int)std::max<long long>(8, (total + wide - 1) / wide);
+  int slot = 0;
   for (const auto& u : units) {
     const int n = u.tile1 - u.tile0, k = (n + cap - 1) / cap;
     for (int i = 0; i < k; ++i) {
@@ -234,12 +280,14 @@ void plan_tc(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vec
       p.tile1 = u.tile0 + (int)((long long)n * (i + 1) / k);
       p.part = i;
       p.n_parts = k;
-      p.ticket = ticket;
       p.slot = slot;  // of part 0
       parts->push_back(p);
     }
     if (k > 1) {
-      ++ticket;
+      PgPart m = u;
+      m.n_parts = k;
+      m.slot = slot;
+      merges->push_back(m);
       slot += k;
     }
   }
@@ -270,16 +318,18 @@ void build_batch(const Ctx* ctx, const std::vector<BatchSeq>& bs, const int* seq
   for (int v = 0; v < (ctx->swa ? 2 : 1); ++v) {
     std::vector<int> first;
     std::vector<PgSeg> segs;
-    std::vector<PgPart> parts;
+    std::vector<PgPart> parts, merges;
     std::vector<PgPrep> prep;
     plan_rows(ctx, v == 1, bs, h.row_nt, &first, &segs);
-    plan_tc(ctx, v == 1, bs, &parts, &prep);
+    plan_tc(ctx, v == 1, bs, &parts, &merges, &prep);
     PgLists& l = h.lists[v];
     l.row_ctas = first.empty() ? 0 : (int)first.size() - 1;
     l.row_first = add(first.data(), first.size() * 4);
     l.row_segs = add(segs.data(), segs.size() * sizeof(PgSeg));
     l.n_tc = (int)parts.size();
     l.tc_parts = add(parts.data(), parts.size() * sizeof(PgPart));
+    l.n_merge = (int)merges.size();
+    l.merges = add(merges.data(), merges.size() * sizeof(PgPart));
     l.n_prep = (int)prep.size();
     l.prep = add(prep.data(), prep.size() * sizeof(PgPrep));
   }
@@ -315,7 +365,7 @@ size_t batch_capacity(const Ctx* ctx) {
   const size_t lists = (units + 2 * kPgMaxCtas + 8) * 16 + kPgMaxCtas + 8;
   const size_t tiles = ctx->bf16 ? 0 : (size_t)c.max_seqs * ((max_len + 127) / 128 + 1) * 4;
   const size_t table = (size_t)c.max_seqs * ((max_len + c.page_size - 1) / c.page_size);
-  return kPgHdrWords + 2 * (lists + lists + tiles) + 2 * (size_t)c.max_tokens + table + 64;
+  return kPgHdrWords + 2 * (lists + lists + lists + tiles) + 2 * (size_t)c.max_tokens + table + 64;
 }
 
 void release(Ctx* ctx) {
@@ -331,7 +381,6 @@ void release(Ctx* ctx) {
   cudaFree(ctx->tickets);
   cudaFree(ctx->tc_o);
   cudaFree(ctx->tc_ml);
-  cudaFree(ctx->tc_tickets);
   cudaFree(ctx->img);
   cudaFree(ctx->v_flags);
   if (ctx->rope_tab_swa != ctx->rope_tab) cudaFree(ctx->rope_tab_swa);

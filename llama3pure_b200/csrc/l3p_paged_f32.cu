@@ -22,12 +22,10 @@ int init_f32(l3p_paged_ctx* ctx) {
     PG_CUDA(ctx, cudaFuncSetAttribute(paged_f32_kernel<2, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, PgF32Cfg<2, 128>::kSmem));
   const size_t rows = 2 * (size_t)ctx->num_sms * f32_rows(ctx);  // as in init_tc
   if (cudaMalloc(&ctx->tc_o, rows * ctx->hd * sizeof(float)) != cudaSuccess ||
-      cudaMalloc(&ctx->tc_ml, rows * 2 * sizeof(float)) != cudaSuccess ||
-      cudaMalloc(&ctx->tc_tickets, 2 * (size_t)ctx->num_sms * sizeof(unsigned)) != cudaSuccess) {
+      cudaMalloc(&ctx->tc_ml, rows * 2 * sizeof(float)) != cudaSuccess) {
     cudaGetLastError();
     return fail(ctx, L3P_E_NOMEM, "the split workspace does not fit on the device");
   }
-  PG_CUDA(ctx, cudaMemset(ctx->tc_tickets, 0, 2 * (size_t)ctx->num_sms * sizeof(unsigned)));
   return L3P_OK;
 }
 
@@ -56,7 +54,7 @@ static int ensure_images(l3p_paged_ctx* ctx, size_t floats, size_t n, cudaStream
 }
 
 template <int CG, int HD>
-static int launch(l3p_paged_ctx* ctx, PgF32Args a, const PgLists& l, cudaStream_t s) {
+static int chunks(l3p_paged_ctx* ctx, PgF32Args a, const PgLists& l, cudaStream_t s) {
   const size_t tile = PfGeom<HD>::kTileFloats;
   const int n_kv = ctx->cfg.n_kv_heads;
   const size_t fit = std::max<size_t>(1, kImageBytes / (tile * sizeof(float) * l.n_prep));
@@ -68,23 +66,8 @@ static int launch(l3p_paged_ctx* ctx, PgF32Args a, const PgLists& l, cudaStream_
   for (int h = 0; h < n_kv; h += group) {
     a.kvh0 = h;
     a.n_kvh = std::min(group, n_kv - h);
-    paged_prep_kernel<CG, HD><<<dim3(l.n_prep, a.n_kvh), 256, 0, s>>>(a);
-    ++ctx->launches;
-    PG_CUDA(ctx, cudaGetLastError());
-    cudaLaunchConfig_t lc{};
-    lc.gridDim = dim3(l.n_tc * CG, 1, 1);
-    lc.blockDim = dim3(384, 1, 1);
-    lc.dynamicSmemBytes = PgF32Cfg<CG, HD>::kSmem;
-    lc.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    lc.attrs = attr;
-    lc.numAttrs = CG == 2 ? 1 : 0;
-    PG_CUDA(ctx, cudaLaunchKernelEx(&lc, paged_f32_kernel<CG, HD>, a));
-    ++ctx->launches;
+    if (int rc = launch(ctx, paged_prep_kernel<CG, HD>, dim3(l.n_prep, a.n_kvh), 256, 0, s, 1, a)) return rc;
+    if (int rc = launch(ctx, paged_f32_kernel<CG, HD>, dim3(l.n_tc * CG), 384, PgF32Cfg<CG, HD>::kSmem, s, CG, a)) return rc;
   }
   return L3P_OK;
 }
@@ -105,15 +88,13 @@ int launch_f32(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void*
   a.G = ctx->G;
   a.win = win ? 1 : 0;
   a.window = ctx->cfg.swa_window;
-  a.n_tokens = ctx->hdr.n_tokens;
-  a.with_rows = l.row_ctas > 0;
-  a.n_prep = l.n_prep;
+  a.lim = limits(ctx, l);
   a.scale_log2 = ctx->scale * kLog2e;
   a.ws_o = ctx->tc_o;
   a.ws_ml = ctx->tc_ml;
-  a.tickets = ctx->tc_tickets;
   a.err = ctx->err_dev;
-  return ctx->hd == 64 ? launch<1, 64>(ctx, a, l, s) : launch<2, 128>(ctx, a, l, s);
+  if (int rc = ctx->hd == 64 ? chunks<1, 64>(ctx, a, l, s) : chunks<2, 128>(ctx, a, l, s)) return rc;
+  return launch_merge(ctx, l, win, f32_rows(ctx), out, os, s);
 }
 
 }  // namespace l3p_pg

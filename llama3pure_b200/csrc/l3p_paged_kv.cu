@@ -71,18 +71,9 @@ PgKvArgs kv_args(l3p_paged_ctx* ctx, int layer) {
 }
 
 template <typename T>
-void launch_rope(l3p_paged_ctx* ctx, const PgKvArgs& a, int grid, cudaStream_t s) {
-  switch (ctx->hd) {
-    case 64:
-      paged_rope_kernel<T, 64><<<grid, kPgKvWarps * 32, 0, s>>>(a);
-      break;
-    case 128:
-      paged_rope_kernel<T, 128><<<grid, kPgKvWarps * 32, 0, s>>>(a);
-      break;
-    default:
-      paged_rope_kernel<T, 256><<<grid, kPgKvWarps * 32, 0, s>>>(a);
-      break;
-  }
+int launch_rope(l3p_paged_ctx* ctx, const PgKvArgs& a, int grid, cudaStream_t s) {
+  auto kernel = ctx->hd == 64 ? paged_rope_kernel<T, 64> : ctx->hd == 128 ? paged_rope_kernel<T, 128> : paged_rope_kernel<T, 256>;
+  return launch(ctx, kernel, dim3(grid), kPgKvWarps * 32, 0, s, 1, a);
 }
 
 int set_rope(l3p_paged_ctx* ctx, const l3p_paged_rope_config& in) {
@@ -243,13 +234,8 @@ L3P_API int l3p_paged_rope_append_dev(l3p_paged_ctx* ctx, int layer, const void*
   a.rows_per_warp = (long long)ctx->hdr.n_tokens * rows <= 64LL * ctx->num_sms * 4 ? 4 : 12;
   const long long items = (long long)ctx->hdr.n_tokens * ((rows + a.rows_per_warp - 1) / a.rows_per_warp);
   const int grid = (int)((items + kPgKvWarps - 1) / kPgKvWarps);
-  if (ctx->bf16)
-    launch_rope<__nv_bfloat16>(ctx, a, grid, static_cast<cudaStream_t>(stream));
-  else
-    launch_rope<float>(ctx, a, grid, static_cast<cudaStream_t>(stream));
-  ++ctx->launches;
-  PG_CUDA(ctx, cudaGetLastError());
-  return L3P_OK;
+  if (ctx->bf16) return launch_rope<__nv_bfloat16>(ctx, a, grid, static_cast<cudaStream_t>(stream));
+  return launch_rope<float>(ctx, a, grid, static_cast<cudaStream_t>(stream));
 }
 
 L3P_API int l3p_paged_append_dev(l3p_paged_ctx* ctx, int layer, const void* k, long long k_stride, const void* v,
@@ -266,10 +252,7 @@ L3P_API int l3p_paged_append_dev(l3p_paged_ctx* ctx, int layer, const void* k, l
   const int vecs = ctx->hd * ctx->es / 16;
   const long long n = (long long)ctx->hdr.n_tokens * 2 * ctx->cfg.n_kv_heads * vecs;
   const int grid = (int)std::min<long long>((n + 255) / 256, (long long)ctx->num_sms * 16);
-  paged_append_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(a, vecs, ctx->es);
-  ++ctx->launches;
-  PG_CUDA(ctx, cudaGetLastError());
-  return L3P_OK;
+  return launch(ctx, paged_append_kernel, dim3(grid), 256, 0, static_cast<cudaStream_t>(stream), 1, a, vecs, ctx->es);
 }
 
 // Checked here with the other row arguments; the kernels are launched by path.

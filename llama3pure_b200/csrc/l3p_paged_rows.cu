@@ -79,8 +79,7 @@ int launch_rows(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void
   a.G = ctx->G;
   a.win = win ? 1 : 0;
   a.window = ctx->cfg.swa_window;
-  a.n_tokens = ctx->hdr.n_tokens;
-  a.with_tc = l.n_tc > 0;
+  a.lim = limits(ctx, l);
   a.scale_log2 = ctx->scale * kLog2e;
   a.ws_o = ctx->ws_o;
   a.ws_ml = ctx->ws_ml;
@@ -88,12 +87,8 @@ int launch_rows(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void
   a.err = ctx->err_dev;
   // a captured launch may meet a batch that uses more CTAs
   const int grid = capturing(s) ? ctx->num_sms : l.row_ctas;
-  return with_kernel(ctx, ctx->hdr.row_nt, [&](auto kernel, int threads, int smem) {
-    kernel<<<grid, threads, smem, s>>>(a);
-    ++ctx->launches;
-    PG_CUDA(ctx, cudaGetLastError());
-    return (int)L3P_OK;
-  });
+  return with_kernel(ctx, ctx->hdr.row_nt,
+                     [&](auto kernel, int threads, int smem) { return launch(ctx, kernel, dim3(grid), threads, smem, s, 1, a); });
 }
 
 }  // namespace l3p_pg

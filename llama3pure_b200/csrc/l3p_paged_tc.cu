@@ -46,12 +46,10 @@ int init_tc(l3p_paged_ctx* ctx) {
   // 1 + its share parts: fewer than 2 num_sms parts of fewer than num_sms units
   const size_t rows_ws = 2 * (size_t)ctx->num_sms * tc_rows(ctx);
   if (cudaMalloc(&ctx->tc_o, rows_ws * ctx->hd * sizeof(float)) != cudaSuccess ||
-      cudaMalloc(&ctx->tc_ml, rows_ws * 2 * sizeof(float)) != cudaSuccess ||
-      cudaMalloc(&ctx->tc_tickets, 2 * (size_t)ctx->num_sms * sizeof(unsigned)) != cudaSuccess) {
+      cudaMalloc(&ctx->tc_ml, rows_ws * 2 * sizeof(float)) != cudaSuccess) {
     cudaGetLastError();
     return fail(ctx, L3P_E_NOMEM, "the split workspace does not fit on the device");
   }
-  PG_CUDA(ctx, cudaMemset(ctx->tc_tickets, 0, 2 * (size_t)ctx->num_sms * sizeof(unsigned)));
   return L3P_OK;
 }
 
@@ -74,21 +72,33 @@ int launch_tc(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void* 
   a.G = ctx->G;
   a.win = win ? 1 : 0;
   a.window = c.swa_window;
-  a.n_tokens = ctx->hdr.n_tokens;
-  a.with_rows = l.row_ctas > 0;
+  a.lim = limits(ctx, l);
   a.scale_log2 = ctx->scale * kLog2e;
   a.ws_o = ctx->tc_o;
   a.ws_ml = ctx->tc_ml;
-  a.tickets = ctx->tc_tickets;
   a.err = ctx->err_dev;
   CUtensorMap map;
   memcpy(&map, ctx->tmap, sizeof map);
-  return with_kernel(ctx, [&](auto kernel, int threads, int smem) {
-    kernel<<<l.n_tc, threads, smem, s>>>(a, map);
-    ++ctx->launches;
-    PG_CUDA(ctx, cudaGetLastError());
-    return (int)L3P_OK;
-  });
+  if (int rc = with_kernel(ctx, [&](auto kernel, int threads, int smem) {
+        return launch(ctx, kernel, dim3(l.n_tc), threads, smem, s, 1, a, map);
+      }))
+    return rc;
+  return launch_merge(ctx, l, win, tc_rows(ctx), out, os, s);
+}
+
+template <typename T, int HD>
+static int merge(l3p_paged_ctx* ctx, const PgLists& l, bool win, int rows, void* out, long long os, cudaStream_t s) {
+  return launch(ctx, paged_merge_kernel<T, HD>, dim3(l.n_merge, rows / 8), 256, 0, s, 1, (const int*)ctx->batch, win ? 1 : 0,
+                limits(ctx, l), rows, (const float*)ctx->tc_o, (const float*)ctx->tc_ml, static_cast<T*>(out), os, ctx->G);
+}
+
+int launch_merge(l3p_paged_ctx* ctx, const PgLists& l, bool win, int rows, void* out, long long os, cudaStream_t s) {
+  if (l.n_merge == 0) return L3P_OK;
+  if (ctx->bf16)
+    return ctx->hd == 64    ? merge<__nv_bfloat16, 64>(ctx, l, win, rows, out, os, s)
+           : ctx->hd == 128 ? merge<__nv_bfloat16, 128>(ctx, l, win, rows, out, os, s)
+                            : merge<__nv_bfloat16, 256>(ctx, l, win, rows, out, os, s);
+  return ctx->hd == 64 ? merge<float, 64>(ctx, l, win, rows, out, os, s) : merge<float, 128>(ctx, l, win, rows, out, os, s);
 }
 
 }  // namespace l3p_pg

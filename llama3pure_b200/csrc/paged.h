@@ -30,9 +30,10 @@ struct PgLists {
   int row_segs;    // word offset: PgSeg[]
   int n_tc;        // parts of the tensor-core kernels (0: none)
   int tc_parts;    // word offset: PgPart[]
+  int n_merge;     // units that are cut into parts
+  int merges;      // word offset: PgPart[], one for each of them
   int n_prep;      // fp32 pools: key tiles to split
   int prep;        // word offset: PgPrep[]
-  int pad;
 };
 struct PgHeader {
   int n_tokens, n_seqs, row_nt, tok;  // tok: word offset of int2[n_tokens] (storage row, position)
@@ -40,7 +41,7 @@ struct PgHeader {
   int pad[3];
   PgLists lists[2];
 };
-constexpr int kPgHdrWords = 32;
+constexpr int kPgHdrWords = 64;
 static_assert(sizeof(PgHeader) <= kPgHdrWords * 4, "batch header");
 
 // Keys [tile0*16, tile1*16) of the rows r0 .. r0+n_rows-1 of one sequence and
@@ -62,10 +63,22 @@ static_assert(sizeof(PgSeg) == 64, "segment");
 struct __align__(16) PgPart {
   int tbl, key_hi, tile0, tile1;
   int q_row0, pos0, r0, n_rows;
-  int kvh, part, n_parts, ticket;
-  int slot, img, pad[2];  // workspace slot of part 0; fp32 pools: image of tile 0
+  int kvh, part, n_parts, slot;
+  int img, pad[3];  // slot: workspace of part 0; img: image of tile 0 (fp32 pools)
 };
 static_assert(sizeof(PgPart) == 64, "part");
+
+// What a launch was made for: a batch that it meets when it is replayed must
+// not exceed it (fits), else nothing is written and the error word is set.
+struct PgLimits {
+  int n_tokens, n_tc, n_merge, n_prep, with_rows, with_tc;
+};
+#ifdef __CUDACC__
+__device__ __forceinline__ bool pg_fits(const PgHeader* h, const PgLists& l, const PgLimits& m) {
+  return h->n_tokens <= m.n_tokens && l.n_tc <= m.n_tc && l.n_merge <= m.n_merge && l.n_prep <= m.n_prep &&
+         (l.row_ctas != 0) == (m.with_rows != 0) && (l.n_tc != 0) == (m.with_tc != 0);
+}
+#endif
 
 struct PgPrep {
   int tbl, key0, key_hi, img;  // keys [key0, key0+128) below key_hi, to image tile img
@@ -118,7 +131,6 @@ struct l3p_paged_ctx {
   unsigned* tickets = nullptr;
   float* tc_o = nullptr;
   float* tc_ml = nullptr;
-  unsigned* tc_tickets = nullptr;
   // fp32 pools on the tensor cores: K/V tile images, flags of tiles with values that are not finite
   float* img = nullptr;
   size_t img_floats = 0;
@@ -193,6 +205,34 @@ inline bool windowed(const l3p_paged_ctx* ctx, int layer) {
   return ctx->swa && layer % ctx->cfg.swa_pattern < ctx->cfg.swa_pattern - 1;
 }
 
+// Launches a kernel that may start while the one before it on the stream ends:
+// every such kernel reads only the batch description (and cache rows of earlier
+// batches) ahead of its griddep_wait.
+template <typename... P, typename... A>
+int launch(l3p_paged_ctx* ctx, void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t s, int cluster, A... args) {
+  cudaLaunchConfig_t lc{};
+  lc.gridDim = grid;
+  lc.blockDim = dim3(threads, 1, 1);
+  lc.dynamicSmemBytes = smem;
+  lc.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  lc.attrs = attr;
+  lc.numAttrs = cluster > 1 ? 2 : 1;
+  PG_CUDA(ctx, cudaLaunchKernelEx(&lc, kernel, args...));
+  ++ctx->launches;
+  return L3P_OK;
+}
+
+inline l3p::PgLimits limits(const l3p_paged_ctx* ctx, const l3p::PgLists& l) {
+  return {ctx->hdr.n_tokens, l.n_tc, l.n_merge, l.n_prep, l.row_ctas > 0, l.n_tc > 0};
+}
+
 // Rows per KV head up to which a sequence takes the row kernel, and the key
 // tile of the tensor-core kernel (l3p_paged_rows.cu, l3p_paged_tc.cu).
 int row_limit(const l3p_paged_ctx* ctx);
@@ -210,6 +250,8 @@ int init_f32(l3p_paged_ctx* ctx);
 int launch_rows(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void* out, long long os, cudaStream_t s);
 int launch_tc(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void* out, long long os, cudaStream_t s);
 int launch_f32(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void* out, long long os, cudaStream_t s);
+// Joins the parts of the split units of the tensor-core kernels (l3p_paged_tc.cu).
+int launch_merge(l3p_paged_ctx* ctx, const l3p::PgLists& l, bool win, int rows, void* out, long long os, cudaStream_t s);
 // Copies rows of pages: jobs (source page, destination page, rows, 0) in device memory.
 int launch_page_copy(l3p_paged_ctx* ctx, int n_jobs, cudaStream_t s);
 

@@ -53,11 +53,10 @@ struct PgF32Args {
   int* flags;             // [head][n_prep]: the tile's V holds values that are not finite (0 in the image)
   int kvh0, n_kvh;        // group of KV heads of this launch
   int shift, G, win, window;
-  int n_tokens, with_rows, n_prep;
+  PgLimits lim;
   float scale_log2;
   float* ws_o;            // [slot][CG * 128][HD]
   float* ws_ml;
-  unsigned* tickets;
   int* err;
 };
 
@@ -70,10 +69,12 @@ __global__ void paged_prep_kernel(const PgF32Args a) {
   using Gm = PfGeom<HD>;
   const PgHeader* h = reinterpret_cast<const PgHeader*>(a.batch);
   const PgLists l = h->lists[a.win];
-  if ((int)blockIdx.x >= l.n_prep) return;
+  griddep_launch();
+  griddep_wait();  // the new rows come from the kernel before this one; the images are still read by it
+  if (!pg_fits(h, l, a.lim) || (int)blockIdx.x >= l.n_prep) return;
   const PgPrep p = reinterpret_cast<const PgPrep*>(a.batch + l.prep)[blockIdx.x];
   const int* table = a.batch + h->tbl + p.tbl;
-  const long long slot = (long long)blockIdx.y * a.n_prep + p.img;
+  const long long slot = (long long)blockIdx.y * a.lim.n_prep + p.img;
   unsigned char* base = reinterpret_cast<unsigned char*>(a.img) + slot * Gm::kTileBytes;
   const long long head = (long long)(a.kvh0 + blockIdx.y) * ((long long)HD << a.shift);
   constexpr int kVRows = HD / CG;
@@ -122,7 +123,6 @@ __global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
   constexpr int S = PgF32Cfg<CG, HD>::kStages;
   extern __shared__ unsigned char f32_smem_raw[];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_last;
   __shared__ float s_alpha[2][128], s_m[128], s_l[128];
   __shared__ __align__(8) uint64_t bar_kv_full[S], bar_kv_empty[S], bar_kv_peer[S];
   __shared__ __align__(8) uint64_t bar_s_full, bar_s_free, bar_p_full[2], bar_p_free[2];
@@ -130,20 +130,25 @@ __global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
 
   const PgHeader* hd = reinterpret_cast<const PgHeader*>(a.batch);
   const PgLists l = hd->lists[a.win];
-  if (hd->n_tokens > a.n_tokens || l.n_tc * CG > (int)gridDim.x || l.n_prep != a.n_prep || (l.row_ctas != 0) != (a.with_rows != 0)) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
+  griddep_launch();
+  const bool fits = pg_fits(hd, l, a.lim);
+  if (!fits || (int)blockIdx.x / CG >= l.n_tc) {
+    griddep_wait();
+    if (!fits && blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
     return;
   }
-  if ((int)blockIdx.x / CG >= l.n_tc) return;
   const PgPart u = reinterpret_cast<const PgPart*>(a.batch + l.tc_parts)[blockIdx.x / CG];
-  if (u.kvh < a.kvh0 || u.kvh >= a.kvh0 + a.n_kvh) return;  // both CTAs of a pair
+  if (u.kvh < a.kvh0 || u.kvh >= a.kvh0 + a.n_kvh) {  // both CTAs of a pair
+    griddep_wait();
+    return;
+  }
   const int* table = a.batch + hd->tbl + u.tbl;
   unsigned char* qlo = (unsigned char*)(((uintptr_t)f32_smem_raw + 1023) & ~(uintptr_t)1023);
   unsigned char* ring = qlo + Gm::kQloBytes;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
   const int nt = u.tile1 - u.tile0;
-  const long long img_slot = (long long)(u.kvh - a.kvh0) * a.n_prep + u.img + u.tile0;
+  const long long img_slot = (long long)(u.kvh - a.kvh0) * a.lim.n_prep + u.img + u.tile0;
 
   if (warp == 0) {
     tc::tmem_alloc_g<CG>(&s_tmem, 512);
@@ -175,6 +180,7 @@ __global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
     __syncthreads();
   tc::fence_after_sync();
   const uint32_t tm = s_tmem;
+  griddep_wait();  // the images and q come from the kernels before this one
   const uint32_t T_QHI = tm + 0, T_O = tm + HD, T_S = tm + 2 * HD, T_P = tm + 2 * HD + kPfBN;
 
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
@@ -476,24 +482,6 @@ __global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
           for (int i = 0; i < HD; i += 4)
             *reinterpret_cast<float4*>(a.ws_o + ws_row * HD + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
           *reinterpret_cast<float2*>(a.ws_ml + ws_row * 2) = make_float2(s_m[row], lsum);
-        }
-        __threadfence();
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if ((tid & 127) == 0) s_last = atomicAdd(a.tickets + u.ticket * 2 + rank, 1u) == (unsigned)u.n_parts - 1;
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (s_last) {
-          __threadfence();
-          if ((tid & 127) == 0) a.tickets[u.ticket * 2 + rank] = 0;
-          for (int x = (warp & 3); x < 128 && (int)rank * 128 + x < u.n_rows; x += 4) {
-            const int q = u.r0 + (int)rank * 128 + x;
-            float* dst = a.out + (long long)(u.q_row0 + q / a.G) * a.out_stride + (long long)(u.kvh * a.G + q % a.G) * HD +
-                         lane * (HD / 32);
-            pg_merge_row<HD>(a.ws_o, a.ws_ml, u.slot, CG * 128, (int)rank * 128 + x, u.n_parts, lane,
-                             [&](const float (&o)[HD / 32]) {
-#pragma unroll
-                               for (int i = 0; i < HD / 32; i += 2) *reinterpret_cast<float2*>(dst + i) = make_float2(o[i], o[i + 1]);
-                             });
-          }
         }
       }
     }

@@ -102,6 +102,8 @@ __global__ void __launch_bounds__(kPgKvWarps * 32) paged_rope_kernel(const PgKvA
   __shared__ __align__(16) float row_s[kPgKvWarps][HD];
   const PgHeader* h = reinterpret_cast<const PgHeader*>(a.batch);
   const int n_tok = h->n_tokens;
+  griddep_launch();
+  griddep_wait();  // the rows come from the kernel before this one
   if (n_tok > a.n_tokens) {  // a replay on a larger batch than the captured one
     if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
     return;
@@ -202,6 +204,8 @@ __global__ void __launch_bounds__(kPgKvWarps * 32) paged_rope_kernel(const PgKvA
 __global__ void paged_append_kernel(const PgKvArgs a, int vecs, int es) {
   const PgHeader* h = reinterpret_cast<const PgHeader*>(a.batch);
   const int n_tok = h->n_tokens;
+  griddep_launch();
+  griddep_wait();
   if (n_tok > a.n_tokens) {
     if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
     return;

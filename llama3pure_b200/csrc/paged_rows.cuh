@@ -46,7 +46,7 @@ struct PgRowArgs {
   const void* storage;  // the layer's K block of page 0, head 0
   long long page_elems, v_off;
   int shift, G, win, window;
-  int n_tokens, with_tc;  // of the launch: what a replay's batch must not exceed
+  PgLimits lim;
   float scale_log2;
   float* ws_o;       // [slot][8*NT][HD]
   float* ws_ml;      // [slot][8*NT][2]
@@ -157,11 +157,12 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
 
   const PgHeader* h = reinterpret_cast<const PgHeader*>(a.batch);
   const PgLists l = h->lists[a.win];
-  if (h->n_tokens > a.n_tokens || h->row_nt != NT || l.row_ctas > (int)gridDim.x || (l.n_tc != 0) != (a.with_tc != 0)) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
+  griddep_launch();
+  if (!pg_fits(h, l, a.lim) || h->row_nt != NT || l.row_ctas > (int)gridDim.x || (int)blockIdx.x >= l.row_ctas) {
+    griddep_wait();
+    if ((int)blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
     return;
   }
-  if ((int)blockIdx.x >= l.row_ctas) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int seg_end = a.batch[l.row_first + blockIdx.x + 1];
   const PgSeg* segs = reinterpret_cast<const PgSeg*>(a.batch + l.row_segs);
@@ -173,10 +174,10 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
   // ---- loads: tiles in the order they are used, across segments ----------------
   int is = a.batch[l.row_first + blockIdx.x];  // segment of the next tile to load
   const int seg0 = is;
-  int it = 0, ie = 0, ilo = 0, ihi = 0, itbl = 0, ikvh = 0, ipage = 0, islot = 0;
+  int it = 0, ie = 0, ilo = 0, ihi = 0, itbl = 0, ikvh = 0, ipos0 = 0, ipage = 0, islot = 0;
   auto load_seg = [&]() {
     const PgSeg& s = segs[is];
-    it = s.tile0 + warp, ie = s.tile1, ilo = s.key_lo, ihi = s.key_hi, itbl = s.tbl, ikvh = s.kvh;
+    it = s.tile0 + warp, ie = s.tile1, ilo = s.key_lo, ihi = s.key_hi, itbl = s.tbl, ikvh = s.kvh, ipos0 = s.pos0;
   };
   auto settle = [&]() {  // to the next tile of this warp, and its page
     while (is < seg_end && it >= ie)
@@ -206,8 +207,17 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
   };
   if (is < seg_end) load_seg();
   settle();
+  // Rows of earlier batches are there already; the new tokens' rows, and q, come from the kernel before this one.
+  bool waited = false;
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i) issue();
+  for (int i = 0; i < NS - 1; ++i) {
+    if (!waited && is < seg_end && (it + 1) * kPgTile > ipos0) {
+      griddep_wait();
+      waited = true;
+    }
+    issue();
+  }
+  if (!waited) griddep_wait();
 
   int cslot = 0;
   for (int si = seg0; si < seg_end; ++si) {
@@ -542,42 +552,77 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
       __syncthreads();
     }
     if (split) {
-      __threadfence();
       __syncthreads();
-      if (tid == 0) s_last = atomicAdd(a.tickets + cta0, 1u) == (unsigned)n_parts - 1;
+      if (tid == 0) {
+        __threadfence();  // the CTA's partial rows, ahead of its ticket
+        s_last = atomicAdd(a.tickets + cta0, 1u) == (unsigned)n_parts - 1;
+        __threadfence();
+      }
       __syncthreads();
       if (s_last) {
-        __threadfence();
         if (tid == 0) a.tickets[cta0] = 0;
-        // weights of the parts for every row: [row][part], then 1/L folded in
         auto part_slot = [&](int p) -> long long { return p == 0 ? 2 * cta0 + 1 : 2 * (cta0 + p); };
-        for (int row = warp; row < n_rows; row += NW) {
-          float M = -INFINITY, L = 0.f;
-          for (int p = lane; p < n_parts; p += 32) M = fmaxf(M, __ldcg(a.ws_ml + (part_slot(p) * 8 * NT + row) * 2));
+        // weights of the parts for every row, 1/L folded in: [row][part].  A warp's rows together, so that their loads overlap.
+        constexpr int RW = 8 * NT / NW;
+        float M[RW], L[RW];
 #pragma unroll
-          for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-          for (int p = lane; p < n_parts; p += 32) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.ws_ml + (part_slot(p) * 8 * NT + row) * 2));
-            const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
-            merge[row * n_parts + p] = w;
-            L += w * ml.y;
+        for (int i = 0; i < RW; ++i) M[i] = -INFINITY, L[i] = 0.f;
+        for (int p = lane; p < n_parts; p += 32) {
+          float2 ml[RW];
+#pragma unroll
+          for (int i = 0; i < RW; ++i)
+            ml[i] = __ldcg(reinterpret_cast<const float2*>(a.ws_ml + (part_slot(p) * 8 * NT + min(warp + i * NW, n_rows - 1)) * 2));
+#pragma unroll
+          for (int i = 0; i < RW; ++i) {
+            const float m1 = fmaxf(M[i], ml[i].x), base = m1 == -INFINITY ? 0.f : m1;
+            L[i] = L[i] * fast_exp2(M[i] - base) + ml[i].y * fast_exp2(ml[i].x - base);
+            M[i] = m1;
+            if (warp + i * NW < n_rows) merge[(warp + i * NW) * n_parts + p] = ml[i].x;
           }
+        }
 #pragma unroll
-          for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
-          const float inv = 1.f / L;
-          for (int p = lane; p < n_parts; p += 32) merge[row * n_parts + p] *= inv;
+        for (int i = 0; i < RW; ++i) {
+#pragma unroll
+          for (int x = 16; x > 0; x >>= 1) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, M[i], x), l2 = __shfl_xor_sync(0xffffffffu, L[i], x);
+            const float m1 = fmaxf(M[i], m2), base = m1 == -INFINITY ? 0.f : m1;
+            L[i] = L[i] * fast_exp2(M[i] - base) + l2 * fast_exp2(m2 - base);
+            M[i] = m1;
+          }
+          const float inv = 1.f / L[i], base = M[i] == -INFINITY ? 0.f : M[i];
+          if (warp + i * NW < n_rows)
+            for (int p = lane; p < n_parts; p += 32) {
+              float* w = merge + (warp + i * NW) * n_parts + p;
+              *w = fast_exp2(*w - base) * inv;
+            }
         }
         __syncthreads();
-        for (int x = tid; x < n_rows * (HD / 4); x += NW * 32) {
-          const int row = x / (HD / 4), d = (x % (HD / 4)) * 4;
-          float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-          for (int p = 0; p < n_parts; ++p) {
-            const float w = merge[row * n_parts + p];
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(a.ws_o + (part_slot(p) * 8 * NT + row) * HD + d));
-            s.x += w * v.x, s.y += w * v.y, s.z += w * v.z, s.w += w * v.w;
+        constexpr int U = 4;  // pieces of a thread in flight
+        const int pieces = n_rows * (HD / 4);
+        for (int x0 = tid; x0 < pieces; x0 += U * NW * 32) {
+          float4 s[U];
+          int row[U], d[U];
+#pragma unroll
+          for (int i = 0; i < U; ++i) {
+            const int x = min(x0 + i * NW * 32, pieces - 1);
+            row[i] = x / (HD / 4), d[i] = (x % (HD / 4)) * 4;
+            s[i] = make_float4(0.f, 0.f, 0.f, 0.f);
           }
-          store4(row, d, s);
+#pragma unroll 4
+          for (int p = 0; p < n_parts; ++p) {
+            const float* base = a.ws_o + part_slot(p) * 8 * NT * HD;
+            float4 v[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(base + row[i] * HD + d[i]));
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+              const float w = merge[row[i] * n_parts + p];
+              s[i].x += w * v[i].x, s[i].y += w * v[i].y, s[i].z += w * v[i].z, s[i].w += w * v[i].w;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < U; ++i)
+            if (x0 + i * NW * 32 < pieces) store4(row[i], d[i], s[i]);
         }
       }
       __syncthreads();  // the merge buffer is free again

@@ -28,8 +28,8 @@
 // taken out and added in the epilogue to the rows that attend to them); warps
 // 4-7 and 8-11 are the softmax of Q tile 0 and 1.
 //
-// Long key ranges with few rows are cut into parts (plan_tc); the part that
-// ends last merges them in part order.
+// Long key ranges with few rows are cut into parts (plan_tc), which
+// paged_merge_kernel joins.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -64,11 +64,10 @@ struct PgTcArgs {
   int row_k;       // storage row of (page 0, layer, K, head 0, slot 0)
   int page_rows;   // storage rows of a page
   int n_kv, shift, G, win, window;
-  int n_tokens, with_rows;
+  PgLimits lim;
   float scale_log2;
   float* ws_o;     // [slot][kNQ * 128][HD]
   float* ws_ml;    // [slot][kNQ * 128][2]
-  unsigned* tickets;
   int* err;
 };
 
@@ -113,40 +112,62 @@ __device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t (&v)[3
       : "memory");
 }
 
-// Merge of a split unit's rows by one warp: out row = sum_p w_p o_p / sum_p w_p l_p
-// with w_p = 2^(m_p - max m), in part order.  Lane holds HD/32 values.
-template <int HD, typename Store>
-__device__ __forceinline__ void pg_merge_row(const float* ws_o, const float* ws_ml, long long slot0, int rows, int row,
-                                             int n_parts, int lane, Store store) {
+// Joins the parts of split units: row = sum_p w_p o_p / sum_p w_p l_p with
+// w_p = 2^(m_p - max m), in part order.  One warp per row, a lane holds HD/32
+// values; a kernel of its own because the last of the parts' CTAs, alone on its SM,
+// took 50 us for what all SMs do in 3.  grid (units, rows / 8).
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) paged_merge_kernel(const int* batch, int win, PgLimits lim, int rows, const float* __restrict__ ws_o,
+                                                          const float* __restrict__ ws_ml, T* out, long long out_stride, int G) {
   constexpr int N = HD / 32;
+  const PgHeader* h = reinterpret_cast<const PgHeader*>(batch);
+  const PgLists& l = h->lists[win];
+  const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);
+  griddep_launch();
+  griddep_wait();
+  if (!pg_fits(h, l, lim) || (int)blockIdx.x >= l.n_merge) return;
+  const PgPart u = reinterpret_cast<const PgPart*>(batch + l.merges)[blockIdx.x];
+  if (row >= u.n_rows) return;
+  const float2* ml = reinterpret_cast<const float2*>(ws_ml) + (long long)u.slot * rows + row;
+  const float* o = ws_o + ((long long)u.slot * rows + row) * HD + lane * N;
   float M = -INFINITY;
-  for (int p = lane; p < n_parts; p += 32) M = fmaxf(M, __ldcg(ws_ml + ((slot0 + p) * rows + row) * 2));
+  for (int p = lane; p < u.n_parts; p += 32) M = fmaxf(M, __ldcg(ml + (long long)p * rows).x);
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+  const float base = M == -INFINITY ? 0.f : M;
   float acc[N], L = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int p = 0; p < n_parts; ++p) {
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(ws_ml + ((slot0 + p) * rows + row) * 2));
-    const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
-    L += w * ml.y;
-    const float* o = ws_o + ((slot0 + p) * rows + row) * HD + lane * N;
+#pragma unroll 8
+  for (int p = 0; p < u.n_parts; ++p) {
+    const float2 t = __ldcg(ml + (long long)p * rows);
+    const float* src = o + (long long)p * rows * HD;
+    float v[N];
     if constexpr (N == 2) {
-      const float2 t = __ldcg(reinterpret_cast<const float2*>(o));
-      acc[0] += w * t.x, acc[1] += w * t.y;
+      const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
+      v[0] = y.x, v[1] = y.y;
     } else {
 #pragma unroll
       for (int i = 0; i < N; i += 4) {
-        const float4 t = __ldcg(reinterpret_cast<const float4*>(o + i));
-        acc[i] += w * t.x, acc[i + 1] += w * t.y, acc[i + 2] += w * t.z, acc[i + 3] += w * t.w;
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(src + i));
+        v[i] = y.x, v[i + 1] = y.y, v[i + 2] = y.z, v[i + 3] = y.w;
       }
     }
+    const float w = fast_exp2(t.x - base);
+    L += w * t.y;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] += w * v[i];
   }
   const float inv = 1.f / L;
+  const int r = u.r0 + row;
+  T* dst = out + (long long)(u.q_row0 + r / G) * out_stride + (long long)(u.kvh * G + r % G) * HD + lane * N;
 #pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] *= inv;
-  store(acc);
+  for (int i = 0; i < N; i += 2) {
+    if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<uint32_t*>(dst + i) = pg_pack_bf16(acc[i] * inv, acc[i + 1] * inv);
+    else
+      *reinterpret_cast<float2*>(dst + i) = make_float2(acc[i] * inv, acc[i + 1] * inv);
+  }
 }
 
 template <int HD>
@@ -156,17 +177,18 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
   constexpr int S = C::kStages, TN = C::kTN, NQ = C::kNQ;
   extern __shared__ unsigned char tc_smem_raw[];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_bad, s_last[2];
+  __shared__ int s_bad;
   __shared__ __align__(8) uint64_t kv_full[S], kv_empty[S], v_ok[S];
   __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_done[2], q_ready[2], mma_idle;
 
   const PgHeader* h = reinterpret_cast<const PgHeader*>(a.batch);
   const PgLists l = h->lists[a.win];
-  if (h->n_tokens > a.n_tokens || l.n_tc > (int)gridDim.x || (l.row_ctas != 0) != (a.with_rows != 0)) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
+  griddep_launch();
+  if (!pg_fits(h, l, a.lim) || (int)blockIdx.x >= l.n_tc) {
+    griddep_wait();
+    if (!pg_fits(h, l, a.lim) && blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
     return;
   }
-  if ((int)blockIdx.x >= l.n_tc) return;
   const PgPart u = reinterpret_cast<const PgPart*>(a.batch + l.tc_parts)[blockIdx.x];
   const int* table = a.batch + h->tbl + u.tbl;
   unsigned char* sq = (unsigned char*)(((uintptr_t)tc_smem_raw + 1023) & ~(uintptr_t)1023);
@@ -202,6 +224,7 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tm = s_tmem;
+  griddep_wait();  // q and the new rows come from the kernel before this one
 
   if (warp == 0) {
     // ---------------- loads ----------------
@@ -482,26 +505,7 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
           }
         }
       }
-      if (split) {
-        if (valid) *reinterpret_cast<float2*>(a.ws_ml + ws_row * 2) = make_float2(m == -INFINITY ? m : m * asl, lsum);
-        __threadfence();
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + b) : "memory");
-        if ((tid & 127) == 0) s_last[b] = atomicAdd(a.tickets + u.ticket * 2 + b, 1u) == (unsigned)u.n_parts - 1;
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + b) : "memory");
-        if (s_last[b]) {
-          __threadfence();
-          if ((tid & 127) == 0) a.tickets[u.ticket * 2 + b] = 0;
-          for (int x = (warp & 3); x < 128 && b * 128 + x < u.n_rows; x += 4) {
-            const int q = u.r0 + b * 128 + x;
-            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (long long)(u.q_row0 + q / a.G) * a.out_stride +
-                                 (long long)(u.kvh * a.G + q % a.G) * HD + lane * (HD / 32);
-            pg_merge_row<HD>(a.ws_o, a.ws_ml, u.slot, NQ * 128, b * 128 + x, u.n_parts, lane, [&](const float (&acc)[HD / 32]) {
-#pragma unroll
-              for (int i = 0; i < HD / 32; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pg_pack_bf16(acc[i], acc[i + 1]);
-            });
-          }
-        }
-      }
+      if (split && valid) *reinterpret_cast<float2*>(a.ws_ml + ws_row * 2) = make_float2(m == -INFINITY ? m : m * asl, lsum);
     }
   }
   tc::fence_before_sync();

@@ -170,6 +170,11 @@ __device__ __forceinline__ bool ll_wait(const unsigned long long* p, long long s
   }
 }
 
+// ---- programmatic dependent launch: let the next kernel of the stream start,
+// wait until the one before has completed
+__device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float fast_exp2(float x) {

@@ -51,6 +51,9 @@ class PagedCache:
         self.dtype = torch.bfloat16 if dtype == "bf16" else torch.float32
         self.n_layers, self.n_heads, self.n_kv_heads, self.head_dim = n_layers, n_heads, n_kv_heads, head_dim
         self.device = device
+        # the handle of torch's current stream, without a Stream object around it where torch offers that
+        self._current_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                                       lambda d: torch.cuda.current_stream(d).cuda_stream)
         self.n_tokens = 0  # of the current batch
         self.h = None
         h = C.c_void_p()
@@ -90,7 +93,7 @@ class PagedCache:
 
     def _stream(self, stream) -> int:
         if stream is None:
-            stream = self.torch.cuda.current_stream(self.device)
+            return self._current_stream(self.device)
         return stream if isinstance(stream, int) else stream.cuda_stream
 
     def check(self, stream=None) -> None:
@@ -198,16 +201,19 @@ class PagedCache:
 
     def _rows(self, t, heads: int, name: str) -> tuple[int, int]:
         """Address and token stride of rows [n_tokens or more][heads][head_dim]."""
-        if not t.is_cuda or t.dtype != self.dtype or t.device.index != self.device:
+        if t.dtype != self.dtype or t.get_device() != self.device:
             raise TypeError(f"{name}: a {self.dtype} tensor on cuda:{self.device}, not {t.dtype} on {t.device}")
-        if t.dim() != 3 or t.shape[0] < self.n_tokens or t.shape[1] != heads or t.shape[2] != self.head_dim:
-            raise ValueError(f"{name}: shape {tuple(t.shape)}, not ({self.n_tokens}, {heads}, {self.head_dim})")
-        s = t.stride()
-        if s[2] != 1 or (heads > 1 and s[1] != self.head_dim):
+        shape = t.shape
+        if len(shape) != 3 or shape[0] < self.n_tokens or shape[1] != heads or shape[2] != self.head_dim:
+            raise ValueError(f"{name}: shape {tuple(shape)}, not ({self.n_tokens}, {heads}, {self.head_dim})")
+        stride, head, one = t.stride()
+        if one != 1 or (heads > 1 and head != self.head_dim):
             raise ValueError(f"{name}: the heads of a token are not dense")
-        if t.shape[0] > 1 and s[0] < heads * self.head_dim:
-            raise ValueError(f"{name}: tokens {s[0]} values apart, rows of {heads * self.head_dim}")
-        return t.data_ptr(), s[0] if t.shape[0] > 1 else 0
+        if shape[0] < 2:
+            stride = 0
+        elif stride < heads * self.head_dim:
+            raise ValueError(f"{name}: tokens {stride} values apart, rows of {heads * self.head_dim}")
+        return t.data_ptr(), stride
 
     def rope_append_dev(self, layer, q, k, v, q_out, stream=None) -> None:
         """Rotates the batch's q (into q_out, which may be q) and k rows, and writes k and v into the pages."""
@@ -223,5 +229,9 @@ class PagedCache:
 
     def attn_dev(self, layer, q, out, stream=None) -> None:
         """Attention of the batch's tokens over their sequences."""
-        self._ok(self.lib.l3p_paged_attn_dev(self.h, layer, *self._rows(q, self.n_heads, "q"),
-                                             *self._rows(out, self.n_heads, "out"), self._stream(stream)), "attn_dev")
+        heads = self.n_heads
+        qp, qs = self._rows(q, heads, "q")
+        op, os_ = self._rows(out, heads, "out")
+        rc = self.lib.l3p_paged_attn_dev(self.h, layer, qp, qs, op, os_, self._stream(stream))
+        if rc:
+            self._ok(rc, "attn_dev")
