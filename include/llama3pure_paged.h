@@ -61,7 +61,7 @@ typedef struct l3p_paged_config {
     int max_tokens;   /* new tokens of one batch at most */
     int max_seq_len;  /* positions of one sequence at most; 0 => n_pages * page_size */
     int dtype;        /* L3P_PAGED_F32 or L3P_PAGED_BF16 */
-    float scale;      /* multiplies q.k; 0 => 1/sqrt(head_dim) */
+    float scale;      /* multiplies q.k, not negative; 0 => 1/sqrt(head_dim) */
     int is_gemma3;    /* sliding-window layers as in l3p_attn_config: with is_gemma3, */
     int swa_window;   /*   swa_window > 0 and swa_pattern > 0, layer l with */
     int swa_pattern;  /*   l % swa_pattern < swa_pattern - 1 attends to the last swa_window positions */

@@ -410,7 +410,7 @@ int create(const l3p_paged_config& in, Ctx** out) {
   if (c.page_size != 16 && c.page_size != 32 && c.page_size != 64 && c.page_size != 128) return L3P_E_UNSUPPORTED;
   if (c.n_pages <= 0 || c.max_seqs <= 0 || c.max_tokens <= 0 || c.max_seq_len < 0) return L3P_E_INVAL;
   if (c.dtype != L3P_PAGED_F32 && c.dtype != L3P_PAGED_BF16) return L3P_E_INVAL;
-  if (!std::isfinite(c.scale) || c.swa_window < 0 || c.swa_pattern < 0 || c.device < 0) return L3P_E_INVAL;
+  if (!std::isfinite(c.scale) || c.scale < 0.f || c.swa_window < 0 || c.swa_pattern < 0 || c.device < 0) return L3P_E_INVAL;
   // positions, storage rows and query rows are counted in 32 bits
   const long long pool_pos = (long long)c.n_pages * c.page_size;
   if (pool_pos > INT_MAX / 2 || c.max_seqs > 65536) return L3P_E_RANGE;

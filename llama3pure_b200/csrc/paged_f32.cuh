@@ -210,7 +210,6 @@ __global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
   const uint32_t lb = (uint32_t)((warp & 3) * 32) << 16;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 || warp == 2) {
       // ---------------- producers, chunks in turn ----------------
       if (lane == 0) {
@@ -335,7 +334,6 @@ __global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
     }
   } else if (warp < 8) {
     // ---------------- softmax: thread = row ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     {
       const float4* src = reinterpret_cast<const float4*>(a.q + (long long)(u.q_row0 + tok) * a.q_stride + (long long)head * HD);
 #pragma unroll 1
@@ -427,7 +425,6 @@ __global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
     if (lane == 0) mbar_arrive(&bar_sm_done);
   } else {
     // ---------------- O: thread = row ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     float acc[HD];
 #pragma unroll
     for (int i = 0; i < HD; ++i) acc[i] = 0.f;

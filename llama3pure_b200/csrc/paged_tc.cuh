@@ -51,6 +51,8 @@ struct PgTcCfg {
   // tensor memory columns: S (and P in its place), then O
   static constexpr int kS = HD == 256 ? 64 : 128;
   static constexpr int kO = 256;
+  static constexpr int kHands = HD == 256 ? 1 : 2;  // parts in which a tile's P is handed to the second product
+  static constexpr int kPoly = 2;     // of 8 pairs of exponentials
   static_assert(kSmem <= 232448 - 512, "shared memory");
 };
 
@@ -83,16 +85,27 @@ __device__ __forceinline__ bool pg_wait(uint64_t* bar, uint32_t parity, int* err
 __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, bool b_mn_major) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
-__device__ __forceinline__ void mma_bf16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+// Issued by the lane for which `leader` is set, in code that the whole warp runs:
+// outside divergent code the descriptors stay in uniform registers (an issue
+// costs a lone thread ~85 cycles, 16 of which a tile has no time for).
+__device__ __forceinline__ void mma_bf16_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc),
+      "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void mma_bf16_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc),
+      "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void pg_commit(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)), "r"(leader)
       : "memory");
 }
 __device__ __forceinline__ void pg_tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
@@ -110,6 +123,56 @@ __device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t (&v)[3
       "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
       "r"(v[31])
       : "memory");
+}
+
+// ---- two fp32 values in one 64-bit register: half the issue slots
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pk2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void un2(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x on the fma pipe for x <= 0: x = n + r with n = round(x), 2^r by a
+// polynomial of degree 4 on [-1/2, 1/2] (least-squares fit of the relative
+// error, weights iterated towards its maximum: 2.6e-6), times 2^n.  Below -126
+// it stays at 2^-126; NaN stays NaN.
+__device__ __forceinline__ f32x2 exp2_poly2(f32x2 x) {
+  const float magic = 12582912.f;  // 1.5 * 2^23: its sum with x has n in the low bits
+  float a, b;
+  un2(x, a, b);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
+  x = pk2(a, b);
+  const f32x2 t = add2(x, pk2(magic, magic));
+  const f32x2 r = fma2(add2(t, pk2(-magic, -magic)), pk2(-1.f, -1.f), x);
+  f32x2 p = fma2(pk2(0.009570101276040077f, 0.009570101276040077f), r, pk2(0.05591786280274391f, 0.05591786280274391f));
+  p = fma2(p, r, pk2(0.240247443318367f, 0.240247443318367f));
+  p = fma2(p, r, pk2(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(p, r, pk2(0.9999992847442627f, 0.9999992847442627f));
+  float ta, tb;
+  un2(t, ta, tb);
+  return mul2(p, pk2(__int_as_float((__float_as_int(ta) << 23) + 0x3F800000), __int_as_float((__float_as_int(tb) << 23) + 0x3F800000)));
 }
 
 // Joins the parts of split units: row = sum_p w_p o_p / sum_p w_p l_p with
@@ -179,7 +242,7 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
   __shared__ uint32_t s_tmem;
   __shared__ int s_bad;
   __shared__ __align__(8) uint64_t kv_full[S], kv_empty[S], v_ok[S];
-  __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_done[2], q_ready[2], mma_idle;
+  __shared__ __align__(8) uint64_t s_full[2], p_full[2][2], o_done[2], q_ready[2], mma_idle;
 
   const PgHeader* h = reinterpret_cast<const PgHeader*>(a.batch);
   const PgLists l = h->lists[a.win];
@@ -212,7 +275,8 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&s_full[b], 1);
-      mbar_init(&p_full[b], 4);
+      mbar_init(&p_full[b][0], 4);
+      mbar_init(&p_full[b][1], 4);
       mbar_init(&o_done[b], 1);
       mbar_init(&q_ready[b], 4);
     }
@@ -226,6 +290,10 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
   const uint32_t tm = s_tmem;
   griddep_wait();  // q and the new rows come from the kernel before this one
 
+  // Registers: 384 x 168 at launch = 128 x 88 + 256 x 208.  Inside the branches: behind their join the compiler would
+  // count with the smaller number.
+  if (warp < 4) {
+  if (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 0) {
     // ---------------- loads ----------------
     const int box = min(1 << a.shift, TN), n_box = TN / box;  // keys of a box, boxes down a tile
@@ -253,81 +321,79 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
     for (int t = max(0, n_used - S); t < n_used; ++t) pg_wait(&kv_full[t % S], (uint32_t)((t / S) & 1), a.err);
   } else if (warp == 1) {
     // ---------------- MMA issue ----------------
-    if (lane == 0) {
-      constexpr uint32_t id_s = idesc_bf16(128, TN, false), id_o = idesc_bf16(128, HD, true);
-      const uint64_t q_d = tc::sdesc_sw128(smem_addr(sq), 16, 1024);
-      const uint64_t k_d = tc::sdesc_sw128(smem_addr(ring), 16, 1024);
-      const uint64_t v_d = tc::sdesc_sw128(smem_addr(ring), TN * 128, 1024);
-      auto add = [](uint64_t d, uint32_t bytes) { return d + (bytes >> 4); };
-      auto qk = [&](int b, int slot, int stage) {  // S[slot] = Q[b] K^T
+    constexpr uint32_t id_s = idesc_bf16(128, TN, false), id_o = idesc_bf16(128, HD, true);
+    uint32_t leader;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+    const uint64_t q_d = tc::sdesc_sw128(smem_addr(sq), 16, 1024);
+    const uint64_t k_d = tc::sdesc_sw128(smem_addr(ring), 16, 1024);
+    const uint64_t v_d = tc::sdesc_sw128(smem_addr(ring), TN * 128, 1024);
+    auto qk = [&](int b, int slot, int stage) {  // S[slot] = Q[b] K^T
+      const uint64_t kd = k_d + (uint64_t)((stage * C::kStage) >> 4), qd = q_d + (uint64_t)(b * (128 * HD * 2) >> 4);
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k)
-          mma_bf16_ss(tm + slot * C::kS, add(q_d, b * (128 * HD * 2) + (k / 4) * 16384 + (k % 4) * 32),
-                      add(k_d, stage * C::kStage + (k / 4) * (TN * 128) + (k % 4) * 32), id_s, k > 0);
-      };
-      auto pv = [&](int b, int slot, int stage, bool acc) {  // O[b] += P[slot] V
+      for (int k = 0; k < HD / 16; ++k)
+        mma_bf16_ss(leader, tm + slot * C::kS, qd + (((k / 4) * 16384 + (k % 4) * 32) >> 4),
+                    kd + (((k / 4) * (TN * 128) + (k % 4) * 32) >> 4), id_s, k > 0);
+    };
+    auto pv = [&](int b, int slot, int stage, int hf, bool acc) {  // O[b] += P[slot] V, the part's keys
+      const uint64_t vd = v_d + (uint64_t)((stage * C::kStage) >> 4);
 #pragma unroll
-        for (int k = 0; k < TN / 16; ++k)
-          mma_bf16_ts(tm + C::kO + b * HD, tm + slot * C::kS + k * 8, add(v_d, stage * C::kStage + k * 2048), id_o, acc || k > 0);
-      };
-      auto wait = [&](uint64_t* bar, int phase) {
-        const bool r = pg_wait(bar, (uint32_t)(phase & 1), a.err);
-        tc::fence_after_sync();
-        return r;
-      };
-      bool ok = true;
+      for (int k = hf * (TN / 16 / C::kHands); k < (hf + 1) * (TN / 16 / C::kHands); ++k)
+        mma_bf16_ts(leader, tm + C::kO + b * HD, tm + slot * C::kS + k * 8, vd + (k * 2048 >> 4), id_o, acc || k > 0);
+    };
+    auto wait = [&](uint64_t* bar, int phase) {
+      const bool r = __all_sync(0xffffffffu, pg_wait(bar, (uint32_t)(phase & 1), a.err));
+      tc::fence_after_sync();
+      return r;
+    };
+    bool ok = wait(&kv_full[0], 0);
+    for (int b = 0; ok && b < nq; ++b) {
+      if (!(ok = wait(&q_ready[b], 0))) break;
+      qk(b, NQ == 2 ? b : 0, 0);
+      pg_commit(leader, &s_full[b]);
+    }
+    pg_commit(leader, &kv_empty[0]);
+    for (int j = 0; ok && j < nt; ++j) {
+      const int tv = 2 * j + 1, tk = 2 * j + 2, sv = tv % S, sk = tk % S;
       if constexpr (NQ == 2) {
-        // S of both tiles, then per key tile and Q tile: O += P V, S of the next key tile.  MMAs run in the order of
-        // issue, so S may overwrite the P that the product before it reads.
-        ok = wait(&kv_full[0], 0);
-        for (int b = 0; ok && b < nq; ++b) {
-          if (!(ok = wait(&q_ready[b], 0))) break;
-          qk(b, b, 0);
-          tc::commit(&s_full[b]);
-        }
-        tc::commit(&kv_empty[0]);
-        for (int j = 0; ok && j < nt; ++j) {
-          const int tv = 2 * j + 1, tk = 2 * j + 2, sv = tv % S, sk = tk % S;
-          for (int b = 0; ok && b < nq; ++b) {
-            if (b == 0 && !(ok = wait(&v_ok[j % S], j / S))) break;
-            if (!(ok = wait(&p_full[b], j))) break;
-            pv(b, b, sv, j > 0);
-            if (b == nq - 1) tc::commit(&kv_empty[sv]);
-            tc::commit(&o_done[b]);
-            if (j + 1 < nt) {
-              if (b == 0 && !(ok = wait(&kv_full[sk], tk / S))) break;
-              qk(b, b, sk);
-              tc::commit(&s_full[b]);
-              if (b == nq - 1) tc::commit(&kv_empty[sk]);
-            }
+        // per Q tile: O += P V, then S of the next key tile.  MMAs run in the order of issue, so S may overwrite the P
+        // that the product before it reads
+        if (!(ok = wait(&v_ok[j % S], j / S) && (j + 1 == nt || wait(&kv_full[sk], tk / S)))) break;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          if (b >= nq || !ok) break;
+#pragma unroll
+          for (int hf = 0; hf < C::kHands; ++hf) {
+            if (!(ok = ok && wait(&p_full[b][hf], j))) break;
+            pv(b, b, sv, hf, j > 0);
+          }
+          if (!ok) break;
+          if (j + 1 < nt) {
+            qk(b, b, sk);
+            pg_commit(leader, &s_full[b]);
+          }
+          pg_commit(leader, &o_done[b]);
+          if (b == nq - 1) {
+            pg_commit(leader, &kv_empty[sv]);
+            if (j + 1 < nt) pg_commit(leader, &kv_empty[sk]);
           }
         }
       } else {
         // one Q tile, S in two places: S of the next key tile is issued ahead of this tile's O += P V
-        ok = wait(&kv_full[0], 0) && wait(&q_ready[0], 0);
-        if (ok) {
-          qk(0, 0, 0);
-          tc::commit(&s_full[0]);
-          tc::commit(&kv_empty[0]);
+        if (j + 1 < nt) {
+          if (!(ok = wait(&kv_full[sk], tk / S))) break;
+          qk(0, (j + 1) & 1, sk);
+          pg_commit(leader, &s_full[(j + 1) & 1]);
+          pg_commit(leader, &kv_empty[sk]);
         }
-        for (int j = 0; ok && j < nt; ++j) {
-          const int tv = 2 * j + 1, tk = 2 * j + 2, sv = tv % S, sk = tk % S;
-          if (j + 1 < nt) {
-            if (!(ok = wait(&kv_full[sk], tk / S))) break;
-            qk(0, (j + 1) & 1, sk);
-            tc::commit(&s_full[(j + 1) & 1]);
-            tc::commit(&kv_empty[sk]);
-          }
-          if (!(ok = wait(&v_ok[j % S], j / S) && wait(&p_full[j & 1], j >> 1))) break;
-          pv(0, j & 1, sv, j > 0);
-          tc::commit(&kv_empty[sv]);
-          tc::commit(&o_done[0]);
-        }
+        if (!(ok = wait(&v_ok[j % S], j / S) && wait(&p_full[j & 1][0], j >> 1))) break;
+        pv(0, j & 1, sv, 0, j > 0);
+        pg_commit(leader, &kv_empty[sv]);
+        pg_commit(leader, &o_done[0]);
       }
-      // every MMA has ended before tensor memory is released
-      tc::commit(&mma_idle);
-      pg_wait(&mma_idle, 0, a.err);
     }
+    // every MMA has ended before tensor memory is released
+    pg_commit(leader, &mma_idle);
+    pg_wait(&mma_idle, 0, a.err);
   } else if (warp == 2) {
     // ---------------- V tiles that are not attended to entirely ----------------
     bool ok = true;
@@ -359,7 +425,10 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
       }
       if (lane == 0) mbar_arrive(&v_ok[j % S]);  // by V tile: a stage holds K tiles in between
     }
-  } else if (warp >= 4 && (warp - 4) / 4 < nq) {
+  }
+  } else {
+  if (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  if ((warp - 4) / 4 < nq) {
     // ---------------- softmax: thread = row ----------------
     const int b = (warp - 4) / 4;
     const int row = (warp & 3) * 32 + lane;  // of this Q tile
@@ -381,9 +450,9 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_ready[b]);
     }
-    float m = -INFINITY, lsum = 0.f;  // m: largest score before scaling (of -score for a negative scale)
+    float m = -INFINITY, lsum = 0.f;  // m: largest score before scaling
     bool ok = true;
-    const float sl = a.scale_log2, asl = fabsf(sl);
+    const float sl = a.scale_log2;
     const uint32_t T_O = tm + C::kO + b * HD + lb;
     for (int j = 0; j < nt; ++j) {
       const int slot = NQ == 2 ? b : j & 1;
@@ -407,58 +476,89 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
       if (!__all_sync(0xffffffffu, key0 >= kmin && key0 + TN - 1 <= qpos)) {
 #pragma unroll
         for (int c = 0; c < TN; ++c)
-          if (key0 + c > qpos || key0 + c < kmin) sv[c] = sl >= 0.f ? -INFINITY : INFINITY;
+          if (key0 + c > qpos || key0 + c < kmin) sv[c] = -INFINITY;
       }
-      // the row's largest scaled score: the largest raw score for a positive scale, the smallest for a negative one
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (sl >= 0.f) {
+      // p = 2^(s scale log2e - m scale log2e): of each eight pairs, kPoly by polynomial, the others on the special-function
+      // unit, whose 16 a cycle the two Q tiles' 32K would otherwise fill
+      constexpr int N2 = TN / 2 / C::kHands;  // pairs of a part
+      const f32x2 sl2 = pk2(sl, sl);
+      f32x2 ls[2], neg2;
+      uint32_t pk[N2];
+      auto weights = [&](int hf) {
 #pragma unroll
-        for (int c = 0; c < TN; ++c) mx[c & 3] = fmaxf(mx[c & 3], sv[c]);
-      } else {
-#pragma unroll
-        for (int c = 0; c < TN; ++c) mx[c & 3] = fmaxf(mx[c & 3], -sv[c]);
-      }
-      const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-      const bool grow = m == -INFINITY ? m_new != -INFINITY : (m_new - m) * asl > 8.f;
-      float alpha = 1.f;
-      if (grow) {
-        alpha = m == -INFINITY ? 0.f : fast_exp2((m - m_new) * asl);
-        lsum *= alpha;
-        m = m_new;
-      }
-      if (j > 0 && __any_sync(0xffffffffu, grow)) {
-        ok = __all_sync(0xffffffffu, pg_wait(&o_done[b], (uint32_t)((j - 1) & 1), a.err));
-        if (!ok) break;
-        tc::fence_after_sync();
-#pragma unroll 1
-        for (int c = 0; c < HD / 32; ++c) {
-          float ov[32];
-          tc::ld32(T_O + c * 32, ov);
-          tc::wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) ov[i] *= alpha;
-          tc::st32(T_O + c * 32, ov);
-        }
-      }
-      const float neg = m == -INFINITY ? 0.f : -m * asl;
-      float ls[2] = {0.f, 0.f};
-#pragma unroll
-      for (int hf = 0; hf < TN / 64; ++hf) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const float p0 = fast_exp2(fmaf(sv[hf * 64 + 2 * c], sl, neg)), p1 = fast_exp2(fmaf(sv[hf * 64 + 2 * c + 1], sl, neg));
-          ls[0] += p0;
-          ls[1] += p1;
+        for (int c = 0; c < N2; ++c) {
+          const int e = 2 * (hf * N2 + c);
+          const f32x2 x = fma2(pk2(sv[e], sv[e + 1]), sl2, neg2);
+          f32x2 p;
+          float p0, p1;
+          if ((c & 7) < C::kPoly) {
+            p = exp2_poly2(x);
+            un2(p, p0, p1);
+          } else {
+            un2(x, p0, p1);
+            p0 = fast_exp2(p0);
+            p1 = fast_exp2(p1);
+            p = pk2(p0, p1);
+          }
+          ls[c & 1] = add2(ls[c & 1], p);
           pk[c] = pg_pack_bf16(p0, p1);
         }
-        tmem_st32u(T_S + hf * 32, pk);
+      };
+      // The first part is computed with the reference of the tiles before while the maximum is found; the reference
+      // changes only when a row's maximum grew by more than 2^8, and then the part is computed again.
+      float neg = m == -INFINITY ? 0.f : -m * sl;
+      neg2 = pk2(neg, neg);
+      ls[0] = ls[1] = 0ull;
+      float mx[4] = {sv[0], sv[1], sv[2], sv[3]};
+#pragma unroll
+      for (int c = 4; c < TN - 4; c += 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], sv[c + 2 * i], sv[c + 2 * i + 1]);
       }
-      lsum += ls[0] + ls[1];
-      tc::wait_st();
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[slot]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], sv[TN - 4 + i]);
+      const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+      const bool grow = m == -INFINITY ? m_new != -INFINITY : (m_new - m) * sl > 8.f;
+      if (j > 0) weights(0);
+      if (__any_sync(0xffffffffu, grow || j == 0)) {
+        float alpha = 1.f;
+        if (grow) {
+          alpha = m == -INFINITY ? 0.f : fast_exp2((m - m_new) * sl);
+          lsum *= alpha;
+          m = m_new;
+        }
+        if (j > 0) {
+          ok = __all_sync(0xffffffffu, pg_wait(&o_done[b], (uint32_t)((j - 1) & 1), a.err));
+          if (!ok) break;
+          tc::fence_after_sync();
+#pragma unroll 1
+          for (int c = 0; c < HD / 32; ++c) {
+            float ov[32];
+            tc::ld32(T_O + c * 32, ov);
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) ov[i] *= alpha;
+            tc::st32(T_O + c * 32, ov);
+          }
+        }
+        neg = m == -INFINITY ? 0.f : -m * sl;
+        neg2 = pk2(neg, neg);
+        ls[0] = ls[1] = 0ull;
+        weights(0);
+      }
+#pragma unroll
+      for (int hf = 0; hf < C::kHands; ++hf) {
+        if (hf > 0) weights(hf);
+        tmem_st32u(T_S + hf * N2, pk);
+        tc::wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[slot][hf]);
+      }
+      float l0, l1, l2, l3;
+      un2(ls[0], l0, l1);
+      un2(ls[1], l2, l3);
+      lsum += (l0 + l1) + (l2 + l3);
     }
     if (NQ == 1 && ok && nt > 1) ok = __all_sync(0xffffffffu, pg_wait(&o_done[b], (uint32_t)(nt & 1), a.err));
     if (ok) ok = __all_sync(0xffffffffu, pg_wait(&o_done[b], (uint32_t)((nt - 1) & 1), a.err));
@@ -505,8 +605,9 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
           }
         }
       }
-      if (split && valid) *reinterpret_cast<float2*>(a.ws_ml + ws_row * 2) = make_float2(m == -INFINITY ? m : m * asl, lsum);
+      if (split && valid) *reinterpret_cast<float2*>(a.ws_ml + ws_row * 2) = make_float2(m * sl, lsum);
     }
+  }
   }
   tc::fence_before_sync();
   __syncthreads();

@@ -27,6 +27,7 @@ def _cfg(**kw):
     (dict(max_seq_len=-1), -1),
     (dict(dtype=2), -1),
     (dict(scale=float("nan")), -1),
+    (dict(scale=-0.1), -1),
     (dict(swa_window=-1), -1),
     (dict(device=-1), -1),
     (dict(n_pages=2**30), -2),                                  # positions beyond 32 bits
