@@ -121,7 +121,18 @@ int refuse_capture(Ctx* ctx, cudaStream_t s, const char* what) {
 
 struct BatchSeq {
   int q_row0, n_new, len, tbl;  // len: with the new tokens
+  bool tc;                      // takes the tensor-core kernels
 };
+
+// Which kernels a sequence takes.  Up to 8 rows per KV head (up to row_limit, if no sequence of the batch has more): the
+// row kernel.  Sequences of 9 to row_limit rows go with the longer ones where there are some: two kernels, each with part
+// of the batch, fill the GPU less than one (16 drafts of 3 to 6 tokens, 8B heads: see the measurements in plan_tc).
+void choose_paths(const Ctx* ctx, std::vector<BatchSeq>* bs) {
+  const int limit = row_limit(ctx);
+  bool any = false;
+  for (const auto& b : *bs) any |= (long long)b.n_new * ctx->G > limit;
+  for (auto& b : *bs) b.tc = (long long)b.n_new * ctx->G > (any ? std::min(limit, 8) : limit);
+}
 
 // First key that the token at `pos` attends to.
 int first_key(const Ctx* ctx, bool win, int pos) { return win ? std::max(0, pos - ctx->cfg.swa_window + 1) : 0; }
@@ -139,13 +150,13 @@ int first_key(const Ctx* ctx, bool win, int pos) { return win ? std::max(0, pos 
 constexpr double kSegRounds = 1.5;
 void plan_rows(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, int nt, std::vector<int>* first,
                std::vector<PgSeg>* segs) {
-  const int limit = row_limit(ctx), rt = 8 * nt, warps = row_warps(ctx), G = ctx->G;
+  const int rt = 8 * nt, warps = row_warps(ctx), G = ctx->G;
   std::vector<PgSeg> units;
   long long total = 0;
   int longest = 0;
   for (const auto& b : bs) {
     const long long rows = (long long)b.n_new * G;
-    if (rows == 0 || rows > limit) continue;
+    if (rows == 0 || b.tc) continue;
     const int pos0 = b.len - b.n_new;
     for (int h = 0; h < ctx->cfg.n_kv_heads; ++h)
       for (int r0 = 0; r0 < rows; r0 += rt) {
@@ -236,15 +247,14 @@ void plan_rows(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, int nt
 // key tiles that the units read.
 void plan_tc(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vector<PgPart>* parts,
              std::vector<PgPart>* merges, std::vector<PgPrep>* prep) {
-  const int limit = row_limit(ctx), tile = ctx->bf16 ? tc_tile(ctx) : 128, G = ctx->G;
+  const int tile = ctx->bf16 ? tc_tile(ctx) : 128, G = ctx->G;
   const int rt = ctx->bf16 ? tc_rows(ctx) : f32_rows(ctx);
   // CTAs (or CTA pairs) that run at once
   const int wide = !ctx->bf16 && rt == 256 ? ctx->num_sms / 2 : ctx->num_sms;
   std::vector<PgPart> units;
-  long long total = 0;
   for (const auto& b : bs) {
     const long long rows = (long long)b.n_new * G;
-    if (rows <= limit) continue;
+    if (!b.tc) continue;
     const int pos0 = b.len - b.n_new;
     int img0 = 0;
     if (!ctx->bf16) {
@@ -265,15 +275,46 @@ void plan_tc(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vec
         u.tile0 = first_key(ctx, win, pos0 + (int)(r0 / G)) / tile;
         u.tile1 = (u.key_hi + tile - 1) / tile;
         u.img = img0;
-        total += u.tile1 - u.tile0;
         units.push_back(u);
       }
   }
-  // no part is shorter than 8 tiles: below that the merge's launch costs more than the split saves
-  const int cap = (int)std::max<long long>(8, (total + wide - 1) / wide);
+  // A part's time is its tiles times what a tile costs: of bf16 blocks of more than 128 rows 3.8K cycles, of up to 128
+  // rows (two streams of tiles) about half of that, more where small pages bound the loads.
+  auto weight = [&](const PgPart& u) { return ctx->bf16 && rt == 256 ? (u.n_rows > 128 ? 5 : 3) : 1; };
+  // no part is shorter than 1024 keys: below that the merge's launch costs more than the split saves
+  const int least = 1024 / tile;
+  auto parts_of = [&](const PgPart& u, long long share) {
+    const int n = u.tile1 - u.tile0, w = weight(u), cap = (int)std::max<long long>(least, (share + w - 1) / w);
+    return (n + cap - 1) / cap;
+  };
+  // the smallest share with which all parts run at once; with more units than that the longest go first and are cut
+  // only when one of them is longer than an SM's part of everything
+  long long total = 0, longest = 0;
+  for (const auto& u : units) {
+    const long long c = (long long)weight(u) * (u.tile1 - u.tile0);
+    total += c;
+    longest = std::max(longest, c);
+  }
+  long long share = (total + wide - 1) / wide;
+  if ((int)units.size() <= wide) {
+    auto count = [&](long long s) {
+      long long n = 0;
+      for (const auto& u : units) n += parts_of(u, s);
+      return n;
+    };
+    long long lo = std::max<long long>(share, 1), hi = std::max(longest, lo);
+    while (lo < hi) {
+      const long long mid = (lo + hi) / 2;
+      if (count(mid) <= wide)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    share = hi;
+  }
   int slot = 0;
   for (const auto& u : units) {
-    const int n = u.tile1 - u.tile0, k = (n + cap - 1) / cap;
+    const int n = u.tile1 - u.tile0, k = parts_of(u, share);
     for (int i = 0; i < k; ++i) {
       PgPart p = u;
       p.tile0 = u.tile0 + (int)((long long)n * i / k);
@@ -291,8 +332,9 @@ void plan_tc(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vec
       slot += k;
     }
   }
-  std::stable_sort(parts->begin(), parts->end(),
-                   [](const PgPart& a, const PgPart& b) { return a.tile1 - a.tile0 > b.tile1 - b.tile0; });
+  std::stable_sort(parts->begin(), parts->end(), [&](const PgPart& a, const PgPart& b) {
+    return weight(a) * (a.tile1 - a.tile0) > weight(b) * (b.tile1 - b.tile0);
+  });
 }
 
 // Lays the current batch out as the kernels read it.
@@ -301,11 +343,10 @@ void build_batch(const Ctx* ctx, const std::vector<BatchSeq>& bs, const int* seq
   PgHeader h{};
   h.n_tokens = n_tokens;
   h.n_seqs = n_seqs;
-  const int limit = row_limit(ctx);
   int max_rows = 0;
   for (const auto& b : bs)
-    if ((long long)b.n_new * ctx->G <= limit) max_rows = std::max(max_rows, b.n_new * ctx->G);
-  h.row_nt = std::min(max_rows <= 8 ? 1 : max_rows <= 16 ? 2 : 4, row_max_nt(ctx));
+    if (!b.tc) max_rows = std::max(max_rows, b.n_new * ctx->G);
+  h.row_nt = std::min(max_rows <= 8 ? 1 : 2, row_max_nt(ctx));
   auto& w = *words;
   w.assign(kPgHdrWords, 0);
   auto add = [&](const void* p, size_t bytes) {
@@ -523,12 +564,13 @@ int begin(Ctx* ctx, int n_seqs, const int* ids, const int* n_new, cudaStream_t s
       ctx->fill[p] = std::max(ctx->fill[p], std::min(ctx->cfg.page_size, len - (pos & ~(ctx->cfg.page_size - 1))));
     }
     q.len = len;
-    bs[i] = {row, n_new[i], len, tbl};
+    bs[i] = {row, n_new[i], len, tbl, false};
     row += n_new[i];
     if (n_new[i] > 0) ctx->max_pos_in_batch = std::max(ctx->max_pos_in_batch, len);
     tbl += (int)q.pages.size();
   }
   if (int rc = copy_pages(ctx, jobs, s)) return rc;
+  choose_paths(ctx, &bs);
   std::vector<int> words;
   build_batch(ctx, bs, ids, n_seqs, row, &words, &ctx->hdr);
   if (words.size() > ctx->batch_words) return fail(ctx, L3P_E_RANGE, "batch description of %zu words", words.size());

@@ -12,14 +12,12 @@ namespace l3p_pg {
 // Sequences with more query rows per KV head take the tensor-core kernels.
 // fp32 with head_dim 256 has none: Q and O alone would fill tensor memory.
 int row_limit(const l3p_paged_ctx* ctx) {
-  if (ctx->bf16) return ctx->hd == 256 ? 16 : 32;
-  return ctx->hd == 256 ? INT_MAX : 16;
+  return !ctx->bf16 && ctx->hd == 256 ? INT_MAX : 16;
 }
 
 // Blocks of 8 rows whose Q and O fit a thread's registers.
 int row_max_nt(const l3p_paged_ctx* ctx) {
-  if (ctx->bf16) return ctx->hd == 256 ? 2 : 4;
-  return ctx->hd == 256 ? 1 : 2;
+  return !ctx->bf16 && ctx->hd == 256 ? 1 : 2;
 }
 
 int row_warps(const l3p_paged_ctx* ctx) {
@@ -33,8 +31,8 @@ static int with_kernel(const l3p_paged_ctx* ctx, int nt, F f) {
   using B = __nv_bfloat16;
 #define PG_ROW(T, HD, NT) f(paged_rows_kernel<T, HD, NT>, PgRowCfg<T, HD>::kWarps * 32, PgRowCfg<T, HD>::kSmem)
   if (ctx->bf16) {
-    if (ctx->hd == 64) return nt == 1 ? PG_ROW(B, 64, 1) : nt == 2 ? PG_ROW(B, 64, 2) : PG_ROW(B, 64, 4);
-    if (ctx->hd == 128) return nt == 1 ? PG_ROW(B, 128, 1) : nt == 2 ? PG_ROW(B, 128, 2) : PG_ROW(B, 128, 4);
+    if (ctx->hd == 64) return nt == 1 ? PG_ROW(B, 64, 1) : PG_ROW(B, 64, 2);
+    if (ctx->hd == 128) return nt == 1 ? PG_ROW(B, 128, 1) : PG_ROW(B, 128, 2);
     return nt == 1 ? PG_ROW(B, 256, 1) : PG_ROW(B, 256, 2);
   }
   if (ctx->hd == 64) return nt == 1 ? PG_ROW(float, 64, 1) : PG_ROW(float, 64, 2);

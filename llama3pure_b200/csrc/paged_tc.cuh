@@ -22,7 +22,7 @@
 // columns, into a ring in consumption order K0 V0 K1 V1 ..., 128-byte swizzled:
 // K is the K-major B operand of S, V the MN-major B operand of O.
 //
-// Roles: warp 0 loads; warp 1 issues MMAs; warp 2 checks V tiles that some row
+// Roles: warp 0 loads; warp 1 issues MMAs; warps 2 and 3 check V tiles that some row
 // does not attend to entirely (masked weights are 0, and 0 times a value that
 // is not finite is NaN: rows outside every window become 0, such values are
 // taken out and added in the epilogue to the rows that attend to them); warps
@@ -52,8 +52,7 @@ struct PgTcCfg {
   static constexpr int kS = HD == 256 ? 64 : 128;
   static constexpr int kO = 256;
   static constexpr int kHands = HD == 256 ? 1 : 2;  // parts in which a tile's P is handed to the second product
-  static constexpr int kPoly = 2;     // of 8 pairs of exponentials
-  static_assert(kSmem <= 232448 - 512, "shared memory");
+  static_assert(kSmem <= 232448 - 1536, "shared memory");
 };
 
 struct PgTcArgs {
@@ -143,38 +142,11 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^x on the fma pipe for x <= 0: x = n + r with n = round(x), 2^r by a
-// polynomial of degree 4 on [-1/2, 1/2] (least-squares fit of the relative
-// error, weights iterated towards its maximum: 2.6e-6), times 2^n.  Below -126
-// it stays at 2^-126; NaN stays NaN.
-__device__ __forceinline__ f32x2 exp2_poly2(f32x2 x) {
-  const float magic = 12582912.f;  // 1.5 * 2^23: its sum with x has n in the low bits
-  float a, b;
-  un2(x, a, b);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
-  x = pk2(a, b);
-  const f32x2 t = add2(x, pk2(magic, magic));
-  const f32x2 r = fma2(add2(t, pk2(-magic, -magic)), pk2(-1.f, -1.f), x);
-  f32x2 p = fma2(pk2(0.009570101276040077f, 0.009570101276040077f), r, pk2(0.05591786280274391f, 0.05591786280274391f));
-  p = fma2(p, r, pk2(0.240247443318367f, 0.240247443318367f));
-  p = fma2(p, r, pk2(0.6931217908859253f, 0.6931217908859253f));
-  p = fma2(p, r, pk2(0.9999992847442627f, 0.9999992847442627f));
-  float ta, tb;
-  un2(t, ta, tb);
-  return mul2(p, pk2(__int_as_float((__float_as_int(ta) << 23) + 0x3F800000), __int_as_float((__float_as_int(tb) << 23) + 0x3F800000)));
-}
-
 // Joins the parts of split units: row = sum_p w_p o_p / sum_p w_p l_p with
 // w_p = 2^(m_p - max m), in part order.  One warp per row, a lane holds HD/32
 // values; a kernel of its own because the last of the parts' CTAs, alone on its SM,
@@ -241,7 +213,8 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
   extern __shared__ unsigned char tc_smem_raw[];
   __shared__ uint32_t s_tmem;
   __shared__ int s_bad;
-  __shared__ __align__(8) uint64_t kv_full[S], kv_empty[S], v_ok[S];
+  __shared__ float s_m1[128], s_l1[128];
+  __shared__ __align__(8) uint64_t kv_full[S + 2], kv_empty[S + 2], v_ok[S];
   __shared__ __align__(8) uint64_t s_full[2], p_full[2][2], o_done[2], q_ready[2], mma_idle;
 
   const PgHeader* h = reinterpret_cast<const PgHeader*>(a.batch);
@@ -255,10 +228,22 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
   const PgPart u = reinterpret_cast<const PgPart*>(a.batch + l.tc_parts)[blockIdx.x];
   const int* table = a.batch + h->tbl + u.tbl;
   unsigned char* sq = (unsigned char*)(((uintptr_t)tc_smem_raw + 1023) & ~(uintptr_t)1023);
-  unsigned char* ring = sq + C::kQBytes;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int nq = u.n_rows > 128 ? NQ : 1;
   const int nt = u.tile1 - u.tile0;
+  // Two streams of key tiles: one per Q tile, each over all key tiles; or, for up to 128 rows, both for the one Q tile,
+  // over the even and the odd key tiles, joined at the end.
+  const bool dual = NQ == 2 && u.n_rows <= 128;
+  const int nq = NQ == 2 && (!dual || nt > 1) ? 2 : 1;
+  // The ring, in the order of use: K0 V0 K1 V1 ... or, with two streams of tiles, K0 K1 V0 K2 V1 K3 ...; then the second Q
+  // tile's place is part of it.  Nearly all of it is in flight at any time, which is what HBM needs: ~19 MB over the GPU
+  // for its full rate.
+  constexpr int kMore = NQ == 2 ? 128 * HD * 2 / C::kStage : 0;  // stages in a Q tile's place
+  static_assert(kMore <= 2, "barriers");
+  unsigned char* ring = sq + C::kQBytes - (dual ? kMore * C::kStage : 0);
+  auto stage_of = [&](int t) { return dual ? t % (S + kMore) : t % S; };
+  auto use_of = [&](int t) { return dual ? t / (S + kMore) : t / S; };
+  auto k_at = [&](int j) { return dual ? (j < 2 ? j : 2 * j - 1) : 2 * j; };             // position of K tile j in the ring's order
+  auto v_at = [&](int j) { return dual ? min(2 * j + 2, 2 * nt - 1) : 2 * j + 1; };      // and of V tile j
   const int first_pos = u.pos0 + u.r0 / a.G, last_pos = u.pos0 + (u.r0 + u.n_rows - 1) / a.G;
   const int lo_first = a.win ? max(0, first_pos - a.window + 1) : 0;  // keys below: no row attends to them
   const int lo_last = a.win ? max(0, last_pos - a.window + 1) : 0;    // keys from here to first_pos: every row does
@@ -268,11 +253,11 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
     tc::tmem_relinquish();
   }
   if (tid == 32) {
-    for (int s = 0; s < S; ++s) {
+    for (int s = 0; s < S + 2; ++s) {
       mbar_init(&kv_full[s], 1);
       mbar_init(&kv_empty[s], 1);
-      mbar_init(&v_ok[s], 1);
     }
+    for (int s = 0; s < S; ++s) mbar_init(&v_ok[s], 2);
     for (int b = 0; b < 2; ++b) {
       mbar_init(&s_full[b], 1);
       mbar_init(&p_full[b][0], 4);
@@ -301,24 +286,27 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
     const bool mine = c < HD / 64;
     bool ok = true;
     int n_used = 0;
-    for (int t = 0; ok && t < 2 * nt; ++t) {  // K and V of a tile in turn
-      const int s = t % S, use = t / S;
+    for (int t = 0; ok && t < 2 * nt; ++t) {
+      // tile j's K or V is the t-th load
+      const bool is_v = dual ? t >= 2 ? (t & 1) == 0 || t == 2 * nt - 1 : t == 1 && nt == 1 : (t & 1) != 0;
+      const int j = !dual ? t / 2 : is_v ? (t == 2 * nt - 1 ? nt - 1 : t / 2 - 1) : t < 2 ? t : (t + 1) / 2;
+      const int s = stage_of(t), use = use_of(t);
+      const int key = (u.tile0 + j) * TN + i * box;
+      const bool load = mine && key < u.key_hi;
+      const int page = load ? table[key >> a.shift] : 0;
       if (use > 0) ok = __all_sync(0xffffffffu, pg_wait(&kv_empty[s], (uint32_t)((use - 1) & 1), a.err));
       if (!ok) break;
-      const int key = (u.tile0 + t / 2) * TN + i * box;
-      const bool load = mine && key < u.key_hi;
       const int n = __popc(__ballot_sync(0xffffffffu, load));
       if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], (uint32_t)(n * box * 128));
       __syncwarp();
       if (load) {
-        const int page = table[key >> a.shift];
-        const int row = page * a.page_rows + a.row_k + (((t & 1) * a.n_kv + u.kvh) << a.shift) + (key & ((1 << a.shift) - 1));
+        const int row = page * a.page_rows + a.row_k + (((is_v ? a.n_kv : 0) + u.kvh) << a.shift) + (key & ((1 << a.shift) - 1));
         pg_tma_2d(smem_addr(ring + s * C::kStage + c * (TN * 128) + i * (box * 128)), &tmap, c * 64, row, &kv_full[s]);
       }
       n_used = t + 1;
     }
     // no copy may still be landing when the CTA ends
-    for (int t = max(0, n_used - S); t < n_used; ++t) pg_wait(&kv_full[t % S], (uint32_t)((t / S) & 1), a.err);
+    for (int t = max(0, n_used - S - (dual ? kMore : 0)); t < n_used; ++t) pg_wait(&kv_full[stage_of(t)], (uint32_t)(use_of(t) & 1), a.err);
   } else if (warp == 1) {
     // ---------------- MMA issue ----------------
     constexpr uint32_t id_s = idesc_bf16(128, TN, false), id_o = idesc_bf16(128, HD, true);
@@ -345,14 +333,41 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
       tc::fence_after_sync();
       return r;
     };
-    bool ok = wait(&kv_full[0], 0);
-    for (int b = 0; ok && b < nq; ++b) {
-      if (!(ok = wait(&q_ready[b], 0))) break;
-      qk(b, NQ == 2 ? b : 0, 0);
-      pg_commit(leader, &s_full[b]);
+    bool ok = true;
+    if (dual) {
+      // stream b = j & 1: O += P V of key tile j, then S of key tile j + 2
+      ok = wait(&q_ready[0], 0);
+      for (int j = -2; ok && j < nt; ++j) {
+        const int b = j & 1, sv = stage_of(max(0, v_at(j))), tk = k_at(j + 2), sk = stage_of(tk);
+        const bool next = j + 2 < nt;
+        if (j >= 0) {
+          if (!(ok = wait(&v_ok[j % S], j / S))) break;
+#pragma unroll
+          for (int hf = 0; hf < C::kHands; ++hf) {
+            if (!(ok = ok && wait(&p_full[b][hf], j >> 1))) break;
+            pv(b, b, sv, hf, j > 1);
+          }
+          if (!ok) break;
+          pg_commit(leader, &kv_empty[sv]);
+          pg_commit(leader, &o_done[b]);
+        }
+        if (next) {
+          if (!(ok = wait(&kv_full[sk], use_of(tk)))) break;
+          qk(0, b, sk);
+          pg_commit(leader, &s_full[b]);
+          pg_commit(leader, &kv_empty[sk]);
+        }
+      }
+    } else {
+      ok = wait(&kv_full[0], 0);
+      for (int b = 0; ok && b < nq; ++b) {
+        if (!(ok = wait(&q_ready[b], 0))) break;
+        qk(b, NQ == 2 ? b : 0, 0);
+        pg_commit(leader, &s_full[b]);
+      }
+      pg_commit(leader, &kv_empty[0]);
     }
-    pg_commit(leader, &kv_empty[0]);
-    for (int j = 0; ok && j < nt; ++j) {
+    for (int j = 0; ok && !dual && j < nt; ++j) {
       const int tv = 2 * j + 1, tk = 2 * j + 2, sv = tv % S, sk = tk % S;
       if constexpr (NQ == 2) {
         // per Q tile: O += P V, then S of the next key tile.  MMAs run in the order of issue, so S may overwrite the P
@@ -388,37 +403,45 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
         if (!(ok = wait(&v_ok[j % S], j / S) && wait(&p_full[j & 1][0], j >> 1))) break;
         pv(0, j & 1, sv, 0, j > 0);
         pg_commit(leader, &kv_empty[sv]);
-        pg_commit(leader, &o_done[0]);
+        pg_commit(leader, &o_done[j & 1]);
       }
     }
     // every MMA has ended before tensor memory is released
     pg_commit(leader, &mma_idle);
     pg_wait(&mma_idle, 0, a.err);
-  } else if (warp == 2) {
-    // ---------------- V tiles that are not attended to entirely ----------------
+  } else {
+    // ---------------- warps 2, 3: V tiles that are not attended to entirely ----------------
     bool ok = true;
     for (int j = 0; ok && j < nt; ++j) {
-      const int t = 2 * j + 1, s = t % S;
-      ok = __all_sync(0xffffffffu, pg_wait(&kv_full[s], (uint32_t)((t / S) & 1), a.err));
+      const int t = v_at(j), s = stage_of(t);
+      ok = __all_sync(0xffffffffu, pg_wait(&kv_full[s], (uint32_t)(use_of(t) & 1), a.err));
       if (!ok) break;
       const int key0 = (u.tile0 + j) * TN;
       if (key0 + TN - 1 > first_pos || key0 < lo_last) {
-        unsigned char* v = ring + s * C::kStage;
         bool bad = false;
+        // keys [a, b) of the tile
+        auto check = [&](int ka, int kb) {
+          const int n = (kb - ka) * 8;  // 16-byte pieces of a 64-column block
+#pragma unroll 1
+          for (int c = 0; c < HD / 64; ++c) {
+            unsigned char* v = ring + s * C::kStage + c * (TN * 128) + (ka - key0) * 128;
 #pragma unroll 4
-        for (int x = lane; x < TN * HD / 8; x += 32) {  // 16-byte pieces: column block, key, piece
-          const int key = key0 + (x / 8) % TN;
-          uint4* p = reinterpret_cast<uint4*>(v + x * 16);
-          if (key >= u.key_hi || key < lo_first) {
-            *p = make_uint4(0u, 0u, 0u, 0u);
-          } else {
-            uint4 w = *p;
-            if (pg_clean<__nv_bfloat16>(w)) {
-              *p = w;
-              bad = true;
+            for (int x = (warp - 2) * 32 + lane; x < n; x += 64) {
+              const int key = ka + x / 8;
+              uint4* p = reinterpret_cast<uint4*>(v + x * 16);
+              uint4 w = *p;
+              if (key >= u.key_hi || key < lo_first) {
+                *p = make_uint4(0u, 0u, 0u, 0u);
+              } else if (pg_clean<__nv_bfloat16>(w)) {
+                *p = w;
+                bad = true;
+              }
             }
           }
-        }
+        };
+        const int k1 = key0 + TN;
+        if (lo_last > key0) check(key0, min(k1, lo_last));                                           // some window starts behind them
+        if (first_pos + 1 < k1) check(max(max(key0, lo_last > key0 ? min(k1, lo_last) : key0), first_pos + 1), k1);  // some rows are before them
         if (bad) *reinterpret_cast<volatile int*>(&s_bad) = 1;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -433,13 +456,13 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
     const int b = (warp - 4) / 4;
     const int row = (warp & 3) * 32 + lane;  // of this Q tile
     const uint32_t lb = (uint32_t)((warp & 3) * 32) << 16;
-    const int rr = b * 128 + row;            // of the part
+    const int rr = dual ? row : b * 128 + row;  // of the part
     const bool valid = rr < u.n_rows;
     const int r = u.r0 + min(rr, u.n_rows - 1);
     const int tok = r / a.G, head = u.kvh * a.G + r % a.G;
     const int qpos = u.pos0 + tok;
     const int kmin = a.win ? max(0, qpos - a.window + 1) : 0;
-    {
+    if (!dual || b == 0) {
       const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) +
                                                         (long long)(u.q_row0 + tok) * a.q_stride + (long long)head * HD);
       unsigned char* dst = sq + b * (128 * HD * 2) + row * 128;
@@ -454,12 +477,11 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
     bool ok = true;
     const float sl = a.scale_log2;
     const uint32_t T_O = tm + C::kO + b * HD + lb;
-    for (int j = 0; j < nt; ++j) {
+    // this stream's key tiles: tile0 + step * j + first
+    const int step = dual ? 2 : 1, first = dual ? b : 0, n_mine = (nt - first + step - 1) / step;
+    for (int j = 0; j < n_mine; ++j) {
       const int slot = NQ == 2 ? b : j & 1;
       ok = __all_sync(0xffffffffu, pg_wait(&s_full[slot], (uint32_t)((NQ == 2 ? j : j >> 1) & 1), a.err));
-      // With S in two places softmax may be two tiles ahead of O; a barrier's parity tells only neighbouring phases apart,
-      // so every phase of o_done is waited for in turn.
-      if (NQ == 1 && ok && j > 1) ok = __all_sync(0xffffffffu, pg_wait(&o_done[b], (uint32_t)(j & 1), a.err));
       if (!ok) break;
       tc::fence_after_sync();
       const uint32_t T_S = tm + slot * C::kS + lb;
@@ -472,14 +494,20 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
         for (int i = 0; i < 32; ++i) sv[c * 32 + i] = t[i];
       }
       tc::wait_ld();
-      const int key0 = (u.tile0 + j) * TN;
+      const int key0 = (u.tile0 + step * j + first) * TN;
       if (!__all_sync(0xffffffffu, key0 >= kmin && key0 + TN - 1 <= qpos)) {
+        const int last = qpos - key0;
 #pragma unroll
         for (int c = 0; c < TN; ++c)
-          if (key0 + c > qpos || key0 + c < kmin) sv[c] = -INFINITY;
+          if (c > last) sv[c] = -INFINITY;
+        if (a.win) {
+          const int from = kmin - key0;
+#pragma unroll
+          for (int c = 0; c < TN; ++c)
+            if (c < from) sv[c] = -INFINITY;
+        }
       }
-      // p = 2^(s scale log2e - m scale log2e): of each eight pairs, kPoly by polynomial, the others on the special-function
-      // unit, whose 16 a cycle the two Q tiles' 32K would otherwise fill
+      // p = 2^(s scale log2e - m scale log2e)
       constexpr int N2 = TN / 2 / C::kHands;  // pairs of a part
       const f32x2 sl2 = pk2(sl, sl);
       f32x2 ls[2], neg2;
@@ -489,18 +517,11 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
         for (int c = 0; c < N2; ++c) {
           const int e = 2 * (hf * N2 + c);
           const f32x2 x = fma2(pk2(sv[e], sv[e + 1]), sl2, neg2);
-          f32x2 p;
           float p0, p1;
-          if ((c & 7) < C::kPoly) {
-            p = exp2_poly2(x);
-            un2(p, p0, p1);
-          } else {
-            un2(x, p0, p1);
-            p0 = fast_exp2(p0);
-            p1 = fast_exp2(p1);
-            p = pk2(p0, p1);
-          }
-          ls[c & 1] = add2(ls[c & 1], p);
+          un2(x, p0, p1);
+          p0 = fast_exp2(p0);
+          p1 = fast_exp2(p1);
+          ls[c & 1] = add2(ls[c & 1], pk2(p0, p1));
           pk[c] = pg_pack_bf16(p0, p1);
         }
       };
@@ -528,7 +549,7 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
           m = m_new;
         }
         if (j > 0) {
-          ok = __all_sync(0xffffffffu, pg_wait(&o_done[b], (uint32_t)((j - 1) & 1), a.err));
+          ok = __all_sync(0xffffffffu, pg_wait(&o_done[NQ == 2 ? b : (j - 1) & 1], (uint32_t)((NQ == 2 ? j - 1 : (j - 1) >> 1) & 1), a.err));
           if (!ok) break;
           tc::fence_after_sync();
 #pragma unroll 1
@@ -560,8 +581,38 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
       un2(ls[1], l2, l3);
       lsum += (l0 + l1) + (l2 + l3);
     }
-    if (NQ == 1 && ok && nt > 1) ok = __all_sync(0xffffffffu, pg_wait(&o_done[b], (uint32_t)(nt & 1), a.err));
-    if (ok) ok = __all_sync(0xffffffffu, pg_wait(&o_done[b], (uint32_t)((nt - 1) & 1), a.err));
+    // With S in two places softmax may be two tiles ahead of O, two phases that one barrier's parity would not tell apart:
+    // o_done is a barrier per place then.
+    if (ok)
+      ok = __all_sync(0xffffffffu, pg_wait(&o_done[NQ == 2 ? b : (n_mine - 1) & 1], (uint32_t)((NQ == 2 ? n_mine - 1 : (n_mine - 1) >> 1) & 1), a.err));
+    float f0 = 1.f, f1 = 0.f;  // factors of this stream's sums and the other's
+    float* xo = reinterpret_cast<float*>(ring);  // the odd stream's O, [column][row], where the tiles were
+    if constexpr (NQ == 2) {
+      if (dual && nq == 2) {
+        // Neither stream's MMAs read the tiles any more once both are done.
+        if (b == 1) {
+          if (ok) ok = __all_sync(0xffffffffu, pg_wait(&o_done[0], (uint32_t)(((nt + 1) / 2 - 1) & 1), a.err));
+          tc::fence_after_sync();
+          s_m1[row] = m;
+          s_l1[row] = lsum;
+#pragma unroll 1
+          for (int c = 0; c < HD / 32; ++c) {
+            float ov[32];
+            tc::ld32(T_O + c * 32, ov);
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) xo[(c * 32 + i) * 128 + row] = ov[i];
+          }
+        }
+        asm volatile("bar.sync 3, 256;" ::: "memory");
+        if (b == 1) ok = false;  // the even stream's warps write the rows
+        const float m1 = s_m1[row], mm = fmaxf(m, m1), base = mm == -INFINITY ? 0.f : mm;
+        f0 = fast_exp2((m - base) * sl);
+        f1 = fast_exp2((m1 - base) * sl);
+        lsum = lsum * f0 + s_l1[row] * f1;
+        m = mm;
+      }
+    }
     if (ok) {
       tc::fence_after_sync();
       const bool split = u.n_parts > 1;
@@ -575,6 +626,10 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
         float ov[32];
         tc::ld32(T_O + c * 32, ov);
         tc::wait_ld();
+        if (NQ == 2 && dual && nq == 2) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) ov[i] = ov[i] * f0 + xo[(c * 32 + i) * 128 + row] * f1;
+        }
         if (bad && valid) {
           for (int key = max(kmin, u.tile0 * TN); key <= min(qpos, u.tile1 * TN - 1); ++key) {
             const int key0 = key / TN * TN;
