@@ -287,30 +287,62 @@ void plan_tc(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vec
     const int n = u.tile1 - u.tile0, w = weight(u), cap = (int)std::max<long long>(least, (share + w - 1) / w);
     return (n + cap - 1) / cap;
   };
-  // the smallest share with which all parts run at once; with more units than that the longest go first and are cut
-  // only when one of them is longer than an SM's part of everything
+  // The share of a part.  Candidates: the smallest with which all parts run at once, and fractions of an SM's part of
+  // everything, whose parts come in more than one wave but even out ragged lengths; each is judged by laying its parts,
+  // longest first, on the SMs that are free first.  A part's start costs about 4.5K cycles, the merge's launch 5K.
+  const double start = ctx->bf16 ? (rt == 256 ? 6 : 2) : 1, join = start;
   long long total = 0, longest = 0;
   for (const auto& u : units) {
     const long long c = (long long)weight(u) * (u.tile1 - u.tile0);
     total += c;
     longest = std::max(longest, c);
   }
-  long long share = (total + wide - 1) / wide;
-  if ((int)units.size() <= wide) {
+  const long long even = std::max<long long>(1, (total + wide - 1) / wide);
+  long long share = even;
+  if ((int)units.size() <= 2 * wide) {
     auto count = [&](long long s) {
       long long n = 0;
       for (const auto& u : units) n += parts_of(u, s);
       return n;
     };
-    long long lo = std::max<long long>(share, 1), hi = std::max(longest, lo);
-    while (lo < hi) {
-      const long long mid = (lo + hi) / 2;
-      if (count(mid) <= wide)
-        hi = mid;
-      else
-        lo = mid + 1;
+    auto makespan = [&](long long s) {
+      std::vector<double> cost;
+      bool split = false;
+      for (const auto& u : units) {
+        const int k = parts_of(u, s);
+        split |= k > 1;
+        cost.insert(cost.end(), k, start + (double)weight(u) * (u.tile1 - u.tile0) / k);
+      }
+      std::sort(cost.begin(), cost.end(), std::greater<double>());
+      std::vector<double> sm(wide, 0.0);  // a min-heap of the times at which SMs are free
+      double end = 0;
+      for (double c : cost) {
+        std::pop_heap(sm.begin(), sm.end(), std::greater<double>());
+        sm.back() += c;
+        end = std::max(end, sm.back());
+        std::push_heap(sm.begin(), sm.end(), std::greater<double>());
+      }
+      return end + (split ? join : 0);
+    };
+    std::vector<long long> tries;
+    if ((int)units.size() <= wide) {
+      long long lo = even, hi = std::max(longest, lo);
+      while (lo < hi) {
+        const long long mid = (lo + hi) / 2;
+        if (count(mid) <= wide)
+          hi = mid;
+        else
+          lo = mid + 1;
+      }
+      tries.push_back(hi);
     }
-    share = hi;
+    for (int f = 1; f <= 3; ++f) tries.push_back(std::max<long long>(1, even / f));
+    double best = 1e300;
+    for (long long s : tries) {
+      if (count(s) > 2 * wide) continue;  // the workspace's parts
+      const double m = makespan(s);
+      if (m < best) best = m, share = s;
+    }
   }
   int slot = 0;
   for (const auto& u : units) {

@@ -42,8 +42,7 @@ int init_tc(l3p_paged_ctx* ctx) {
         return (int)L3P_OK;
       }))
     return rc;
-  // a unit is split when it is longer than 1/num_sms of all tiles, into at most
-  // 1 + its share parts: fewer than 2 num_sms parts of fewer than num_sms units
+  // plan_tc makes at most 2 num_sms parts of the units that it splits
   const size_t rows_ws = 2 * (size_t)ctx->num_sms * tc_rows(ctx);
   if (cudaMalloc(&ctx->tc_o, rows_ws * ctx->hd * sizeof(float)) != cudaSuccess ||
       cudaMalloc(&ctx->tc_ml, rows_ws * 2 * sizeof(float)) != cudaSuccess) {
