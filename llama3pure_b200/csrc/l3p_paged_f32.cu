@@ -67,7 +67,7 @@ static int chunks(l3p_paged_ctx* ctx, PgF32Args a, const PgLists& l, cudaStream_
     a.kvh0 = h;
     a.n_kvh = std::min(group, n_kv - h);
     if (int rc = launch(ctx, paged_prep_kernel<CG, HD>, dim3(l.n_prep, a.n_kvh), 256, 0, s, 1, a)) return rc;
-    if (int rc = launch(ctx, paged_f32_kernel<CG, HD>, dim3(l.n_tc * CG), 384, PgF32Cfg<CG, HD>::kSmem, s, CG, a)) return rc;
+    if (int rc = launch(ctx, paged_f32_kernel<CG, HD>, dim3(l.n_tc * CG), 512, PgF32Cfg<CG, HD>::kSmem, s, CG, a)) return rc;
   }
   return L3P_OK;
 }

@@ -24,9 +24,10 @@
 // CG = 2 (head_dim 128): the CTAs of a pair take 128 rows each of the same KV
 // head; every MMA is cta_group::2 with M = 256, and each CTA stages half of
 // every chunk.  CG = 1 for head_dim 64.
-// Roles (384 threads per CTA): warps 0, 2 load chunks in turn (1-D bulk copies);
+// Roles (512 threads per CTA): warps 0, 2 load chunks in turn (1-D bulk copies);
 // warp 1 issues S (the odd CTA's relays landed chunks), warp 3 issues P V; warps
-// 4-7 softmax, thread = row; warps 8-11 hold O, thread = row.
+// 4-7 and 8-11 are the softmax of a tile's first and last 64 keys, thread = row
+// (one warpgroup for all 128 took 11K cycles a tile); warps 12-15 hold O, thread = row.
 #pragma once
 #include "paged_tc.cuh"
 #include "prefill_tc.cuh"
@@ -39,7 +40,7 @@ template <int CG, int HD>
 struct PgF32Cfg {
   static constexpr int kStages = PfCfg<CG, HD>::kStages - 1;
   static constexpr int kSmem = PfGeom<HD>::kQloBytes + kStages * PfCfg<CG, HD>::kStageBytes + 1024;
-  static_assert(kStages >= PfGeom<HD>::kKChunks + 1 && kSmem <= 232448 - 3072, "shared memory");
+  static_assert(kStages >= PfGeom<HD>::kKChunks + 1 && kSmem <= 232448 - 6144, "shared memory");
 };
 
 struct PgF32Args {
@@ -117,15 +118,15 @@ __global__ void paged_prep_kernel(const PgF32Args a) {
 }
 
 template <int CG, int HD>
-__global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
+__global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
   using C = PfCfg<CG, HD>;
   using Gm = PfGeom<HD>;
   constexpr int S = PgF32Cfg<CG, HD>::kStages;
   extern __shared__ unsigned char f32_smem_raw[];
   __shared__ uint32_t s_tmem;
-  __shared__ float s_alpha[2][128], s_m[128], s_l[128];
+  __shared__ float s_alpha[2][128], s_m[128], s_l[2][128], s_max[2][2][128];
   __shared__ __align__(8) uint64_t bar_kv_full[S], bar_kv_empty[S], bar_kv_peer[S];
-  __shared__ __align__(8) uint64_t bar_s_full, bar_s_free, bar_p_full[2], bar_p_free[2];
+  __shared__ __align__(8) uint64_t bar_s_full, bar_s_free, bar_p_full[2], bar_p_free[2][2];
   __shared__ __align__(8) uint64_t bar_o_full, bar_o_free, bar_q_ready, bar_sm_done, bar_mma_idle[2];
 
   const PgHeader* hd = reinterpret_cast<const PgHeader*>(a.batch);
@@ -161,16 +162,17 @@ __global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
       mbar_init(&bar_kv_peer[s], 1);
     }
     mbar_init(&bar_s_full, 1);
-    mbar_init(&bar_s_free, 4 * CG);
+    mbar_init(&bar_s_free, 8 * CG);
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bar_p_full[b], 4 * CG);
-      mbar_init(&bar_p_free[b], 1);
+      mbar_init(&bar_p_free[0][b], 1);
+      mbar_init(&bar_p_free[1][b], 1);
       mbar_init(&bar_mma_idle[b], 1);
     }
     mbar_init(&bar_o_full, 1);
     mbar_init(&bar_o_free, 4 * CG);
-    mbar_init(&bar_q_ready, 4 * CG);
-    mbar_init(&bar_sm_done, 4);
+    mbar_init(&bar_q_ready, 8 * CG);
+    mbar_init(&bar_sm_done, 8);
     fence_mbar_init();
   }
   tc::fence_before_sync();
@@ -209,7 +211,9 @@ __global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
   const int kmin = a.win ? max(0, qpos - a.window + 1) : 0;
   const uint32_t lb = (uint32_t)((warp & 3) * 32) << 16;
 
+  // registers: 512 x 128 at launch >= 128 x 56 + 256 x 120 + 128 x 208
   if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 || warp == 2) {
       // ---------------- producers, chunks in turn ----------------
       if (lane == 0) {
@@ -324,7 +328,7 @@ __global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) tc::mma_tf32_ts_g<CG>(T_O, p_hi + ks * 8, desc_add(vh, ks * 1024), id_o, true);
             commit_all(&bar_kv_empty[c % S]);
-            commit_all(&bar_p_free[slot]);
+            commit_all(&bar_p_free[qq >> 1][slot]);
             if (slot == 1) commit_all(&bar_o_full);
           }
         }
@@ -332,12 +336,14 @@ __global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
         wait(&bar_mma_idle[1], 0);
       }
     }
-  } else if (warp < 8) {
-    // ---------------- softmax: thread = row ----------------
+  } else if (warp < 12) {
+    // ---------------- softmax: thread = row and half of the tile's keys ----------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+    const int half = (warp - 4) >> 2;
     {
       const float4* src = reinterpret_cast<const float4*>(a.q + (long long)(u.q_row0 + tok) * a.q_stride + (long long)head * HD);
 #pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
+      for (int c = half; c < HD / 32; c += 2) {
         float hi[32], lo[32];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -363,13 +369,12 @@ __global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
     bool ok = true;
     for (int j = 0; j < nt; ++j) {
       ok = __all_sync(0xffffffffu, wait(&bar_s_full, (uint32_t)(j & 1)));
-      if (!ok) break;
       tc::fence_after_sync();
-      float sv[kPfBN];
+      float sv[64];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         float t[32];
-        tc::ld32(T_S + lb + c * 32, t);
+        tc::ld32(T_S + lb + half * 64 + c * 32, t);
 #pragma unroll
         for (int i = 0; i < 32; ++i) sv[c * 32 + i] = t[i];
       }
@@ -377,54 +382,63 @@ __global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) arrive_issuer(&bar_s_free);
-      const int key0 = (u.tile0 + j) * kPfBN;
-      const bool full = __all_sync(0xffffffffu, key0 >= kmin && key0 + kPfBN - 1 <= qpos);
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      const int key0 = (u.tile0 + j) * kPfBN + half * 64;
+      if (!__all_sync(0xffffffffu, key0 >= kmin && key0 + 63 <= qpos)) {
+        const int last = qpos - key0, from = kmin - key0;
 #pragma unroll
-      for (int c = 0; c < kPfBN; ++c) {
-        sv[c] *= a.scale_log2;
-        if (!full && (key0 + c > qpos || key0 + c < kmin)) sv[c] = -INFINITY;
-        mx[c & 3] = fmaxf(mx[c & 3], sv[c]);
+        for (int c = 0; c < 64; ++c)
+          if (c > last || c < from) sv[c] = -INFINITY;
       }
-      const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+      float mx[4] = {sv[0], sv[1], sv[2], sv[3]};
+#pragma unroll
+      for (int c = 4; c < 60; c += 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], sv[c + 2 * i], sv[c + 2 * i + 1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], sv[60 + i]);
+      s_max[j & 1][half][row] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      // both halves of a row meet here once a tile, whether their waits succeeded or not
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      if (!ok) break;
+      const float m_new = fmaxf(m, fmaxf(s_max[j & 1][0][row], s_max[j & 1][1][row]) * a.scale_log2);
       const float base = m_new == -INFINITY ? 0.f : m_new;
       const float alpha = fast_exp2(m - base);
       m = m_new;
-      s_alpha[j & 1][row] = alpha;
+      if (half == 0) s_alpha[j & 1][row] = alpha;
       lsum *= alpha;
 #pragma unroll
-      for (int qq = 0; qq < 4; ++qq) {
-        const int slot = qq & 1;
-        if (j >= 1 || qq >= 2) {
-          // the slot's quarter before has been multiplied: p_free[slot] number 2 j + qq / 2 - 1
-          ok = __all_sync(0xffffffffu, wait(&bar_p_free[slot], (uint32_t)((qq >> 1) ^ 1)));
-          if (!ok) break;
-          tc::fence_after_sync();
-        }
-        float ph[32], pl[32], ls = 0.f;
+      for (int qq = 0; qq < 2; ++qq) {
+        float ph[32], pl[32], ls[2] = {0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
-          const float p = fast_exp2(sv[qq * 32 + c] - base);
-          ls += p;
+          const float p = fast_exp2(fmaf(sv[qq * 32 + c], a.scale_log2, -base));
+          ls[c & 1] += p;
           ph[c] = pg_tf32(p);
           pl[c] = p - ph[c];
         }
-        lsum += ls;
-        tc::st32(T_P + lb + slot * 64, ph);
-        tc::st32(T_P + lb + slot * 64 + 32, pl);
+        lsum += ls[0] + ls[1];
+        if (j >= 1 || half > 0) {
+          // the slot's quarter before, the other half's, has been multiplied (a barrier for each half: of one that both
+          // halves' quarters complete, a warpgroup could be two phases behind)
+          ok = __all_sync(0xffffffffu, wait(&bar_p_free[half ^ 1][qq], (uint32_t)((half ? j : j - 1) & 1)));
+          tc::fence_after_sync();
+        }
+        tc::st32(T_P + lb + qq * 64, ph);
+        tc::st32(T_P + lb + qq * 64 + 32, pl);
         tc::wait_st();
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) arrive_issuer(&bar_p_full[slot]);
+        if (lane == 0 && ok) arrive_issuer(&bar_p_full[qq]);
       }
-      if (!ok) break;
     }
-    s_m[row] = m;
-    s_l[row] = lsum;
+    if (half == 0) s_m[row] = m;
+    s_l[half][row] = lsum;
     __syncwarp();
     if (lane == 0) mbar_arrive(&bar_sm_done);
   } else {
     // ---------------- O: thread = row ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     float acc[HD];
 #pragma unroll
     for (int i = 0; i < HD; ++i) acc[i] = 0.f;
@@ -463,7 +477,7 @@ __global__ void __launch_bounds__(384, 1) paged_f32_kernel(const PgF32Args a) {
           }
         }
       }
-      const float lsum = s_l[row];
+      const float lsum = s_l[0][row] + s_l[1][row];
       const bool split = u.n_parts > 1;
       if (!split) {
         const float inv = 1.f / lsum;
