@@ -117,6 +117,52 @@ __global__ void paged_prep_kernel(const PgF32Args a) {
   if (threadIdx.x == 0) a.flags[slot] = bad;
 }
 
+// MMAs and commits as in tc.cuh, issued by the lane for which `leader` is set in code that the whole warp runs (see
+// mma_bf16_ss).
+template <int CG>
+__device__ __forceinline__ void pg_tf32_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc),
+        "r"(leader)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc),
+        "r"(leader)
+        : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void pg_tf32_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::tf32 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc),
+        "r"(leader)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc),
+        "r"(leader)
+        : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void pg_commit_g(uint32_t leader, uint32_t bar_cluster_addr) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar_cluster_addr), "r"(leader)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar_cluster_addr), "r"(leader)
+        : "memory");
+}
+
 template <int CG, int HD>
 __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
   using C = PfCfg<CG, HD>;
@@ -197,9 +243,9 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
     else
       mbar_arrive(bar);
   };
-  auto commit_all = [&](uint64_t* bar) {
-    tc::commit_g<CG>(smem_addr(bar));
-    if constexpr (CG == 2) tc::commit_g<CG>(mapa_shared(smem_addr(bar), 1));
+  auto commit_all = [&](uint32_t leader, uint64_t* bar) {
+    pg_commit_g<CG>(leader, smem_addr(bar));
+    if constexpr (CG == 2) pg_commit_g<CG>(leader, mapa_shared(smem_addr(bar), 1));
   };
   // row of this thread (softmax and O warpgroups); rows behind the last one compute what it computes
   const int row = (warp & 3) * 32 + lane;
@@ -255,54 +301,56 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
           if (!wait(&bar_kv_full[c % S], (uint32_t)((c / S) & 1))) break;
           mbar_arrive_cluster(mapa_shared(smem_addr(&bar_kv_peer[c % S]), 0));
         }
-    } else if (rank == 0 && lane == 0) {
+    } else if (rank == 0) {
       // ---------------- MMA issuers: warp 1 S, warp 3 O ----------------
       constexpr int nK = Gm::kKChunks, nKV = Gm::kChunks;
+      uint32_t leader;
+      asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, wait(bar, parity)); };
       auto k_chunk0 = [&](int t) { return t == 0 ? 0 : nK + (t - 1) * nKV; };
       auto v_chunk0 = [&](int t) { return t + 1 < nt ? 2 * nK + t * nKV : nK + t * nKV; };
-      auto chunk_ready = [&](int c, uint32_t& off) -> bool {
+      auto chunk_ready = [&](int c) -> bool {
         const int s = c % S, use = c / S;
-        off = (uint32_t)(s * C::kStageBytes);
-        if (!wait(&bar_kv_full[s], (uint32_t)(use & 1))) return false;
-        if (CG == 2 && !wait(&bar_kv_peer[s], (uint32_t)(use & 1))) return false;
+        if (!wait_all(&bar_kv_full[s], (uint32_t)(use & 1))) return false;
+        if (CG == 2 && !wait_all(&bar_kv_peer[s], (uint32_t)(use & 1))) return false;
         tc::fence_after_sync();
         return true;
       };
+      auto stage = [&](int c) { return (uint32_t)((c % S) * C::kStageBytes); };
       bool ok = true;
       if (warp == 1) {
         constexpr uint32_t id_s = tc::idesc_tf32(kPfBM * CG, kPfBN, false);
         const uint64_t qlo_d = tc::sdesc_sw128(smem_addr(qlo), 16, 1024);
         const uint64_t k_d = tc::sdesc_sw128(smem_addr(ring), 16, 1024);
-        ok = wait(&bar_q_ready, 0);
+        ok = wait_all(&bar_q_ready, 0);
         tc::fence_after_sync();
         for (int t = 0; ok && t < nt; ++t) {
           if (t >= 1) {
-            if (!(ok = wait(&bar_s_free, (uint32_t)((t - 1) & 1)))) break;
+            if (!(ok = wait_all(&bar_s_free, (uint32_t)((t - 1) & 1)))) break;
             tc::fence_after_sync();
           }
-          uint32_t off[nK];
-#pragma unroll
+#pragma unroll 1
           for (int ch = 0; ch < nK; ++ch) {  // the small products
-            if (!(ok = chunk_ready(k_chunk0(t) + ch, off[ch]))) break;
-            const uint64_t kh = desc_add(k_d, off[ch]), kl = desc_add(k_d, off[ch] + C::kStageBytes / 2);
+            if (!(ok = chunk_ready(k_chunk0(t) + ch))) break;
+            const uint64_t kh = desc_add(k_d, stage(k_chunk0(t) + ch)), kl = desc_add(kh, C::kStageBytes / 2);
+            const uint64_t ql = desc_add(qlo_d, ch * 16384);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
-              tc::mma_tf32_ts_g<CG>(T_S, T_QHI + ch * 32 + kk * 8, desc_add(kl, kk * 32), id_s, ch > 0 || kk > 0);
-              tc::mma_tf32_ss_g<CG>(T_S, desc_add(qlo_d, ch * 16384 + kk * 32), desc_add(kh, kk * 32), id_s, true);
+              pg_tf32_ts<CG>(leader, T_S, T_QHI + ch * 32 + kk * 8, desc_add(kl, kk * 32), id_s, ch > 0 || kk > 0);
+              pg_tf32_ss<CG>(leader, T_S, desc_add(ql, kk * 32), desc_add(kh, kk * 32), id_s, true);
             }
           }
           if (!ok) break;
-#pragma unroll
+#pragma unroll 1
           for (int ch = 0; ch < nK; ++ch) {  // hi * hi
-            const uint64_t kh = desc_add(k_d, off[ch]);
+            const uint64_t kh = desc_add(k_d, stage(k_chunk0(t) + ch));
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              tc::mma_tf32_ts_g<CG>(T_S, T_QHI + ch * 32 + kk * 8, desc_add(kh, kk * 32), id_s, true);
-            commit_all(&bar_kv_empty[(k_chunk0(t) + ch) % S]);
+            for (int kk = 0; kk < 4; ++kk) pg_tf32_ts<CG>(leader, T_S, T_QHI + ch * 32 + kk * 8, desc_add(kh, kk * 32), id_s, true);
+            commit_all(leader, &bar_kv_empty[(k_chunk0(t) + ch) % S]);
           }
-          commit_all(&bar_s_full);
+          commit_all(leader, &bar_s_full);
         }
-        tc::commit_g<CG>(smem_addr(&bar_mma_idle[0]));
+        pg_commit_g<CG>(leader, smem_addr(&bar_mma_idle[0]));
         wait(&bar_mma_idle[0], 0);
       } else {
         constexpr uint32_t id_o = tc::idesc_tf32(kPfBM * CG, HD, true);
@@ -311,28 +359,27 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
 #pragma unroll 1
           for (int qq = 0; ok && qq < Gm::kVChunks; ++qq) {
             const int c = v_chunk0(t) + qq, slot = qq & 1;
-            uint32_t off;
-            if (!(ok = chunk_ready(c, off))) break;
-            if (!(ok = wait(&bar_p_full[slot], (uint32_t)((qq >> 1) & 1)))) break;
+            if (!(ok = chunk_ready(c))) break;
             // a new partial sum every 64 keys: the one before has been taken
             const int half = 2 * t + (qq >> 1);
-            if (slot == 0 && half >= 1 && !(ok = wait(&bar_o_free, (uint32_t)((half - 1) & 1)))) break;
+            if (slot == 0 && half >= 1 && !(ok = wait_all(&bar_o_free, (uint32_t)((half - 1) & 1)))) break;
+            if (!(ok = wait_all(&bar_p_full[slot], (uint32_t)((qq >> 1) & 1)))) break;
             tc::fence_after_sync();
-            const uint64_t vh = desc_add(v_d, off), vl = desc_add(v_d, off + C::kVBytes / 2);
+            const uint64_t vh = desc_add(v_d, stage(c)), vl = desc_add(vh, C::kVBytes / 2);
             const uint32_t p_hi = T_P + slot * 64, p_lo = p_hi + 32;
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
-              tc::mma_tf32_ts_g<CG>(T_O, p_hi + ks * 8, desc_add(vl, ks * 1024), id_o, slot > 0 || ks > 0);
-              tc::mma_tf32_ts_g<CG>(T_O, p_lo + ks * 8, desc_add(vh, ks * 1024), id_o, true);
+              pg_tf32_ts<CG>(leader, T_O, p_hi + ks * 8, desc_add(vl, ks * 1024), id_o, slot > 0 || ks > 0);
+              pg_tf32_ts<CG>(leader, T_O, p_lo + ks * 8, desc_add(vh, ks * 1024), id_o, true);
             }
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) tc::mma_tf32_ts_g<CG>(T_O, p_hi + ks * 8, desc_add(vh, ks * 1024), id_o, true);
-            commit_all(&bar_kv_empty[c % S]);
-            commit_all(&bar_p_free[qq >> 1][slot]);
-            if (slot == 1) commit_all(&bar_o_full);
+            for (int ks = 0; ks < 4; ++ks) pg_tf32_ts<CG>(leader, T_O, p_hi + ks * 8, desc_add(vh, ks * 1024), id_o, true);
+            commit_all(leader, &bar_kv_empty[c % S]);
+            commit_all(leader, &bar_p_free[qq >> 1][slot]);
+            if (slot == 1) commit_all(leader, &bar_o_full);
           }
         }
-        tc::commit_g<CG>(smem_addr(&bar_mma_idle[1]));
+        pg_commit_g<CG>(leader, smem_addr(&bar_mma_idle[1]));
         wait(&bar_mma_idle[1], 0);
       }
     }
