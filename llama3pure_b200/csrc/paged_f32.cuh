@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
   __shared__ float s_alpha[2][128], s_m[128], s_l[2][128], s_max[2][2][128];
   __shared__ __align__(8) uint64_t bar_kv_full[S], bar_kv_empty[S], bar_kv_peer[S];
   __shared__ __align__(8) uint64_t bar_s_full, bar_s_free, bar_p_full[2], bar_p_free[2][2];
-  __shared__ __align__(8) uint64_t bar_o_full, bar_o_free, bar_q_ready, bar_sm_done, bar_mma_idle[2];
+  __shared__ __align__(8) uint64_t bar_o_full, bar_o_free, bar_q_ready, bar_sm_done, bar_alpha[2], bar_mma_idle[2];
 
   const PgHeader* hd = reinterpret_cast<const PgHeader*>(a.batch);
   const PgLists l = hd->lists[a.win];
@@ -214,6 +214,7 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
       mbar_init(&bar_p_free[0][b], 1);
       mbar_init(&bar_p_free[1][b], 1);
       mbar_init(&bar_mma_idle[b], 1);
+      mbar_init(&bar_alpha[b], 4);
     }
     mbar_init(&bar_o_full, 1);
     mbar_init(&bar_o_free, 4 * CG);
@@ -231,15 +232,13 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
   griddep_wait();  // the images and q come from the kernels before this one
   const uint32_t T_QHI = tm + 0, T_O = tm + HD, T_S = tm + 2 * HD, T_P = tm + 2 * HD + kPfBN;
 
-  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-    for (uint32_t i = 0; i < (1u << 18); ++i)
-      if (CG == 2 ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
-    *reinterpret_cast<volatile int*>(a.err) = kErrTimeout;
-    return false;
-  };
+  // Barriers that carry tensor memory, copies that have landed or room (not ordinary stores) between the CTAs of a pair are
+  // used at their default scope: with .release.cluster / .acquire.cluster every arrive and poll is a memory barrier of
+  // 300 to 1000 cycles, of which a tile has 40.
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool { return pg_wait(bar, parity, a.err); };
   auto arrive_issuer = [&](uint64_t* bar) {
     if constexpr (CG == 2)
-      mbar_arrive_cluster(mapa_shared(smem_addr(bar), 0));
+      asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mapa_shared(smem_addr(bar), 0)) : "memory");
     else
       mbar_arrive(bar);
   };
@@ -299,7 +298,7 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
       if (lane == 0)  // relay: chunk landed here -> issuers
         for (int c = 0; c < Gm::kChunks * nt; ++c) {
           if (!wait(&bar_kv_full[c % S], (uint32_t)((c / S) & 1))) break;
-          mbar_arrive_cluster(mapa_shared(smem_addr(&bar_kv_peer[c % S]), 0));
+          asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mapa_shared(smem_addr(&bar_kv_peer[c % S]), 0)) : "memory");
         }
     } else if (rank == 0) {
       // ---------------- MMA issuers: warp 1 S, warp 3 O ----------------
@@ -322,7 +321,7 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
         constexpr uint32_t id_s = tc::idesc_tf32(kPfBM * CG, kPfBN, false);
         const uint64_t qlo_d = tc::sdesc_sw128(smem_addr(qlo), 16, 1024);
         const uint64_t k_d = tc::sdesc_sw128(smem_addr(ring), 16, 1024);
-        ok = wait_all(&bar_q_ready, 0);
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded_cluster(&bar_q_ready, 0, a.err));
         tc::fence_after_sync();
         for (int t = 0; ok && t < nt; ++t) {
           if (t >= 1) {
@@ -410,7 +409,12 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) arrive_issuer(&bar_q_ready);
+      if (lane == 0) {
+        if constexpr (CG == 2)
+          mbar_arrive_cluster(mapa_shared(smem_addr(&bar_q_ready), 0));  // ordinary stores: the image of Q lo
+        else
+          mbar_arrive(&bar_q_ready);
+      }
     }
     float m = -INFINITY, lsum = 0.f;
     bool ok = true;
@@ -452,7 +456,11 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
       const float base = m_new == -INFINITY ? 0.f : m_new;
       const float alpha = fast_exp2(m - base);
       m = m_new;
-      if (half == 0) s_alpha[j & 1][row] = alpha;
+      if (half == 0) {
+        s_alpha[j & 1][row] = alpha;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_alpha[j & 1]);
+      }
       lsum *= alpha;
 #pragma unroll
       for (int qq = 0; qq < 2; ++qq) {
@@ -492,6 +500,7 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
     bool ok = true;
     for (int x = 0; ok && x < 2 * nt; ++x) {
       ok = __all_sync(0xffffffffu, wait(&bar_o_full, (uint32_t)(x & 1)));
+      if (ok && !(x & 1)) ok = __all_sync(0xffffffffu, wait(&bar_alpha[(x >> 1) & 1], (uint32_t)((x >> 2) & 1)));
       if (!ok) break;
       tc::fence_after_sync();
       const float f = x & 1 ? 1.f : s_alpha[(x >> 1) & 1][row];
