@@ -59,14 +59,14 @@ static int chunks(l3p_paged_ctx* ctx, PgF32Args a, const PgLists& l, cudaStream_
   const int n_kv = ctx->cfg.n_kv_heads;
   const size_t fit = std::max<size_t>(1, kImageBytes / (tile * sizeof(float) * l.n_prep));
   const int group = (int)std::min<size_t>(fit, n_kv);
-  if (int rc = ensure_images(ctx, tile * l.n_prep * group, (size_t)l.n_prep * group, s)) return rc;
+  if (int rc = ensure_images(ctx, tile * l.n_prep * group, 4 * (size_t)l.n_prep * group, s)) return rc;
   ctx->img_captured |= capturing(s);
   a.img = ctx->img;
   a.flags = ctx->v_flags;
   for (int h = 0; h < n_kv; h += group) {
     a.kvh0 = h;
     a.n_kvh = std::min(group, n_kv - h);
-    if (int rc = launch(ctx, paged_prep_kernel<CG, HD>, dim3(l.n_prep, a.n_kvh), 256, 0, s, 1, a)) return rc;
+    if (int rc = launch(ctx, paged_prep_kernel<CG, HD>, dim3(l.n_prep, a.n_kvh, 4), 256, 0, s, 1, a)) return rc;
     if (int rc = launch(ctx, paged_f32_kernel<CG, HD>, dim3(l.n_tc * CG), 512, PgF32Cfg<CG, HD>::kSmem, s, CG, a)) return rc;
   }
   return L3P_OK;

@@ -51,7 +51,7 @@ struct PgF32Args {
   const float* storage;   // the layer's K block of page 0, head 0
   long long page_elems, v_off;
   float* img;             // [head of the group of heads][n_prep] tile images
-  int* flags;             // [head][n_prep]: the tile's V holds values that are not finite (0 in the image)
+  int* flags;             // [head][n_prep][4]: 32 keys' V hold values that are not finite (0 in the image)
   int kvh0, n_kvh;        // group of KV heads of this launch
   int shift, G, win, window;
   PgLimits lim;
@@ -63,7 +63,7 @@ struct PgF32Args {
 
 __device__ __forceinline__ float pg_tf32(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xFFFFE000u); }
 
-// Tile images of the keys that the batch's chunks attend to.  grid (tiles, KV heads of the group), 256 threads.
+// Tile images of the keys that the batch's chunks attend to.  grid (tiles, KV heads of the group, 4: 32 keys each), 256 threads.
 template <int CG, int HD>
 __global__ void paged_prep_kernel(const PgF32Args a) {
   using C = PfCfg<CG, HD>;
@@ -82,8 +82,8 @@ __global__ void paged_prep_kernel(const PgF32Args a) {
   constexpr int kVBase = Gm::kKChunks * C::kKBytes;
   int bad = 0;
 #pragma unroll 4
-  for (int idx = threadIdx.x; idx < kPfBN * HD / 4; idx += 256) {
-    const int key = idx / (HD / 4), c16 = idx % (HD / 4);
+  for (int idx = threadIdx.x; idx < 32 * HD / 4; idx += 256) {
+    const int key = blockIdx.z * 32 + idx / (HD / 4), c16 = idx % (HD / 4);
     const int pos = p.key0 + key;
     float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
     if (pos < p.key_hi) {
@@ -114,7 +114,7 @@ __global__ void paged_prep_kernel(const PgF32Args a) {
     *reinterpret_cast<float4*>(base + vb + C::kVBytes / 2) = vl;
   }
   bad = __syncthreads_or(bad);
-  if (threadIdx.x == 0) a.flags[slot] = bad;
+  if (threadIdx.x == 0) a.flags[4 * slot + blockIdx.z] = bad;
 }
 
 // MMAs and commits as in tc.cuh, issued by the lane for which `leader` is set in code that the whole warp runs (see
@@ -252,9 +252,12 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
   const bool valid = rr < u.n_rows;
   const int r = u.r0 + min(rr, u.n_rows - 1);
   const int tok = r / a.G, head = u.kvh * a.G + r % a.G;
+  const long long q_off = (long long)(u.q_row0 + tok) * a.q_stride + (long long)head * HD;
+  const long long o_off = (long long)(u.q_row0 + tok) * a.out_stride + (long long)head * HD;
   const int qpos = u.pos0 + tok;
   const int kmin = a.win ? max(0, qpos - a.window + 1) : 0;
   const uint32_t lb = (uint32_t)((warp & 3) * 32) << 16;
+  const bool any_row = (int)rank * 128 + (warp & 3) * 32 < u.n_rows;
 
   // registers: 512 x 128 at launch >= 128 x 56 + 256 x 120 + 128 x 208
   if (warp < 4) {
@@ -387,20 +390,35 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
     const int half = (warp - 4) >> 2;
     {
-      const float4* src = reinterpret_cast<const float4*>(a.q + (long long)(u.q_row0 + tok) * a.q_stride + (long long)head * HD);
-#pragma unroll 1
-      for (int c = half; c < HD / 32; c += 2) {
+      // This half's 32-column chunks of the warp's 32 rows: whole 128-byte lines into the place of the Q lo image, then every
+      // thread its row from there.
+      float4 t[HD / 64][8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float* src = a.q + __shfl_sync(0xffffffffu, q_off, i * 4 + (lane >> 3)) + (lane & 7) * 4;
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c) t[c][i] = *reinterpret_cast<const float4*>(src + (2 * c + half) * 32);
+      }
+#pragma unroll
+      for (int c = 0; c < HD / 64; ++c) {
+        unsigned char* img = qlo + (2 * c + half) * 16384;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int x = (warp & 3) * 32 + i * 4 + (lane >> 3);
+          *reinterpret_cast<float4*>(img + x * 128 + (((lane & 7) ^ (x & 7)) << 4)) = t[c][i];
+        }
+        __syncwarp();
+        unsigned char* rp = img + row * 128;
         float hi[32], lo[32];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float4 t = src[c * 8 + i];
-          hi[4 * i] = pg_tf32(t.x), lo[4 * i] = t.x - hi[4 * i];
-          hi[4 * i + 1] = pg_tf32(t.y), lo[4 * i + 1] = t.y - hi[4 * i + 1];
-          hi[4 * i + 2] = pg_tf32(t.z), lo[4 * i + 2] = t.z - hi[4 * i + 2];
-          hi[4 * i + 3] = pg_tf32(t.w), lo[4 * i + 3] = t.w - hi[4 * i + 3];
+          const float4 y = *reinterpret_cast<const float4*>(rp + ((i ^ (row & 7)) << 4));
+          hi[4 * i] = pg_tf32(y.x), lo[4 * i] = y.x - hi[4 * i];
+          hi[4 * i + 1] = pg_tf32(y.y), lo[4 * i + 1] = y.y - hi[4 * i + 1];
+          hi[4 * i + 2] = pg_tf32(y.z), lo[4 * i + 2] = y.z - hi[4 * i + 2];
+          hi[4 * i + 3] = pg_tf32(y.w), lo[4 * i + 3] = y.w - hi[4 * i + 3];
         }
-        tc::st32(T_QHI + lb + c * 32, hi);
-        unsigned char* rp = qlo + c * 16384 + row * 128;
+        tc::st32(T_QHI + lb + (2 * c + half) * 32, hi);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           *reinterpret_cast<float4*>(rp + ((i ^ (row & 7)) << 4)) = make_float4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
@@ -421,6 +439,17 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
     for (int j = 0; j < nt; ++j) {
       ok = __all_sync(0xffffffffu, wait(&bar_s_full, (uint32_t)(j & 1)));
       tc::fence_after_sync();
+      if (!any_row) {  // lanes without a row: S, P and O as they come (MMA rows are independent)
+        if (lane == 0) arrive_issuer(&bar_s_free);
+        asm volatile("bar.sync 2, 256;" ::: "memory");
+        if (!ok) break;
+        if (half == 0 && lane == 0) mbar_arrive(&bar_alpha[j & 1]);
+        for (int qq = 0; qq < 2; ++qq) {
+          if (j >= 1 || half > 0) ok = ok && __all_sync(0xffffffffu, wait(&bar_p_free[half ^ 1][qq], (uint32_t)((half ? j : j - 1) & 1)));
+          if (lane == 0 && ok) arrive_issuer(&bar_p_full[qq]);
+        }
+        continue;
+      }
       float sv[64];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -503,6 +532,10 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
       if (ok && !(x & 1)) ok = __all_sync(0xffffffffu, wait(&bar_alpha[(x >> 1) & 1], (uint32_t)((x >> 2) & 1)));
       if (!ok) break;
       tc::fence_after_sync();
+      if (!any_row) {
+        if (lane == 0) arrive_issuer(&bar_o_free);
+        continue;
+      }
       const float f = x & 1 ? 1.f : s_alpha[(x >> 1) & 1][row];
 #pragma unroll
       for (int c = 0; c < HD / 32; ++c) {
@@ -517,11 +550,12 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
       if (lane == 0) arrive_issuer(&bar_o_free);
     }
     if (ok) ok = __all_sync(0xffffffffu, wait(&bar_sm_done, 0));
-    if (ok) {
+    if (ok && any_row) {
       // values of V that are not finite, to the rows that attend to them
-      const int* flags = a.flags + img_slot;
+      const int* flags = a.flags + 4 * img_slot;
       for (int t = 0; t < nt; ++t) {
-        if (flags[t] == 0) continue;
+        const int4 f4 = reinterpret_cast<const int4*>(flags)[t];
+        if ((f4.x | f4.y | f4.z | f4.w) == 0) continue;
         const int key0 = (u.tile0 + t) * kPfBN;
         for (int key = max(kmin, key0); key <= min(qpos, key0 + kPfBN - 1); ++key) {
           const float* v = a.storage + a.v_off + (long long)table[key >> a.shift] * a.page_elems +
@@ -534,22 +568,26 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
         }
       }
       const float lsum = s_l[0][row] + s_l[1][row];
+      // rows through the ring, which no MMA reads any more, so that the warp stores whole rows
       const bool split = u.n_parts > 1;
-      if (!split) {
-        const float inv = 1.f / lsum;
-        float* dst = a.out + (long long)(u.q_row0 + tok) * a.out_stride + (long long)head * HD;
-        if (valid)
+      const float inv = split ? 1.f : 1.f / lsum;
+      unsigned char* buf = ring + (warp & 3) * (32 * HD * 4);
 #pragma unroll
-          for (int i = 0; i < HD; i += 4)
-            *reinterpret_cast<float4*>(dst + i) = make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
-      } else {
-        const long long ws_row = (long long)(u.slot + u.part) * (CG * 128) + rr;
-        if (valid) {
-#pragma unroll
-          for (int i = 0; i < HD; i += 4)
-            *reinterpret_cast<float4*>(a.ws_o + ws_row * HD + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-          *reinterpret_cast<float2*>(a.ws_ml + ws_row * 2) = make_float2(s_m[row], lsum);
-        }
+      for (int i = 0; i < HD / 4; ++i)
+        *reinterpret_cast<float4*>(buf + lane * (HD * 4) + ((i ^ (lane & 7)) << 4)) =
+            make_float4(acc[4 * i] * inv, acc[4 * i + 1] * inv, acc[4 * i + 2] * inv, acc[4 * i + 3] * inv);
+      __syncwarp();
+      const long long ws_row0 = (long long)(u.slot + u.part) * (CG * 128);
+      if (split && valid) *reinterpret_cast<float2*>(a.ws_ml + (ws_row0 + rr) * 2) = make_float2(s_m[row], lsum);
+      constexpr int kPieces = HD / 4, kRows = 32 / kPieces > 0 ? 32 / kPieces : 1;  // rows a warp stores at once
+#pragma unroll 4
+      for (int x = 0; x < 32 / kRows; ++x) {
+        const int y = x * kRows + lane / kPieces, pc = lane % kPieces;
+        const int yr = (int)rank * 128 + (warp & 3) * 32 + y;
+        const long long off = __shfl_sync(0xffffffffu, o_off, y);
+        float* dst = split ? a.ws_o + (ws_row0 + yr) * HD : a.out + off;
+        if (yr < u.n_rows)
+          *reinterpret_cast<float4*>(dst + 4 * pc) = *reinterpret_cast<const float4*>(buf + y * (HD * 4) + ((pc ^ (y & 7)) << 4));
       }
     }
   }

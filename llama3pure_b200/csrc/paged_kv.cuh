@@ -99,7 +99,8 @@ constexpr int kPgKvWarps = 8;
 template <typename T, int HD>
 __global__ void __launch_bounds__(kPgKvWarps * 32) paged_rope_kernel(const PgKvArgs a) {
   constexpr int N = HD / 32;
-  __shared__ __align__(16) float row_s[kPgKvWarps][HD];
+  constexpr int U = 4;  // rows that a warp turns at once
+  __shared__ __align__(16) float row_s[kPgKvWarps][U][HD];
   const PgHeader* h = reinterpret_cast<const PgHeader*>(a.batch);
   const int n_tok = h->n_tokens;
   griddep_launch();
@@ -145,7 +146,11 @@ __global__ void __launch_bounds__(kPgKvWarps * 32) paged_rope_kernel(const PgKvA
   const T* vt = static_cast<const T*>(a.v) + tok * a.v_stride + d0;
   T* qo = static_cast<T*>(a.q_out) + tok * a.q_out_stride + d0;
   const long long head_elems = (long long)a.page_size * HD;
-  constexpr int U = 4;  // rows in flight
+  float wq[N], wk[N];
+  if (a.q_norm != nullptr && r0 < a.n_heads + a.n_kv) {
+    pg_load<N>(a.q_norm + d0, wq);
+    pg_load<N>(a.k_norm + d0, wk);
+  }
   for (int r = r0; r < r1; r += U) {
     float x[U][N];
 #pragma unroll
@@ -156,46 +161,75 @@ __global__ void __launch_bounds__(kPgKvWarps * 32) paged_rope_kernel(const PgKvA
                                                : vt + (rr - a.n_heads - a.n_kv) * HD;
       pg_load<N>(src, x[u]);
     }
+    // the U rows together, so that their reductions and exchanges overlap; V rows are only copied
+    const bool turns = r < a.n_heads + a.n_kv;
+    if (turns && a.q_norm != nullptr) {
+      float ss[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        ss[u] = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) ss[u] += x[u][i] * x[u][i];
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u) ss[u] += __shfl_xor_sync(0xffffffffu, ss[u], o);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float f = 1.0f / sqrtf(ss[u] * (1.0f / HD) + a.eps);
+        if (r + u < a.n_heads + a.n_kv) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) x[u][i] = x[u][i] * f * (r + u < a.n_heads ? wq[i] : wk[i]);
+        }
+      }
+    }
+    if (turns && a.interleaved) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + u < a.n_heads + a.n_kv) {
+#pragma unroll
+          for (int i = 0; i < N; i += 2) {
+            const float p = x[u][i], q = x[u][i + 1];
+            if (d0 + i < a.rotary) {
+              x[u][i] = p * cs[i] + q * sn[i];
+              x[u][i + 1] = q * cs[i + 1] + p * sn[i + 1];
+            }
+          }
+        }
+    } else if (turns) {
+      __syncwarp();  // the rows before have been read
+#pragma unroll
+      for (int u = 0; u < U; ++u) pg_store<N>(row_s[warp][u] + d0, x[u]);
+      __syncwarp();
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + u < a.n_heads + a.n_kv) {
+          float y[N];  // the partners
+          if (half % N == 0) {
+            pg_load<N>(row_s[warp][u] + (d0 < half ? d0 + half : d0 < a.rotary ? d0 - half : d0), y);
+          } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              const int d = d0 + i;
+              y[i] = row_s[warp][u][d < half ? d + half : d < a.rotary ? d - half : d];
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (d0 + i < a.rotary) x[u][i] = x[u][i] * cs[i] + y[i] * sn[i];
+        }
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int rr = r + u;
       if (rr >= r1) break;
-      if (rr >= a.n_heads + a.n_kv) {
-        pg_store<N>(page_k + a.v_off + (rr - a.n_heads - a.n_kv) * head_elems, x[u]);
-        continue;
-      }
-      const float* w = rr < a.n_heads ? a.q_norm : a.k_norm;
-      if (w != nullptr) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) ss += x[u][i] * x[u][i];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float f = 1.0f / sqrtf(ss * (1.0f / HD) + a.eps);
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[u][i] = x[u][i] * f * w[d0 + i];
-      }
-      if (a.interleaved) {
-#pragma unroll
-        for (int i = 0; i < N; i += 2) {
-          const float p = x[u][i], q = x[u][i + 1];
-          x[u][i] = d0 + i < a.rotary ? p * cs[i] + q * sn[i] : p;
-          x[u][i + 1] = d0 + i < a.rotary ? q * cs[i + 1] + p * sn[i + 1] : q;
-        }
-      } else {
-        __syncwarp();  // the row before has been read
-        pg_store<N>(row_s[warp] + d0, x[u]);
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int d = d0 + i;
-          if (d < a.rotary) x[u][i] = x[u][i] * cs[i] + row_s[warp][d < half ? d + half : d - half] * sn[i];
-        }
-      }
       if (rr < a.n_heads)
         pg_store<N>(qo + rr * HD, x[u]);
-      else
+      else if (rr < a.n_heads + a.n_kv)
         pg_store<N>(page_k + (rr - a.n_heads) * head_elems, x[u]);
+      else
+        pg_store<N>(page_k + a.v_off + (rr - a.n_heads - a.n_kv) * head_elems, x[u]);
     }
   }
 }
