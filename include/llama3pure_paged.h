@@ -31,8 +31,8 @@
  *     launch nothing.  A page that is freed may be given out by the next begin
  *     or copy; work on it that is already enqueued comes first when the stream
  *     is the same.
- *   - begin, truncate, free, copy and compact check everything first: a
- *     call that fails changes nothing.
+ *   - new, fork, begin, truncate, free, copy and compact check everything
+ *     first: a call that they refuse changes nothing.
  *   - Freeing, truncating or compacting ends the current batch: append and
  *     attention are refused until the next begin.
  */

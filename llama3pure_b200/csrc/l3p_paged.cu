@@ -107,7 +107,7 @@ int copy_pages(Ctx* ctx, const std::vector<int4>& jobs, cudaStream_t st) {
   if (int rc = take_slot(ctx, jobs.size() * 4, &s)) return rc;
   memcpy(s->host, jobs.data(), jobs.size() * sizeof(int4));
   if (int rc = upload(ctx, s, ctx->jobs, jobs.size() * 4, st)) return rc;
-  return launch_page_copy(ctx, (int)jobs.size(), st);
+  return launch_page_copy(ctx, ctx->jobs, (int)jobs.size(), st);
 }
 
 cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
@@ -148,10 +148,11 @@ int first_key(const Ctx* ctx, bool win, int pos) { return win ? std::max(0, pos 
 // costs about kSegRounds rounds that its prefetched tiles do not hide (16
 // sequences x 2 tokens x 3000 keys, 8B heads: 46.8 us end to end, 39.5 us by units).
 constexpr double kSegRounds = 1.5;
-void plan_rows(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, int nt, std::vector<int>* first,
+void plan_rows(Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, int nt, std::vector<int>* first,
                std::vector<PgSeg>* segs) {
   const int rt = 8 * nt, warps = row_warps(ctx), G = ctx->G;
-  std::vector<PgSeg> units;
+  std::vector<PgSeg>& units = ctx->row_units;
+  units.clear();
   long long total = 0;
   int longest = 0;
   for (const auto& b : bs) {
@@ -177,6 +178,7 @@ void plan_rows(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, int nt
       }
   }
   if (units.empty()) return;
+  segs->reserve(units.size() + kPgMaxCtas);
   const int max_ctas = std::min(ctx->num_sms, kPgMaxCtas);
   auto rounds = [&](long long tiles) { return (tiles + warps - 1) / warps; };
   const long long run = rounds((total + max_ctas - 1) / max_ctas) * warps;
@@ -245,13 +247,14 @@ void plan_rows(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, int nt
 // of them for the GPU, long key ranges are cut into parts of equal size, which a
 // second kernel merges.  Longest parts first.  fp32 pools: also the list of the
 // key tiles that the units read.
-void plan_tc(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vector<PgPart>* parts,
+void plan_tc(Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vector<PgPart>* parts,
              std::vector<PgPart>* merges, std::vector<PgPrep>* prep) {
   const int tile = ctx->bf16 ? tc_tile(ctx) : 128, G = ctx->G;
   const int rt = ctx->bf16 ? tc_rows(ctx) : f32_rows(ctx);
   // CTAs (or CTA pairs) that run at once
   const int wide = !ctx->bf16 && rt == 256 ? ctx->num_sms / 2 : ctx->num_sms;
-  std::vector<PgPart> units;
+  std::vector<PgPart>& units = ctx->tc_units;
+  units.clear();
   for (const auto& b : bs) {
     const long long rows = (long long)b.n_new * G;
     if (!b.tc) continue;
@@ -369,76 +372,96 @@ void plan_tc(const Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vec
   });
 }
 
-// Lays the current batch out as the kernels read it.
-void build_batch(const Ctx* ctx, const std::vector<BatchSeq>& bs, const int* seqs, int n_seqs, int n_tokens,
-                 std::vector<int>* words, PgHeader* hdr) {
+// Lays the current batch out as the kernels read it, in a pinned slot, with the page copies behind it (*jobs_at: their
+// word offset).  The lists are the context's, so that a step allocates nothing.
+int build_batch(Ctx* ctx, const std::vector<BatchSeq>& bs, const int* seqs, int n_seqs, int n_tokens,
+                const std::vector<int4>& jobs, Ctx::Slot** out, size_t* words, size_t* jobs_at) {
   PgHeader h{};
   h.n_tokens = n_tokens;
   h.n_seqs = n_seqs;
   int max_rows = 0;
-  for (const auto& b : bs)
-    if (!b.tc) max_rows = std::max(max_rows, b.n_new * ctx->G);
-  h.row_nt = std::min(max_rows <= 8 ? 1 : 2, row_max_nt(ctx));
-  auto& w = *words;
-  w.assign(kPgHdrWords, 0);
-  auto add = [&](const void* p, size_t bytes) {
-    while (w.size() % 4) w.push_back(0);  // records are read 16 bytes at a time
-    const size_t at = w.size();
-    w.resize(at + bytes / 4);
-    if (bytes) memcpy(w.data() + at, p, bytes);
-    return (int)at;
-  };
-  for (int v = 0; v < (ctx->swa ? 2 : 1); ++v) {
-    std::vector<int> first;
-    std::vector<PgSeg> segs;
-    std::vector<PgPart> parts, merges;
-    std::vector<PgPrep> prep;
-    plan_rows(ctx, v == 1, bs, h.row_nt, &first, &segs);
-    plan_tc(ctx, v == 1, bs, &parts, &merges, &prep);
-    PgLists& l = h.lists[v];
-    l.row_ctas = first.empty() ? 0 : (int)first.size() - 1;
-    l.row_first = add(first.data(), first.size() * 4);
-    l.row_segs = add(segs.data(), segs.size() * sizeof(PgSeg));
-    l.n_tc = (int)parts.size();
-    l.tc_parts = add(parts.data(), parts.size() * sizeof(PgPart));
-    l.n_merge = (int)merges.size();
-    l.merges = add(merges.data(), merges.size() * sizeof(PgPart));
-    l.n_prep = (int)prep.size();
-    l.prep = add(prep.data(), prep.size() * sizeof(PgPrep));
-  }
-  std::vector<int2> tok(n_tokens);
-  h.tbl = 0;
   size_t tbl_words = 0;
+  for (int i = 0; i < n_seqs; ++i) {
+    if (!bs[i].tc) max_rows = std::max(max_rows, bs[i].n_new * ctx->G);
+    tbl_words += ctx->seqs[seqs[i]].pages.size();
+  }
+  h.row_nt = std::min(max_rows <= 8 ? 1 : 2, row_max_nt(ctx));
+  size_t at = kPgHdrWords;
+  auto place = [&](size_t bytes) {
+    at = (at + 3) & ~(size_t)3;  // records are read 16 bytes at a time
+    const size_t here = at;
+    at += bytes / 4;
+    return here;
+  };
+  const int n_lists = ctx->swa ? 2 : 1;
+  for (int v = 0; v < n_lists; ++v) {
+    auto& p = ctx->plan[v];
+    p.first.clear(), p.segs.clear(), p.parts.clear(), p.merges.clear(), p.prep.clear();
+    plan_rows(ctx, v == 1, bs, h.row_nt, &p.first, &p.segs);
+    plan_tc(ctx, v == 1, bs, &p.parts, &p.merges, &p.prep);
+    PgLists& l = h.lists[v];
+    l.row_ctas = p.first.empty() ? 0 : (int)p.first.size() - 1;
+    l.row_first = (int)place(p.first.size() * 4);
+    l.row_segs = (int)place(p.segs.size() * sizeof(PgSeg));
+    l.n_tc = (int)p.parts.size();
+    l.tc_parts = (int)place(p.parts.size() * sizeof(PgPart));
+    l.n_merge = (int)p.merges.size();
+    l.merges = (int)place(p.merges.size() * sizeof(PgPart));
+    l.n_prep = (int)p.prep.size();
+    l.prep = (int)place(p.prep.size() * sizeof(PgPrep));
+  }
+  h.tok = (int)place((size_t)n_tokens * sizeof(int2));
+  h.tbl = (int)place(tbl_words * 4);
+  *jobs_at = place(jobs.size() * sizeof(int4));
+  if (at > ctx->batch_words) return fail(ctx, L3P_E_RANGE, "batch description of %zu words", at);
+  if (int rc = take_slot(ctx, at, out)) return rc;
+  int* w = (*out)->host;
+  auto put = [&](size_t where, const void* p, size_t bytes) {
+    if (bytes) memcpy(w + where, p, bytes);
+  };
+  memset(w, 0, kPgHdrWords * 4);
+  memcpy(w, &h, sizeof h);
+  for (int v = 0; v < n_lists; ++v) {
+    const auto& p = ctx->plan[v];
+    const PgLists& l = h.lists[v];
+    put(l.row_first, p.first.data(), p.first.size() * 4);
+    put(l.row_segs, p.segs.data(), p.segs.size() * sizeof(PgSeg));
+    put(l.tc_parts, p.parts.data(), p.parts.size() * sizeof(PgPart));
+    put(l.merges, p.merges.data(), p.merges.size() * sizeof(PgPart));
+    put(l.prep, p.prep.data(), p.prep.size() * sizeof(PgPrep));
+  }
+  int* tbl = w + h.tbl;
   for (int i = 0; i < n_seqs; ++i) {
     const auto& s = ctx->seqs[seqs[i]];
     const auto& b = bs[i];
-    tbl_words += s.pages.size();
     for (int t = 0; t < b.n_new; ++t) {
       const int pos = b.len - b.n_new + t;
-      tok[b.q_row0 + t] = make_int2(s.pages[pos >> ctx->shift] * ctx->cfg.page_size + (pos & (ctx->cfg.page_size - 1)), pos);
+      int* tok = w + h.tok + 2 * (b.q_row0 + t);
+      tok[0] = s.pages[pos >> ctx->shift] * ctx->cfg.page_size + (pos & (ctx->cfg.page_size - 1));
+      tok[1] = pos;
     }
+    put(tbl - w, s.pages.data(), s.pages.size() * 4);
+    tbl += s.pages.size();
   }
-  h.tok = add(tok.data(), tok.size() * sizeof(int2));
-  h.tbl = add(nullptr, 0);
-  w.reserve(w.size() + tbl_words);
-  for (int i = 0; i < n_seqs; ++i) {
-    const auto& s = ctx->seqs[seqs[i]];
-    w.insert(w.end(), s.pages.begin(), s.pages.end());
-  }
-  memcpy(w.data(), &h, sizeof h);
-  *hdr = h;
+  put(*jobs_at, jobs.data(), jobs.size() * sizeof(int4));
+  ctx->hdr = h;
+  *words = at;
+  return L3P_OK;
 }
 
 // Words of the largest batch block: bounds on what build_batch lays out.
 size_t batch_capacity(const Ctx* ctx) {
   const auto& c = ctx->cfg;
-  const size_t max_len = c.max_seq_len;
-  // units of either path: blocks of at least 8 rows (row kernel), plus one part or segment per CTA and per unit
-  const size_t units = (size_t)c.n_kv_heads * (((size_t)c.max_tokens * ctx->G + 7) / 8 + c.max_seqs);
-  const size_t lists = (units + 2 * kPgMaxCtas + 8) * 16 + kPgMaxCtas + 8;
-  const size_t tiles = ctx->bf16 ? 0 : (size_t)c.max_seqs * ((max_len + 127) / 128 + 1) * 4;
-  const size_t table = (size_t)c.max_seqs * ((max_len + c.page_size - 1) / c.page_size);
-  return kPgHdrWords + 2 * (lists + lists + lists + tiles) + 2 * (size_t)c.max_tokens + table + 64;
+  const size_t max_len = c.max_seq_len, rows = (size_t)c.max_tokens * ctx->G, kv = c.n_kv_heads, seqs = c.max_seqs;
+  const bool only_rows = row_limit(ctx) == INT_MAX;
+  // units of the row kernel: blocks of at least 8 rows; segments: one more per CTA at most
+  const size_t row_units = only_rows ? kv * (rows / 8 + seqs) : kv * 2 * seqs;
+  // units of the tensor-core kernels: blocks of at least 128 rows; parts: 3 num_sms more at most, as many merged units
+  const size_t tc_units = only_rows ? 0 : kv * (rows / 128 + seqs);
+  const size_t tiles = only_rows || ctx->bf16 ? 0 : 4 * seqs * ((max_len + 127) / 128 + 1);
+  const size_t list = (row_units + kPgMaxCtas) * 16 + kPgMaxCtas + 1 + (tc_units + 6 * (size_t)ctx->num_sms) * 16 + tiles + 5 * 4;
+  const size_t table = seqs * ((max_len + c.page_size - 1) / c.page_size);
+  return kPgHdrWords + (ctx->swa ? 2 : 1) * list + 2 * (size_t)c.max_tokens + table + 4 * seqs + 64;
 }
 
 void release(Ctx* ctx) {
@@ -601,15 +624,13 @@ int begin(Ctx* ctx, int n_seqs, const int* ids, const int* n_new, cudaStream_t s
     if (n_new[i] > 0) ctx->max_pos_in_batch = std::max(ctx->max_pos_in_batch, len);
     tbl += (int)q.pages.size();
   }
-  if (int rc = copy_pages(ctx, jobs, s)) return rc;
   choose_paths(ctx, &bs);
-  std::vector<int> words;
-  build_batch(ctx, bs, ids, n_seqs, row, &words, &ctx->hdr);
-  if (words.size() > ctx->batch_words) return fail(ctx, L3P_E_RANGE, "batch description of %zu words", words.size());
   Ctx::Slot* slot;
-  if (int rc = take_slot(ctx, words.size(), &slot)) return rc;
-  memcpy(slot->host, words.data(), words.size() * 4);
-  if (int rc = upload(ctx, slot, ctx->batch, words.size(), s)) return rc;
+  size_t words, jobs_at;
+  if (int rc = build_batch(ctx, bs, ids, n_seqs, row, jobs, &slot, &words, &jobs_at)) return rc;
+  if (int rc = upload(ctx, slot, ctx->batch, words, s)) return rc;
+  if (!jobs.empty())
+    if (int rc = launch_page_copy(ctx, ctx->batch + jobs_at, (int)jobs.size(), s)) return rc;
   ctx->batch_valid = true;
   return L3P_OK;
 }

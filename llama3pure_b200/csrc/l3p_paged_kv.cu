@@ -13,13 +13,13 @@ using namespace l3p_pg;
 
 namespace l3p_pg {
 
-int launch_page_copy(l3p_paged_ctx* ctx, int n_jobs, cudaStream_t s) {
+int launch_page_copy(l3p_paged_ctx* ctx, const int* jobs, int n_jobs, cudaStream_t s) {
   const int blocks = ctx->cfg.n_layers * 2 * ctx->cfg.n_kv_heads;
   const int want = std::max(1, 8 * ctx->num_sms / n_jobs);  // CTAs of a job: a few per SM over all jobs
   const int gx = std::min((blocks + 7) / 8, want);
   for (int at = 0; at < n_jobs; at += 65535) {  // grid y
     const int n = std::min(n_jobs - at, 65535);
-    paged_copy_kernel<<<dim3(gx, n), 256, 0, s>>>(reinterpret_cast<const int4*>(ctx->jobs) + at,
+    paged_copy_kernel<<<dim3(gx, n), 256, 0, s>>>(reinterpret_cast<const int4*>(jobs) + at,
                                                   static_cast<char*>(ctx->storage), (long long)ctx->page_bytes, blocks,
                                                   (int)ctx->block_bytes, ctx->hd * ctx->es);
     ++ctx->launches;
@@ -266,10 +266,14 @@ L3P_API int l3p_paged_attn_dev(l3p_paged_ctx* ctx, int layer, const void* q, lon
   DeviceScope dev(ctx->cfg.device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const PgLists& l = ctx->hdr.lists[windowed(ctx, layer) ? 1 : 0];
-  if (l.n_tc > 0)
-    if (int rc = ctx->bf16 ? launch_tc(ctx, layer, q, q_stride, out, out_stride, s)
-                           : launch_f32(ctx, layer, q, q_stride, out, out_stride, s))
-      return rc;
-  if (l.row_ctas > 0) return launch_rows(ctx, layer, q, q_stride, out, out_stride, s);
+  try {
+    if (l.n_tc > 0)
+      if (int rc = ctx->bf16 ? launch_tc(ctx, layer, q, q_stride, out, out_stride, s)
+                             : launch_f32(ctx, layer, q, q_stride, out, out_stride, s))
+        return rc;
+    if (l.row_ctas > 0) return launch_rows(ctx, layer, q, q_stride, out, out_stride, s);
+  } catch (...) {
+    return fail(ctx, L3P_E_NOMEM, "host memory is exhausted");
+  }
   return L3P_OK;
 }

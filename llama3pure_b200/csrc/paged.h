@@ -123,6 +123,14 @@ struct l3p_paged_ctx {
   // current batch
   bool batch_valid = false;
   l3p::PgHeader hdr{};
+  struct Plan {
+    std::vector<int> first;
+    std::vector<l3p::PgSeg> segs;
+    std::vector<l3p::PgPart> parts, merges;
+    std::vector<l3p::PgPrep> prep;
+  } plan[2];
+  std::vector<l3p::PgSeg> row_units;
+  std::vector<l3p::PgPart> tc_units;
   int max_pos_in_batch = 0;  // one more than the highest position of a new token
 
   // split workspace: partial rows, (m, l) pairs, tickets (0 between launches)
@@ -253,6 +261,6 @@ int launch_f32(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void*
 // Joins the parts of the split units of the tensor-core kernels (l3p_paged_tc.cu).
 int launch_merge(l3p_paged_ctx* ctx, const l3p::PgLists& l, bool win, int rows, void* out, long long os, cudaStream_t s);
 // Copies rows of pages: jobs (source page, destination page, rows, 0) in device memory.
-int launch_page_copy(l3p_paged_ctx* ctx, int n_jobs, cudaStream_t s);
+int launch_page_copy(l3p_paged_ctx* ctx, const int* jobs, int n_jobs, cudaStream_t s);
 
 }  // namespace l3p_pg

@@ -28,10 +28,14 @@ SCALINGS = {"none": 0, "linear": 1, "bands": 2, "yarn": 3}
 
 
 def _ints(x) -> np.ndarray:
-    a = np.asarray(x, dtype=np.int64).reshape(-1)
-    if a.size and (a.min() < -(2**31) or a.max() >= 2**31):
-        raise ValueError("values outside 32 bits")
-    return np.ascontiguousarray(a, dtype=np.int32)
+    """x as int32; fractions and values outside 32 bits raise."""
+    a = np.asarray(x).reshape(-1)
+    if not a.size:
+        return np.empty(0, np.int32)
+    out = a.astype(np.int32)
+    if a.dtype.kind not in "iu" or (out != a).any():
+        raise ValueError("sequences and counts are whole numbers of 32 bits")
+    return out
 
 
 class PagedCache:

@@ -182,7 +182,7 @@ def test_sliding_window_layers(torch, dtype, dim, window):
 
 
 @pytest.mark.parametrize("dtype,heads,kv,dim,lengths", [
-    ("f32", 32, 8, 128, [9000, 3]), ("bf16", 32, 8, 128, [20000]), ("bf16", 8, 1, 64, [33000]), ("f32", 8, 1, 256, [5000, 1]),
+    ("f32", 32, 8, 128, [9000, 3]), ("f32", 16, 8, 128, [66100]), ("bf16", 32, 8, 128, [20000]), ("bf16", 8, 1, 64, [33000]), ("f32", 8, 1, 256, [5000, 1]),
     ("bf16", 8, 1, 256, [7000]), ("bf16", 16, 8, 128, [40, 6000, 1, 2500, 777]),
 ])
 def test_long_sequences_are_split_and_joined(torch, dtype, heads, kv, dim, lengths):
@@ -562,6 +562,56 @@ def test_captured_step_serves_later_batches(torch):
             c.begin(seqs, [1] * 6)
             graph.replay()
             c.check()
+            del graph
+
+
+@pytest.mark.parametrize("dtype,dim", [("f32", 64), ("f32", 128), ("bf16", 64), ("bf16", 128), ("bf16", 256)])
+def test_captured_chunks(torch, dtype, dim):
+    """A captured batch of chunks beside single tokens, replayed on smaller ones, with parts to be joined; one that is larger is
+    reported and written nothing for."""
+    with _cache(n_heads=8, n_kv_heads=2, head_dim=dim, dtype=dtype, n_layers=1, n_pages=800, max_tokens=6000, page_size=16) as c:
+        b = Books(torch, c)
+        seqs = [b.new() for _ in range(3)]
+        for x, n in zip(seqs, [5000, 900, 17]):
+            b.step([x], [n], attend=False)
+        big, small = [200, 130, 1], [60, 40, 1]
+        c.begin(seqs, big)
+        q, out = b.randn(sum(big), 8, dim), torch.empty(sum(big), 8, dim, device="cuda", dtype=c.dtype)
+        kv = [b.randn(sum(big), 2, dim) for _ in range(2)]
+        s = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            c.append_dev(0, *kv)
+            c.attn_dev(0, q, out)
+            c.check()
+            want = out.clone()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                c.append_dev(0, *kv)
+                c.attn_dev(0, q, out)
+            for new in (big, small):
+                for x, n in zip(seqs, [5000, 900, 17]):
+                    c.truncate(x, n)
+                c.begin(seqs, new)
+                out.fill_(9.0)
+                graph.replay()
+                c.check()
+                got = out.clone()
+                out.fill_(9.0)
+                c.attn_dev(0, q, out)
+                c.check()
+                assert bool((got == out).all()) and bool((got[sum(new):] == 9.0).all())
+                if new == big:
+                    assert bool((got == want).all())
+            for new in ([200, 131, 1], [600, 1, 1], [1, 1, 1]):
+                c.begin(seqs, new)
+                out.fill_(9.0)
+                graph.replay()
+                with pytest.raises(AttnError) as e:
+                    c.check()
+                assert e.value.code == -1
+                if new != [1, 1, 1]:  # single tokens alone: the captured row launch meets no chunk, and neither writes
+                    assert bool((out == 9.0).all())
             del graph
 
 
