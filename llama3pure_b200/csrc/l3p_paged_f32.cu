@@ -65,6 +65,7 @@ static int chunks(l3p_paged_ctx* ctx, PgF32Args a, const PgLists& l, cudaStream_
   a.flags = ctx->v_flags;
   for (int h = 0; h < n_kv; h += group) {
     a.kvh0 = h;
+    a.n_kv = n_kv;
     a.n_kvh = std::min(group, n_kv - h);
     if (int rc = launch(ctx, paged_prep_kernel<CG, HD>, dim3(l.n_prep, a.n_kvh, 4), 256, 0, s, 1, a)) return rc;
     if (int rc = launch(ctx, paged_f32_kernel<CG, HD>, dim3(l.n_tc * CG), 512, PgF32Cfg<CG, HD>::kSmem, s, CG, a)) return rc;
@@ -93,8 +94,7 @@ int launch_f32(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void*
   a.ws_o = ctx->tc_o;
   a.ws_ml = ctx->tc_ml;
   a.err = ctx->err_dev;
-  if (int rc = ctx->hd == 64 ? chunks<1, 64>(ctx, a, l, s) : chunks<2, 128>(ctx, a, l, s)) return rc;
-  return launch_merge(ctx, l, win, f32_rows(ctx), out, os, s);
+  return ctx->hd == 64 ? chunks<1, 64>(ctx, a, l, s) : chunks<2, 128>(ctx, a, l, s);
 }
 
 }  // namespace l3p_pg

@@ -271,9 +271,10 @@ L3P_API int l3p_paged_attn_dev(l3p_paged_ctx* ctx, int layer, const void* q, lon
       if (int rc = ctx->bf16 ? launch_tc(ctx, layer, q, q_stride, out, out_stride, s)
                              : launch_f32(ctx, layer, q, q_stride, out, out_stride, s))
         return rc;
-    if (l.row_ctas > 0) return launch_rows(ctx, layer, q, q_stride, out, out_stride, s);
+    if (l.row_ctas > 0)
+      if (int rc = launch_rows(ctx, layer, q, q_stride, out, out_stride, s)) return rc;
+    return launch_merge(ctx, l, windowed(ctx, layer), out, out_stride, s);
   } catch (...) {
     return fail(ctx, L3P_E_NOMEM, "host memory is exhausted");
   }
-  return L3P_OK;
 }

@@ -78,6 +78,7 @@ int launch_rows(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void
   a.win = win ? 1 : 0;
   a.window = ctx->cfg.swa_window;
   a.lim = limits(ctx, l);
+  a.late = l.n_tc > 0;
   a.scale_log2 = ctx->scale * kLog2e;
   a.ws_o = ctx->ws_o;
   a.ws_ml = ctx->ws_ml;

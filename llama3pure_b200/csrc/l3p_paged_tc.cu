@@ -78,11 +78,9 @@ int launch_tc(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void* 
   a.err = ctx->err_dev;
   CUtensorMap map;
   memcpy(&map, ctx->tmap, sizeof map);
-  if (int rc = with_kernel(ctx, [&](auto kernel, int threads, int smem) {
-        return launch(ctx, kernel, dim3(l.n_tc), threads, smem, s, 1, a, map);
-      }))
-    return rc;
-  return launch_merge(ctx, l, win, tc_rows(ctx), out, os, s);
+  return with_kernel(ctx, [&](auto kernel, int threads, int smem) {
+    return launch(ctx, kernel, dim3(l.n_tc), threads, smem, s, 1, a, map);
+  });
 }
 
 template <typename T, int HD>
@@ -91,7 +89,8 @@ static int merge(l3p_paged_ctx* ctx, const PgLists& l, bool win, int rows, void*
                 limits(ctx, l), rows, (const float*)ctx->tc_o, (const float*)ctx->tc_ml, static_cast<T*>(out), os, ctx->G);
 }
 
-int launch_merge(l3p_paged_ctx* ctx, const PgLists& l, bool win, int rows, void* out, long long os, cudaStream_t s) {
+int launch_merge(l3p_paged_ctx* ctx, const PgLists& l, bool win, void* out, long long os, cudaStream_t s) {
+  const int rows = ctx->bf16 ? tc_rows(ctx) : f32_rows(ctx);
   if (l.n_merge == 0) return L3P_OK;
   if (ctx->bf16)
     return ctx->hd == 64    ? merge<__nv_bfloat16, 64>(ctx, l, win, rows, out, os, s)

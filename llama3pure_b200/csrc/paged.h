@@ -259,7 +259,7 @@ int launch_rows(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void
 int launch_tc(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void* out, long long os, cudaStream_t s);
 int launch_f32(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void* out, long long os, cudaStream_t s);
 // Joins the parts of the split units of the tensor-core kernels (l3p_paged_tc.cu).
-int launch_merge(l3p_paged_ctx* ctx, const l3p::PgLists& l, bool win, int rows, void* out, long long os, cudaStream_t s);
+int launch_merge(l3p_paged_ctx* ctx, const l3p::PgLists& l, bool win, void* out, long long os, cudaStream_t s);
 // Copies rows of pages: jobs (source page, destination page, rows, 0) in device memory.
 int launch_page_copy(l3p_paged_ctx* ctx, const int* jobs, int n_jobs, cudaStream_t s);
 

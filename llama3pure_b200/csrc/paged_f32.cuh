@@ -52,7 +52,7 @@ struct PgF32Args {
   long long page_elems, v_off;
   float* img;             // [head of the group of heads][n_prep] tile images
   int* flags;             // [head][n_prep][4]: 32 keys' V hold values that are not finite (0 in the image)
-  int kvh0, n_kvh;        // group of KV heads of this launch
+  int kvh0, n_kvh, n_kv;  // group of KV heads of this launch, of all
   int shift, G, win, window;
   PgLimits lim;
   float scale_log2;
@@ -177,16 +177,19 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
 
   const PgHeader* hd = reinterpret_cast<const PgHeader*>(a.batch);
   const PgLists l = hd->lists[a.win];
-  griddep_launch();
+  const bool rows_next = a.lim.with_rows && a.kvh0 + a.n_kvh == a.n_kv;
+  if (!rows_next) griddep_launch();
   const bool fits = pg_fits(hd, l, a.lim);
   if (!fits || (int)blockIdx.x / CG >= l.n_tc) {
     griddep_wait();
+    griddep_launch();
     if (!fits && blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
     return;
   }
   const PgPart u = reinterpret_cast<const PgPart*>(a.batch + l.tc_parts)[blockIdx.x / CG];
   if (u.kvh < a.kvh0 || u.kvh >= a.kvh0 + a.n_kvh) {  // both CTAs of a pair
     griddep_wait();
+    griddep_launch();
     return;
   }
   const int* table = a.batch + hd->tbl + u.tbl;
@@ -230,6 +233,7 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
   tc::fence_after_sync();
   const uint32_t tm = s_tmem;
   griddep_wait();  // the images and q come from the kernels before this one
+  if (rows_next) griddep_launch();  // the row kernel relies on that wait
   const uint32_t T_QHI = tm + 0, T_O = tm + HD, T_S = tm + 2 * HD, T_P = tm + 2 * HD + kPfBN;
 
   // Barriers that carry tensor memory, copies that have landed or room (not ordinary stores) between the CTAs of a pair are

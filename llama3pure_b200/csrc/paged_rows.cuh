@@ -47,6 +47,7 @@ struct PgRowArgs {
   long long page_elems, v_off;
   int shift, G, win, window;
   PgLimits lim;
+  int late;          // the kernel before is a tensor-core kernel of the same call: wait for it at the end only
   float scale_log2;
   float* ws_o;       // [slot][8*NT][HD]
   float* ws_ml;      // [slot][8*NT][2]
@@ -158,6 +159,9 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
   const PgHeader* h = reinterpret_cast<const PgHeader*>(a.batch);
   const PgLists l = h->lists[a.win];
   griddep_launch();
+  // In a batch with chunks this kernel follows a tensor-core kernel, which lets it start once all of its CTAs have seen the
+  // kernel before them complete.  The two read the same rows and write others, so they run side by side; this one's CTAs
+  // wait at their end, so that what follows this kernel follows both.
   if (!pg_fits(h, l, a.lim) || h->row_nt != NT || l.row_ctas > (int)gridDim.x || (int)blockIdx.x >= l.row_ctas) {
     griddep_wait();
     if ((int)blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
@@ -208,7 +212,7 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
   if (is < seg_end) load_seg();
   settle();
   // Rows of earlier batches are there already; the new tokens' rows, and q, come from the kernel before this one.
-  bool waited = false;
+  bool waited = a.late != 0;
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) {
     if (!waited && is < seg_end && (it + 1) * kPgTile > ipos0) {
@@ -629,6 +633,7 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
+  if (a.late) griddep_wait();
 }
 
 }  // namespace l3p

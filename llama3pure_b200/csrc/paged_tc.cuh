@@ -219,9 +219,10 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
 
   const PgHeader* h = reinterpret_cast<const PgHeader*>(a.batch);
   const PgLists l = h->lists[a.win];
-  griddep_launch();
+  if (!a.lim.with_rows) griddep_launch();
   if (!pg_fits(h, l, a.lim) || (int)blockIdx.x >= l.n_tc) {
     griddep_wait();
+    griddep_launch();
     if (!pg_fits(h, l, a.lim) && blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
     return;
   }
@@ -274,6 +275,7 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
   tc::fence_after_sync();
   const uint32_t tm = s_tmem;
   griddep_wait();  // q and the new rows come from the kernel before this one
+  if (a.lim.with_rows) griddep_launch();  // the row kernel relies on that wait
 
   // Registers: 384 x 168 at launch = 128 x 88 + 256 x 208.  Inside the branches: behind their join the compiler would
   // count with the smaller number.
