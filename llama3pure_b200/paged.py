@@ -17,6 +17,7 @@ torch's current stream of the cache's device.
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 
 import numpy as np
 
@@ -27,15 +28,10 @@ LAYOUTS = {"interleaved": 0, "half": 1}
 SCALINGS = {"none": 0, "linear": 1, "bands": 2, "yarn": 3}
 
 
-def _ints(x) -> np.ndarray:
-    """x as int32; fractions and values outside 32 bits raise."""
-    a = np.asarray(x).reshape(-1)
-    if not a.size:
-        return np.empty(0, np.int32)
-    out = a.astype(np.int32)
-    if a.dtype.kind not in "iu" or (out != a).any():
-        raise ValueError("sequences and counts are whole numbers of 32 bits")
-    return out
+def _ints(x) -> tuple[int, int, array]:
+    """Whole numbers of 32 bits: address, count, and the array that holds them (others raise)."""
+    a = array("i", x.tolist() if hasattr(x, "tolist") else x)
+    return *a.buffer_info(), a
 
 
 class PagedCache:
@@ -132,24 +128,23 @@ class PagedCache:
 
     def fork(self, seq: int, n: int = 1, n_tokens: int = -1) -> list[int]:
         """n sequences that share the first n_tokens positions of `seq` (default: all of them)."""
-        ids = np.empty(max(n, 0), np.int32)
-        self._ok(self.lib.l3p_paged_seq_fork(self.h, seq, n_tokens, n, ids.ctypes.data), "fork")
-        return ids.tolist()
+        out = array("i", bytes(4 * max(n, 1)))
+        self._ok(self.lib.l3p_paged_seq_fork(self.h, seq, n_tokens, n, out.buffer_info()[0]), "fork")
+        return out.tolist()[:n]
 
     def copy(self, seqs, stream=None) -> list[int]:
         """Sequences with pages of their own and the rows of `seqs`."""
-        ids = _ints(seqs)
-        out = np.empty_like(ids)
-        self._ok(self.lib.l3p_paged_seq_copy(self.h, len(ids), ids.ctypes.data, out.ctypes.data, self._stream(stream)),
-                 "copy")
+        p, n, ids = _ints(seqs)
+        out = array("i", ids)
+        self._ok(self.lib.l3p_paged_seq_copy(self.h, n, p, out.buffer_info()[0], self._stream(stream)), "copy")
         return out.tolist()
 
     def truncate(self, seq: int, n_tokens: int) -> None:
         self._ok(self.lib.l3p_paged_seq_truncate(self.h, seq, n_tokens), "truncate")
 
     def free(self, seqs) -> None:
-        ids = _ints(seqs)
-        self._ok(self.lib.l3p_paged_seq_free(self.h, len(ids), ids.ctypes.data), "free")
+        p, n, ids = _ints(seqs)
+        self._ok(self.lib.l3p_paged_seq_free(self.h, n, p), "free")
 
     def length(self, seq: int) -> int:
         n = C.c_int()
@@ -158,10 +153,11 @@ class PagedCache:
 
     def tables(self, seqs) -> np.ndarray:
         """Page tables of `seqs`, int32 [n][widest], filled up with -1."""
-        ids, need = _ints(seqs), C.c_int()
-        self._ok(self.lib.l3p_paged_tables(self.h, len(ids), ids.ctypes.data, 0, None, C.byref(need)), "tables")
-        out = np.empty((len(ids), need.value), np.int32)
-        self._ok(self.lib.l3p_paged_tables(self.h, len(ids), ids.ctypes.data, need.value, out.ctypes.data, None), "tables")
+        p, n, ids = _ints(seqs)
+        need = array("i", [0])
+        self._ok(self.lib.l3p_paged_tables(self.h, n, p, 0, None, need.buffer_info()[0]), "tables")
+        out = np.empty((n, need[0]), np.int32)
+        self._ok(self.lib.l3p_paged_tables(self.h, n, p, need[0], out.ctypes.data, None), "tables")
         return out
 
     def free_pages(self) -> int:
@@ -178,12 +174,12 @@ class PagedCache:
     # -- a step ----------------------------------------------------------------------
     def begin(self, seqs, n_new, stream=None) -> None:
         """Begins a batch: sequence seqs[i] grows by n_new[i] tokens."""
-        ids, new = _ints(seqs), _ints(n_new)
-        if len(ids) != len(new):
+        p, n, ids = _ints(seqs)
+        q, m, new = _ints(n_new)
+        if n != m:
             raise ValueError("seqs and n_new differ in length")
-        self._ok(self.lib.l3p_paged_begin(self.h, len(ids), ids.ctypes.data, new.ctypes.data, self._stream(stream)),
-                 "begin")
-        self.n_tokens = int(new.sum())
+        self._ok(self.lib.l3p_paged_begin(self.h, n, p, q, self._stream(stream)), "begin")
+        self.n_tokens = sum(new)
 
     def set_rope(self, max_pos: int, layout: str = "interleaved", rotary_dim: int = 0, scaling: str = "none",
                  theta: float = 0.0, theta_swa: float = 0.0, factor: float = 1.0, low_freq: float = 0.0,
