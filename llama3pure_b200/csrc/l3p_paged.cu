@@ -549,6 +549,7 @@ int create(const l3p_paged_config& in, Ctx** out) {
   ctx->fill.assign(c.n_pages, 0);
   ctx->free_heap.resize(c.n_pages);
   for (int i = 0; i < c.n_pages; ++i) ctx->free_heap[i] = i;  // ascending: a min-heap already
+  if (int rc = init_kv(ctx)) return rc;
   if (int rc = init_rows(ctx)) return rc;
   if (int rc = ctx->bf16 ? init_tc(ctx) : init_f32(ctx)) return rc;
   PG_CUDA(ctx, cudaDeviceSynchronize());  // the storage is zero before any stream of the caller's writes it

@@ -251,6 +251,7 @@ int tc_rows(const l3p_paged_ctx* ctx);  // rows of a part, bf16 pools
 int f32_rows(const l3p_paged_ctx* ctx);  // rows of a part, fp32 pools
 
 // Set-up of the kernels at create: shared-memory attributes, tensor map, workspaces.
+int init_kv(l3p_paged_ctx* ctx);
 int init_rows(l3p_paged_ctx* ctx);
 int init_tc(l3p_paged_ctx* ctx);
 int init_f32(l3p_paged_ctx* ctx);

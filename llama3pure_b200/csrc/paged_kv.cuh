@@ -64,6 +64,9 @@ __device__ __forceinline__ void pg_store(__nv_bfloat16* __restrict__ p, const fl
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(w);
 }
 
+__device__ __forceinline__ float pg_f32(float x) { return x; }
+__device__ __forceinline__ float pg_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+
 struct PgKvArgs {
   const int* batch;
   int n_tokens;  // of the launch: a replay must not find more tokens,
@@ -88,7 +91,8 @@ struct PgKvArgs {
 
 constexpr int kPgKvWarps = 8;
 
-// Rotation and write of the new rows.  One warp takes `rows_per_warp`
+// Rotation and write of the new rows, for what the streamed form below does not take: tokens of which two do not fit its
+// ring, and odd numbers of pairs.  One warp takes `rows_per_warp`
 // consecutive head rows (query heads first, then K heads, then V heads) of one
 // token; cosines and sines are read once for all of them.
 //   x' = x * rsqrt(mean x^2 + eps) * w              (where norm weights are given)
@@ -231,6 +235,156 @@ __global__ void __launch_bounds__(kPgKvWarps * 32) paged_rope_kernel(const PgKvA
       else
         pg_store<N>(page_k + a.v_off + (rr - a.n_heads - a.n_kv) * head_elems, x[u]);
     }
+  }
+}
+
+// The same, streamed: one producer warp brings whole tokens (q, k, v rows and the token's row of the table) into a ring in
+// shared memory with bulk copies, eight warps turn a head row each from there; partners are read where they lie.  Norm
+// weights are folded into the cosines and sines once a token, so a row costs ~80 instructions (8191 tokens, 8B heads, fp32,
+// 403 MB with norms: 77 us = 5.2 TB/s, 81 % of a copy; half of the issue slots).
+constexpr int kPgRingThreads = (kPgKvWarps + 1) * 32;
+constexpr int kPgRingStages = 4;  // at most
+struct PgRingArgs {
+  int stages, stage_bytes;            // of the ring; a stage: q rows, k rows, v rows, table row
+  int q_bytes, kv_bytes, tab_bytes;
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kPgRingThreads) paged_rope_ring_kernel(const PgKvArgs a, const PgRingArgs g) {
+  constexpr int N = HD / 32;
+  extern __shared__ __align__(128) unsigned char rope_ring[];
+  __shared__ __align__(8) uint64_t full[kPgRingStages], empty[kPgRingStages];
+  __shared__ int2 s_tok[kPgRingStages];
+  const PgHeader* h = reinterpret_cast<const PgHeader*>(a.batch);
+  const int n_tok = h->n_tokens;
+  griddep_launch();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < g.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kPgKvWarps);
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
+  griddep_wait();  // the rows come from the kernel before this one
+  if (n_tok > a.n_tokens) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int half = a.rotary / 2;
+  if (warp == kPgKvWarps) {
+    if (lane == 0) {
+      int i = 0;
+      for (int tok = blockIdx.x; tok < n_tok; tok += gridDim.x, ++i) {
+        const int s = i % g.stages, use = i / g.stages;
+        const int2 tp = *reinterpret_cast<const int2*>(a.batch + h->tok + 2 * tok);
+        if (use > 0 && !mbar_wait_bounded(&empty[s], (uint32_t)((use - 1) & 1), a.err)) break;
+        const bool ok = tp.y < a.max_pos;  // else the warps report it
+        s_tok[s] = tp;
+        unsigned char* st = rope_ring + s * g.stage_bytes;
+        mbar_arrive_expect_tx(&full[s], (uint32_t)(g.q_bytes + 2 * g.kv_bytes + (ok ? g.tab_bytes : 0)));
+        auto copy = [&](unsigned char* dst, const void* src, int bytes) {
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_addr(dst)),
+                       "l"(src), "r"(bytes), "r"(smem_addr(&full[s]))
+                       : "memory");
+        };
+        copy(st, static_cast<const T*>(a.q) + tok * a.q_stride, g.q_bytes);
+        copy(st + g.q_bytes, static_cast<const T*>(a.k) + tok * a.k_stride, g.kv_bytes);
+        copy(st + g.q_bytes + g.kv_bytes, static_cast<const T*>(a.v) + tok * a.v_stride, g.kv_bytes);
+        if (ok) copy(st + g.q_bytes + 2 * g.kv_bytes, a.tab + (long long)tp.y * half, g.tab_bytes);
+      }
+      for (int x = i > g.stages ? i - g.stages : 0; x < i; ++x)  // no copy may still be landing when the CTA ends
+        mbar_wait_bounded(&full[x % g.stages], (uint32_t)((x / g.stages) & 1), a.err);
+    }
+    return;
+  }
+  const int d0 = lane * N;
+  const long long head_elems = (long long)a.page_size * HD;
+  // the partner of this lane's value e
+  auto partner = [&](int e) {
+    const int d = d0 + e;
+    return a.interleaved ? d ^ 1 : d < half ? d + half : d < a.rotary ? d - half : d;
+  };
+  const bool norm = a.q_norm != nullptr;
+  float wq[N], wqp[N], wk[N], wkp[N];  // norm weights of the values and of their partners
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    wq[e] = norm ? a.q_norm[d0 + e] : 1.f;
+    wk[e] = norm ? a.k_norm[d0 + e] : 1.f;
+    wqp[e] = norm ? a.q_norm[partner(e)] : 1.f;
+    wkp[e] = norm ? a.k_norm[partner(e)] : 1.f;
+  }
+  // x' = f (x c + partner s) with c = cos w, s = +-sin w of the partner, and f of the row's norm
+  auto turn = [&](const T* row, T* dst, const float (&c)[N], const float (&sn)[N]) {
+    float x[N], y[N], f = 1.f;
+    pg_load<N>(row + d0, x);
+    if (a.interleaved) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) y[e] = x[e ^ 1];
+    } else if (half % N == 0) {
+      pg_load<N>(row + partner(0), y);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) y[e] = pg_f32(row[partner(e)]);
+    }
+    if (norm) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) ss += x[e] * x[e];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      f = rsqrtf(ss * (1.0f / HD) + a.eps);  // within 2 units of the last place
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float z = x[e] * c[e];
+      x[e] = (d0 + e < a.rotary ? z + y[e] * sn[e] : z) * f;
+    }
+    pg_store<N>(dst, x);
+  };
+  int i = 0;
+  for (int tok = blockIdx.x; tok < n_tok; tok += gridDim.x, ++i) {
+    const int s = i % g.stages;
+    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[s], (uint32_t)((i / g.stages) & 1), a.err))) return;
+    const unsigned char* st = rope_ring + s * g.stage_bytes;
+    const int2 tp = s_tok[s];
+    if (tp.y >= a.max_pos) {
+      if (lane == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
+    } else {
+      const float2* tab = reinterpret_cast<const float2*>(st + g.q_bytes + 2 * g.kv_bytes);
+      float cq[N], sq[N], ck[N], sk[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int d = d0 + e;
+        float2 t = make_float2(1.f, 0.f);
+        if (d < a.rotary) {
+          t = tab[a.interleaved ? d / 2 : d < half ? d : d - half];
+          if (a.interleaved ? (d & 1) == 0 : d < half) t.y = -t.y;  // the first of a pair
+        }
+        cq[e] = t.x * wq[e], sq[e] = t.y * wqp[e];
+        ck[e] = t.x * wk[e], sk[e] = t.y * wkp[e];
+      }
+      const int page = tp.x >> a.shift, slot = tp.x & (a.page_size - 1);
+      T* page_k = static_cast<T*>(a.storage) + (long long)page * a.page_elems + (long long)slot * HD + d0;
+      T* qo = static_cast<T*>(a.q_out) + tok * a.q_out_stride + d0;
+      const T* rows = reinterpret_cast<const T*>(st);  // q, k and v rows, one after the other
+      int r = warp;
+#pragma unroll 4
+      for (; r < a.n_heads; r += kPgKvWarps) turn(rows + r * HD, qo + r * HD, cq, sq);
+      r -= a.n_heads;
+      rows += a.n_heads * HD;
+      for (; r < a.n_kv; r += kPgKvWarps) turn(rows + r * HD, page_k + r * head_elems, ck, sk);
+      r -= a.n_kv;
+      rows += a.n_kv * HD;
+      for (; r < a.n_kv; r += kPgKvWarps) {
+        float x[N];
+        pg_load<N>(rows + r * HD + d0, x);
+        pg_store<N>(page_k + a.v_off + r * head_elems, x);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[s]);
   }
 }
 

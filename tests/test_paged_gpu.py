@@ -405,7 +405,7 @@ def test_rotary_and_append(torch, dtype, dim, kw):
                    original_len=original, attn_factor=kw["attn"], **norm)
         seqs = [b.new() for _ in range(3)]
         c.begin(seqs, [2900, 0, 17])
-        for new in ([5, 1, 0], [1, 1, 1], [700, 100, 30]):
+        for new in ([5, 1, 0], [1, 1, 1], [700, 100, 30], [5, 900, 400]):
             past = [c.length(s) for s in seqs]
             c.begin(seqs, new)
             n = sum(new)
@@ -432,6 +432,30 @@ def test_rotary_and_append(torch, dtype, dim, kw):
                         _rope_near(torch, rows[:, 0], want_k[at:at + m], dtype, "k")
                         assert bool((rows[:, 1] == want_v[at:at + m]).all())
                     at += m
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_rotary_large_tokens(torch, dtype, layout):
+    """Tokens of which two do not fit a CTA's shared memory."""
+    with _cache(n_heads=96, n_kv_heads=8, head_dim=256, dtype=dtype, n_layers=1, n_pages=20, max_tokens=200) as c:
+        b = Books(torch, c)
+        wq, wk = (np.linspace(0.5, 1.5, 256, dtype=np.float32)[None] * f for f in (1, -1))
+        c.set_rope(max_pos=200, layout=layout, theta=10000.0, q_norm=wq, k_norm=wk)
+        s = b.new()
+        for past, n in ((0, 1), (1, 130)):
+            c.begin([s], [n])
+            q, k, v = b.randn(n, 96, 256), b.randn(n, 8, 256), b.randn(n, 8, 256)
+            out = torch.empty_like(q)
+            c.rope_append_dev(0, q, k, v, out)
+            c.check()
+            pos = torch.arange(past, past + n, device="cuda")
+            args = (pos, 256, layout, 0, "none", 1.0, 0.0, 10000.0, 0)
+            _rope_near(torch, out, _turned(torch, q, *args, w=torch.from_numpy(wq[0]).cuda()), dtype, "q")
+            t = torch.from_numpy(c.tables([s])[0]).cuda().long()
+            rows = c.storage()[t, 0].permute(0, 3, 1, 2, 4).reshape(-1, 2, 8, 256)[past:past + n]
+            _rope_near(torch, rows[:, 0], _turned(torch, k, *args, w=torch.from_numpy(wk[0]).cuda()), dtype, "k")
+            assert bool((rows[:, 1] == v).all())
 
 
 def test_rotary_far_positions_and_window_layers(torch):
