@@ -21,8 +21,7 @@ int row_max_nt(const l3p_paged_ctx* ctx) {
 }
 
 int row_warps(const l3p_paged_ctx* ctx) {
-  const int stage = 2 * kPgTile * ctx->hd * ctx->es;
-  return stage <= 8192 ? 8 : 65536 / stage;
+  return ctx->hd == 256 ? PgRowCfg<float, 256>::kWarps : PgRowCfg<float, 128>::kWarps;
 }
 
 // Calls f with the kernel of the context's type and head size for blocks of nt * 8 rows.

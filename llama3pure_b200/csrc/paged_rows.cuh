@@ -13,7 +13,7 @@
 // units end to end and cuts them into one equal run per CTA (plan_rows), so
 // every SM streams the same number of bytes whatever the lengths are.  Inside
 // a run the CTA's warps take tiles in turn, each through its own ring of
-// cp.async stages; a warp prefetches across the end of a segment, so the merge
+// cp.async places; a warp prefetches across the end of a segment, so the merge
 // of one sequence overlaps the loads of the next.  A unit cut by a run boundary
 // is merged by the part that ends last, in the order of the parts.
 //
@@ -59,16 +59,20 @@ template <typename T, int HD>
 struct PgRowCfg {
   static constexpr int kEs = (int)sizeof(T);
   static constexpr int kRow = HD * kEs;               // bytes of a K or V row
-  static constexpr int kTileBytes = kPgTile * kRow;
-  static constexpr int kStage = 2 * kTileBytes;       // K then V
-  // 192 KB of rings per CTA: as many warps as keep three stages each
-  static constexpr int kWarps = kStage <= 8192 ? 8 : 65536 / kStage;
-  static constexpr int kStages = 196608 / (kWarps * kStage);
-  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kTileBytes = kPgTile * kRow;  // a tile's K or V
+  // 192 KB of rings per CTA, at least three places per warp: the one that it computes on and those in flight.  A place
+  // holds K and V of a tile; for fp32, whose split products keep a warp on a tile for 2.5K cycles, K or V, which makes room
+  // for twice the warps (one token on 128K keys, 8B heads: 175 -> 157 us; Gemma heads, 64 sequences: 264 -> 152; bf16 loses
+  // 5 % to the second wait a tile).  Four warps for head_dim 256, whose merge buffer is twice as large.
+  static constexpr bool kPair = kEs == 2;
+  static constexpr int kPlaceBytes = kPair ? 2 * kTileBytes : kTileBytes;
+  static constexpr int kWarps = HD == 256 ? 4 : 8;
+  static constexpr int kPlaces = 196608 / (kWarps * kPlaceBytes);
+  static constexpr int kRing = kWarps * kPlaces * kPlaceBytes;
   // one block of 8 rows per warp; at least the weights of kPgMaxCtas parts for 32 rows
   static constexpr int kMerge = kWarps * 8 * HD * 4 > 32 * kPgMaxCtas * 4 ? kWarps * 8 * HD * 4 : 32 * kPgMaxCtas * 4;
   static constexpr int kSmem = kRing + kMerge + kWarps * 32 * 2 * 4;
-  static_assert(kStages >= 3 && kSmem <= 232448 - 64, "shared memory of the row kernel");
+  static_assert(kPlaces >= 3 && kSmem <= 232448 - 64, "shared memory of the row kernel");
 };
 
 __device__ __forceinline__ void pg_cp16(uint32_t dst, const void* src, int bytes) {
@@ -148,7 +152,7 @@ template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_kernel(const PgRowArgs a) {
   using C = PgRowCfg<T, HD>;
   constexpr bool kB = sizeof(T) == 2;
-  constexpr int NW = C::kWarps, NS = C::kStages;
+  constexpr int NW = C::kWarps, NP = C::kPlaces;
   constexpr int MT = HD / 16;        // 16-value blocks of O^T
   constexpr int KS = HD / 16;        // bf16: k-steps of S; fp32: pairs of k-steps
   extern __shared__ __align__(128) unsigned char sm[];
@@ -171,14 +175,14 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
   const int seg_end = a.batch[l.row_first + blockIdx.x + 1];
   const PgSeg* segs = reinterpret_cast<const PgSeg*>(a.batch + l.row_segs);
   const int* tables = a.batch + h->tbl;
-  const uint32_t ring = smem_addr(sm) + warp * NS * C::kStage;
+  const uint32_t ring = smem_addr(sm) + warp * NP * C::kPlaceBytes;
   const T* kbase = static_cast<const T*>(a.storage);
   const long long head_elems = (long long)HD << a.shift;
 
   // ---- loads: tiles in the order they are used, across segments ----------------
   int is = a.batch[l.row_first + blockIdx.x];  // segment of the next tile to load
   const int seg0 = is;
-  int it = 0, ie = 0, ilo = 0, ihi = 0, itbl = 0, ikvh = 0, ipos0 = 0, ipage = 0, islot = 0;
+  int it = 0, ie = 0, ilo = 0, ihi = 0, itbl = 0, ikvh = 0, ipos0 = 0, ipage = 0;
   auto load_seg = [&]() {
     const PgSeg& s = segs[is];
     it = s.tile0 + warp, ie = s.tile1, ilo = s.key_lo, ihi = s.key_hi, itbl = s.tbl, ikvh = s.kvh, ipos0 = s.pos0;
@@ -188,11 +192,13 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
       if (++is < seg_end) load_seg();
     if (is < seg_end) ipage = tables[itbl + ((it * kPgTile) >> a.shift)];
   };
+  int iplace = 0;
+  bool iv = false;  // V of the tile is next, not K (places that hold one of the two)
   auto issue = [&]() {
     if (is < seg_end) {
-      const uint32_t dst = ring + islot * C::kStage;
+      const uint32_t dst = ring + iplace * C::kPlaceBytes;
       const int key0 = it * kPgTile;
-      const T* src = kbase + (long long)ipage * a.page_elems + ikvh * head_elems +
+      const T* src = kbase + (iv ? a.v_off : 0) + (long long)ipage * a.page_elems + ikvh * head_elems +
                      (long long)(key0 & ((1 << a.shift) - 1)) * HD;
 #pragma unroll
       for (int i = 0; i < C::kTileBytes / 512; ++i) {
@@ -201,20 +207,23 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
         const int bytes = key0 + r >= ilo && key0 + r < ihi ? 16 : 0;
         const uint32_t off = pg_piece<T, HD>(r, c);
         pg_cp16(dst + off, src + p * (16 / C::kEs), bytes);
-        pg_cp16(dst + C::kTileBytes + off, src + a.v_off + p * (16 / C::kEs), bytes);
+        if (C::kPair) pg_cp16(dst + C::kTileBytes + off, src + a.v_off + p * (16 / C::kEs), bytes);
       }
-      it += NW;
-      settle();
+      if (C::kPair || iv) {
+        it += NW;
+        settle();
+      }
+      if (!C::kPair) iv = !iv;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    islot = islot + 1 == NS ? 0 : islot + 1;
+    iplace = iplace + 1 == NP ? 0 : iplace + 1;
   };
   if (is < seg_end) load_seg();
   settle();
   // Rows of earlier batches are there already; the new tokens' rows, and q, come from the kernel before this one.
   bool waited = a.late != 0;
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i) {
+  for (int i = 0; i < NP - 1; ++i) {
     if (!waited && is < seg_end && (it + 1) * kPgTile > ipos0) {
       griddep_wait();
       waited = true;
@@ -223,7 +232,16 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
   }
   if (!waited) griddep_wait();
 
-  int cslot = 0;
+  // the next place in the order of use, once it is there; the place used before it goes to the load after the last
+  int cplace = 0;
+  auto next_place = [&]() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(NP - 2) : "memory");
+    __syncwarp();
+    issue();
+    const uint32_t at = ring + cplace * C::kPlaceBytes;
+    cplace = cplace + 1 == NP ? 0 : cplace + 1;
+    return at;
+  };
   for (int si = seg0; si < seg_end; ++si) {
     const PgSeg& sg = segs[si];
     const int n_rows = sg.n_rows, r0 = sg.r0, pos0 = sg.pos0, q_row0 = sg.q_row0, kvh = sg.kvh, key_lo = sg.key_lo,
@@ -270,11 +288,7 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
     }
 
     for (int t = tile0 + warp; t < tile1; t += NW) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(NS - 2) : "memory");
-      __syncwarp();
-      issue();  // into the stage that the tile before has left
-      const uint32_t ks = ring + cslot * C::kStage, vs = ks + C::kTileBytes;
-      cslot = cslot + 1 == NS ? 0 : cslot + 1;
+      const uint32_t ks = next_place();
       const int key0 = t * kPgTile;
       // ---- S^T = K Q^T --------------------------------------------------------------
       float sc[NT][4], sd[NT][4];
@@ -366,6 +380,7 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
             o[n][i][3] *= alpha[n][1];
           }
       }
+      const uint32_t vs = C::kPair ? ks + C::kTileBytes : next_place();
       // A tile that some rows attend to and others do not: a weight of 0 times a
       // value that is not finite would reach the others, so such values are
       // taken out and added below to the rows that attend to them.
