@@ -162,10 +162,10 @@ int l3p_paged_append_dev(l3p_paged_ctx* ctx, int layer, const void* k, long long
  * Capture: a captured launch reads the batch's description when it is
  * replayed, so one graph of a decoding step serves every later step whose
  * batch takes the same path with at most as many tokens as the captured one:
- * all of its sequences bring few tokens (at most 8, or at most 16, query rows
- * n_new * n_heads / n_kv_heads per KV head, the class of the largest).  A
- * replay on a batch that does not fit writes nothing for it and
- * l3p_paged_check reports L3P_E_INVAL.  An F32 chunk may need a workspace that
+ * with n_new * n_heads / n_kv_heads query rows per KV head, the largest count
+ * of a batch of few tokens is at most 8, or 9 to 16 (F32 pools: 9 to 64, with
+ * head_dim 256 9 and more).  A replay on a batch that does not fit writes
+ * nothing for it and l3p_paged_check reports L3P_E_INVAL.  An F32 chunk may need a workspace that
  * cannot grow during capture: make one call of the size before. */
 int l3p_paged_attn_dev(l3p_paged_ctx* ctx, int layer, const void* q, long long q_stride, void* out,
                        long long out_stride, void* stream);

@@ -124,14 +124,14 @@ struct BatchSeq {
   bool tc;                      // takes the tensor-core kernels
 };
 
-// Which kernels a sequence takes.  Up to 8 rows per KV head (up to row_limit, if no sequence of the batch has more): the
-// row kernel.  Sequences of 9 to row_limit rows go with the longer ones where there are some: two kernels, each with part
-// of the batch, fill the GPU less than one (16 drafts of 3 to 6 tokens, 8B heads: see the measurements in plan_tc).
+// Which kernels a sequence takes: the row kernel up to row_limit rows per KV head.  In bf16, sequences of 9 to row_limit
+// rows go with the longer ones where there are some: two kernels, each with part of the batch, fill the GPU less than one
+// (16 drafts of 12 to 24 rows, 8B heads: 58.6 us, by two kernels 72.5).
 void choose_paths(const Ctx* ctx, std::vector<BatchSeq>* bs) {
   const int limit = row_limit(ctx);
   bool any = false;
   for (const auto& b : *bs) any |= (long long)b.n_new * ctx->G > limit;
-  for (auto& b : *bs) b.tc = (long long)b.n_new * ctx->G > (any ? std::min(limit, 8) : limit);
+  for (auto& b : *bs) b.tc = (long long)b.n_new * ctx->G > (any && ctx->bf16 ? std::min(limit, 8) : limit);
 }
 
 // First key that the token at `pos` attends to.
@@ -146,7 +146,7 @@ int first_key(const Ctx* ctx, bool win, int pos) { return win ? std::max(0, pos 
 // A run or part is a multiple of the CTA's warps, which take its tiles in turn,
 // so both are counted in rounds of one tile per warp.  A further segment of a CTA
 // costs about kSegRounds rounds that its prefetched tiles do not hide (16
-// sequences x 2 tokens x 3000 keys, 8B heads: 46.8 us end to end, 39.5 us by units).
+// sequences x 4 tokens x 3000 keys, 8B heads: 46.8 us end to end, 38.5 us by units).
 constexpr double kSegRounds = 1.5;
 void plan_rows(Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, int nt, std::vector<int>* first,
                std::vector<PgSeg>* segs) {
@@ -455,7 +455,7 @@ size_t batch_capacity(const Ctx* ctx) {
   const size_t max_len = c.max_seq_len, rows = (size_t)c.max_tokens * ctx->G, kv = c.n_kv_heads, seqs = c.max_seqs;
   const bool only_rows = row_limit(ctx) == INT_MAX;
   // units of the row kernel: blocks of at least 8 rows; segments: one more per CTA at most
-  const size_t row_units = only_rows ? kv * (rows / 8 + seqs) : kv * 2 * seqs;
+  const size_t row_units = only_rows ? kv * (rows / 8 + seqs) : kv * (row_limit(ctx) / 8) * seqs;
   // units of the tensor-core kernels: blocks of at least 128 rows; parts: 3 num_sms more at most, as many merged units
   const size_t tc_units = only_rows ? 0 : kv * (rows / 128 + seqs);
   const size_t tiles = only_rows || ctx->bf16 ? 0 : 4 * seqs * ((max_len + 127) / 128 + 1);

@@ -9,10 +9,12 @@ using namespace l3p;
 
 namespace l3p_pg {
 
-// Sequences with more query rows per KV head take the tensor-core kernels.
-// fp32 with head_dim 256 has none: Q and O alone would fill tensor memory.
+// Sequences with more query rows per KV head take the tensor-core kernels.  16 sequences of 3000 keys, 8B heads, by the
+// row kernel and by the tensor-core kernel: bf16 16 rows 38.3 and 40.4 us (one such sequence 10.7 and 18.5), 32 rows 75.6
+// (blocks of 32 rows, since dropped) and 42.6; fp32, whose tensor-core kernel first splits every key tile, 64 rows 391 and
+// 459 us, 128 rows 751 and 465.  fp32 with head_dim 256 has none: Q and O alone would fill tensor memory.
 int row_limit(const l3p_paged_ctx* ctx) {
-  return !ctx->bf16 && ctx->hd == 256 ? INT_MAX : 16;
+  return ctx->bf16 ? 16 : ctx->hd == 256 ? INT_MAX : 64;
 }
 
 // Blocks of 8 rows whose Q and O fit a thread's registers.

@@ -19,7 +19,7 @@
 // That warpgroup also applies the running maximum's factors, so O is never
 // rescaled in tensor memory.
 //
-// What bounds it: 2 x 3072 tensor-core cycles per 128 rows x 128 keys.
+// What bounds it: 6144 tensor-core cycles per 128 rows x 128 keys.
 //
 // CG = 2 (head_dim 128): the CTAs of a pair take 128 rows each of the same KV
 // head; every MMA is cta_group::2 with M = 256, and each CTA stages half of

@@ -639,6 +639,61 @@ def test_captured_chunks(torch, dtype, dim):
             del graph
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 64), (32, 8, 128), (6, 3, 256), (71, 1, 64), (32, 1, 128), (20, 1, 256)])
+def test_few_tokens_of_every_sequence(torch, dtype, heads, kv, dim):
+    """As many sequences as the cache takes, with token counts around the ends of each path, alone and beside a long chunk."""
+    with _cache(n_heads=heads, n_kv_heads=kv, head_dim=dim, dtype=dtype, n_layers=1, max_seqs=12, n_pages=400, max_tokens=420) as c:
+        b = Books(torch, c, dim)
+        seqs = [b.new() for _ in range(12)]
+        b.step(seqs, [20 + i for i in range(12)])
+        for n in (2, 3, 4, 5, 8, 9, 16, 17, 32, 33):
+            b.step(seqs, [n] * 12)
+            for x in seqs:
+                c.truncate(x, 20)
+                b.rows[x] = [r[:20] for r in b.rows[x]]
+        b.step(seqs, [16] * 11 + [140])
+        b.step(seqs, [1, 2, 3, 4, 5, 8, 9, 16, 17, 32, 33, 34])
+
+
+@pytest.mark.parametrize("dtype,largest", [("f32", 16), ("bf16", 4)])
+def test_captured_few_tokens(torch, dtype, largest):
+    """A captured batch of few tokens serves up to the largest count of the same path."""
+    with _cache(n_heads=8, n_kv_heads=2, head_dim=128, dtype=dtype, n_layers=1, max_seqs=8, n_pages=400, max_tokens=500) as c:
+        b = Books(torch, c)
+        seqs = [b.new() for _ in range(8)]
+        past = [10 + 40 * i for i in range(8)]
+        for x, n in zip(seqs, past):
+            b.step([x], [n], attend=False)
+        n = largest * 8
+        q, out = b.randn(n, 8, 128), torch.empty(n, 8, 128, device="cuda", dtype=c.dtype)
+        kv = [b.randn(n, 2, 128) for _ in range(2)]
+        c.begin(seqs, [largest] * 8)
+        s = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            c.append_dev(0, *kv)
+            c.attn_dev(0, q, out)
+            c.check()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                c.append_dev(0, *kv)
+                c.attn_dev(0, q, out)
+            for new in ([largest] * 8, [3] * 8, [largest, 1, 2, 3, 1, 1, 1, 1], [0, largest, 0, 1, 0, 2, 0, 3]):
+                for x, m in zip(seqs, past):
+                    c.truncate(x, m)
+                c.begin(seqs, new)
+                out.fill_(9.0)
+                graph.replay()
+                c.check()
+                got = out.clone()
+                out.fill_(9.0)
+                c.attn_dev(0, q, out)
+                c.check()
+                assert bool((got == out).all()) and bool((got[sum(new):] == 9.0).all())
+            del graph
+
+
 def test_calls_during_capture_are_refused(torch):
     with _cache(n_layers=1) as c:
         b = Books(torch, c)
