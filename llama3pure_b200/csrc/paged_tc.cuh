@@ -283,29 +283,41 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
   if (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 0) {
     // ---------------- loads ----------------
+    // Few instructions a load: the softmax warps want the issue slots, and at 16 or 32 positions a page these loads bound
+    // the kernel (16 sequences x 9 tokens x 3000 keys, 8B heads, pages of 16: 49.5 us with stages and tiles found by
+    // division from the load's number, 44.0 us with running counters and a page looked up once for K and V, a tile ahead).
     const int box = min(1 << a.shift, TN), n_box = TN / box;  // keys of a box, boxes down a tile
     const int i = lane % n_box, c = lane / n_box;             // this lane's box and column block
-    const bool mine = c < HD / 64;
+    const int n_stage = dual ? S + kMore : S, lag = dual ? 1 : 0;
+    const int v_row = a.n_kv << a.shift, in_page = (1 << a.shift) - 1;
+    const int base = a.row_k + (u.kvh << a.shift);
+    const uint32_t to = smem_addr(ring) + c * (TN * 128) + i * (box * 128);
+    int key = u.tile0 * TN + i * box;  // this lane's first key of K tile j
+    const int key_end = c < HD / 64 ? u.key_hi : 0;
     bool ok = true;
-    int n_used = 0;
-    for (int t = 0; ok && t < 2 * nt; ++t) {
-      // tile j's K or V is the t-th load
-      const bool is_v = dual ? t >= 2 ? (t & 1) == 0 || t == 2 * nt - 1 : t == 1 && nt == 1 : (t & 1) != 0;
-      const int j = !dual ? t / 2 : is_v ? (t == 2 * nt - 1 ? nt - 1 : t / 2 - 1) : t < 2 ? t : (t + 1) / 2;
-      const int s = stage_of(t), use = use_of(t);
-      const int key = (u.tile0 + j) * TN + i * box;
-      const bool load = mine && key < u.key_hi;
-      const int page = load ? table[key >> a.shift] : 0;
-      if (use > 0) ok = __all_sync(0xffffffffu, pg_wait(&kv_empty[s], (uint32_t)((use - 1) & 1), a.err));
-      if (!ok) break;
-      const int n = __popc(__ballot_sync(0xffffffffu, load));
+    int n_used = 0, s = 0;
+    uint32_t free_parity = 1;  // of a stage's last release; at first no stage has to be waited for
+    auto load = [&](int row, bool mine) {
+      ok = __all_sync(0xffffffffu, pg_wait(&kv_empty[s], free_parity, a.err));
+      if (!ok) return;
+      const int n = __popc(__ballot_sync(0xffffffffu, mine));
       if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], (uint32_t)(n * box * 128));
       __syncwarp();
-      if (load) {
-        const int row = page * a.page_rows + a.row_k + (((is_v ? a.n_kv : 0) + u.kvh) << a.shift) + (key & ((1 << a.shift) - 1));
-        pg_tma_2d(smem_addr(ring + s * C::kStage + c * (TN * 128) + i * (box * 128)), &tmap, c * 64, row, &kv_full[s]);
-      }
-      n_used = t + 1;
+      if (mine) pg_tma_2d(to + s * C::kStage, &tmap, c * 64, row, &kv_full[s]);
+      ++n_used;
+      if (++s == n_stage) s = 0, free_parity ^= 1;
+    };
+    int page = key < key_end ? table[key >> a.shift] : 0, row_v = 0;
+    bool mine_v = false;
+    for (int j = 0; ok && j < nt + lag; ++j) {
+      const bool mine = key < key_end;
+      const int row = page * a.page_rows + base + (key & in_page);
+      key += TN;
+      if (j + 1 < nt) page = key < key_end ? table[key >> a.shift] : 0;
+      if (!dual) row_v = row + v_row, mine_v = mine;
+      if (j < nt) load(row, mine);
+      if (ok && j >= lag) load(row_v, mine_v);
+      row_v = row + v_row, mine_v = mine;
     }
     // no copy may still be landing when the CTA ends
     for (int t = max(0, n_used - S - (dual ? kMore : 0)); t < n_used; ++t) pg_wait(&kv_full[stage_of(t)], (uint32_t)(use_of(t) & 1), a.err);
