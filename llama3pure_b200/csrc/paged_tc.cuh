@@ -14,16 +14,18 @@
 // than 2^8 since its reference was set; the reference is exact, so this
 // changes no result but by rounding.
 //
-// What bounds it: for head_dim 128 the MMAs of a tile pair take 2048 cycles and
-// so do its 32K exponentials at 16 a cycle.  Two Q tiles in turn keep the tensor
-// core on one while the other's softmax runs.
+// What bounds it: for head_dim 128 the MMAs of a key tile and both Q tiles take
+// 2048 cycles, and so do its 32K exponentials at 16 a cycle; with the rest of
+// softmax and its hand-over to the tensor core it is 3.8K cycles (four chunks of
+// 2K tokens on up to 8K keys: 981 TFLOP/s).  Two Q tiles in turn keep the tensor core
+// on one while the other's softmax runs.  Up to 128 rows: the loads, 4.8 TB/s.
 //
 // Tiles come from the pages by TMA, one box per page (or 128-key tile) and 64
 // columns, into a ring in consumption order K0 V0 K1 V1 ..., 128-byte swizzled:
 // K is the K-major B operand of S, V the MN-major B operand of O.
 //
-// Roles: warp 0 loads; warp 1 issues MMAs; warps 2 and 3 check V tiles that some row
-// does not attend to entirely (masked weights are 0, and 0 times a value that
+// Roles: warps 0 and 3 load K and V; warp 1 issues MMAs; warp 2, of the last tiles with
+// warp 3, checks V tiles that some row does not attend to entirely (masked weights are 0, and 0 times a value that
 // is not finite is NaN: rows outside every window become 0, such values are
 // taken out and added in the epilogue to the rows that attend to them); warps
 // 4-7 and 8-11 are the softmax of Q tile 0 and 1.
@@ -214,7 +216,7 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
   __shared__ uint32_t s_tmem;
   __shared__ int s_bad;
   __shared__ float s_m1[128], s_l1[128];
-  __shared__ __align__(8) uint64_t kv_full[S + 2], kv_empty[S + 2], v_ok[S];
+  __shared__ __align__(8) uint64_t k_full[S], v_full[S], v_ok[S], kv_empty[S + 2];
   __shared__ __align__(8) uint64_t s_full[2], p_full[2][2], o_done[2], q_ready[2], mma_idle;
 
   const PgHeader* h = reinterpret_cast<const PgHeader*>(a.batch);
@@ -242,23 +244,26 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
   static_assert(kMore <= 2, "barriers");
   unsigned char* ring = sq + C::kQBytes - (dual ? kMore * C::kStage : 0);
   auto stage_of = [&](int t) { return dual ? t % (S + kMore) : t % S; };
-  auto use_of = [&](int t) { return dual ? t / (S + kMore) : t / S; };
   auto k_at = [&](int j) { return dual ? (j < 2 ? j : 2 * j - 1) : 2 * j; };             // position of K tile j in the ring's order
   auto v_at = [&](int j) { return dual ? min(2 * j + 2, 2 * nt - 1) : 2 * j + 1; };      // and of V tile j
   const int first_pos = u.pos0 + u.r0 / a.G, last_pos = u.pos0 + (u.r0 + u.n_rows - 1) / a.G;
   const int lo_first = a.win ? max(0, first_pos - a.window + 1) : 0;  // keys below: no row attends to them
   const int lo_last = a.win ? max(0, last_pos - a.window + 1) : 0;    // keys from here to first_pos: every row does
 
+  // Barriers.  A wait tells one phase from its neighbours only, so a barrier's phases follow what its waiter has seen:
+  // k_full, v_full and v_ok are by the tile's number (the stage alternates between K and V in most rings, and the
+  // waiter for one has not seen the other land), kv_empty by stage, in about whose order stages are released.
   if (warp == 0) {
     tc::tmem_alloc(&s_tmem, 512);
     tc::tmem_relinquish();
   }
   if (tid == 32) {
-    for (int s = 0; s < S + 2; ++s) {
-      mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_ok[s], 2);
     }
-    for (int s = 0; s < S; ++s) mbar_init(&v_ok[s], 2);
+    for (int s = 0; s < S + 2; ++s) mbar_init(&kv_empty[s], 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(&s_full[b], 1);
       mbar_init(&p_full[b][0], 4);
@@ -280,47 +285,49 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
   // Registers: 384 x 168 at launch = 128 x 88 + 256 x 208.  Inside the branches: behind their join the compiler would
   // count with the smaller number.
   if (warp < 4) {
+  bool loaded = true;
   if (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-  if (warp == 0) {
-    // ---------------- loads ----------------
+  if (warp == 0 || warp == 3) {
+    // ---------------- loads: warp 0 K, warp 3 V ----------------
     // Few instructions a load: the softmax warps want the issue slots, and at 16 or 32 positions a page these loads bound
     // the kernel (16 sequences x 9 tokens x 3000 keys, 8B heads, pages of 16: 49.5 us with stages and tiles found by
-    // division from the load's number, 44.0 us with running counters and a page looked up once for K and V, a tile ahead).
+    // division from the load's number, 44.0 us with running counters and a page looked up a tile ahead, 41.1 us with a warp
+    // for K and one for V).  A load waits for the release one ring earlier, and the warp's load before it has waited for a
+    // later release than the one two rings earlier: one phase.
+    const bool is_v = warp == 3;
     const int box = min(1 << a.shift, TN), n_box = TN / box;  // keys of a box, boxes down a tile
     const int i = lane % n_box, c = lane / n_box;             // this lane's box and column block
-    const int n_stage = dual ? S + kMore : S, lag = dual ? 1 : 0;
-    const int v_row = a.n_kv << a.shift, in_page = (1 << a.shift) - 1;
-    const int base = a.row_k + (u.kvh << a.shift);
+    const int n_stage = dual ? S + kMore : S, in_page = (1 << a.shift) - 1;
+    const int base = a.row_k + ((u.kvh + (is_v ? a.n_kv : 0)) << a.shift);
     const uint32_t to = smem_addr(ring) + c * (TN * 128) + i * (box * 128);
-    int key = u.tile0 * TN + i * box;  // this lane's first key of K tile j
     const int key_end = c < HD / 64 ? u.key_hi : 0;
-    bool ok = true;
-    int n_used = 0, s = 0;
+    auto at = [&](int j) { return is_v ? v_at(j) : k_at(j); };
+    int key = u.tile0 * TN + i * box;  // this lane's first key of tile j
+    int page = key < key_end ? table[key >> a.shift] : 0;
+    uint64_t* fulls = is_v ? v_full : k_full;
+    int s = at(0), n_used = 0, fb = 0;
     uint32_t free_parity = 1;  // of a stage's last release; at first no stage has to be waited for
-    auto load = [&](int row, bool mine) {
-      ok = __all_sync(0xffffffffu, pg_wait(&kv_empty[s], free_parity, a.err));
-      if (!ok) return;
-      const int n = __popc(__ballot_sync(0xffffffffu, mine));
-      if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], (uint32_t)(n * box * 128));
-      __syncwarp();
-      if (mine) pg_tma_2d(to + s * C::kStage, &tmap, c * 64, row, &kv_full[s]);
-      ++n_used;
-      if (++s == n_stage) s = 0, free_parity ^= 1;
-    };
-    int page = key < key_end ? table[key >> a.shift] : 0, row_v = 0;
-    bool mine_v = false;
-    for (int j = 0; ok && j < nt + lag; ++j) {
+    while (n_used < nt) {
       const bool mine = key < key_end;
       const int row = page * a.page_rows + base + (key & in_page);
       key += TN;
-      if (j + 1 < nt) page = key < key_end ? table[key >> a.shift] : 0;
-      if (!dual) row_v = row + v_row, mine_v = mine;
-      if (j < nt) load(row, mine);
-      if (ok && j >= lag) load(row_v, mine_v);
-      row_v = row + v_row, mine_v = mine;
+      page = key < key_end ? table[key >> a.shift] : 0;
+      if (!__all_sync(0xffffffffu, pg_wait(&kv_empty[s], free_parity, a.err))) break;
+      const int n = __popc(__ballot_sync(0xffffffffu, mine));
+      uint64_t* full = fulls + fb;
+      if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(n * box * 128));
+      __syncwarp();
+      if (mine) pg_tma_2d(to + s * C::kStage, &tmap, c * 64, row, full);
+      ++n_used;
+      if (++fb == S) fb = 0;
+      s += dual && n_used == (is_v ? nt - 1 : 1) ? 1 : 2;  // the next one's place in the order of use
+      if (s >= n_stage) s -= n_stage, free_parity ^= 1;
     }
-    // no copy may still be landing when the CTA ends
-    for (int t = max(0, n_used - S - (dual ? kMore : 0)); t < n_used; ++t) pg_wait(&kv_full[stage_of(t)], (uint32_t)(use_of(t) & 1), a.err);
+    loaded = n_used == nt;
+    // no copy may still be landing when the CTA ends (of V, warp 3 waits for the last three tiles below; the ones before had
+    // landed when it could load the last)
+    if (!is_v || !loaded)
+      for (int j = max(0, n_used - S); j < n_used; ++j) pg_wait(&fulls[j % S], (uint32_t)(j / S & 1), a.err);
   } else if (warp == 1) {
     // ---------------- MMA issue ----------------
     constexpr uint32_t id_s = idesc_bf16(128, TN, false), id_o = idesc_bf16(128, HD, true);
@@ -348,14 +355,23 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
       return r;
     };
     bool ok = true;
+    // running numbers instead of divisions (16 sequences x 9 tokens x 3000 keys, head_dim 64: 29.3 -> 26.8 us): V tile j's and
+    // the next K tile's barriers, phases and stages
+    int vb = 0, vp = 0, kb = 0, kp = 0;
+    auto next_v = [&] { if (++vb == S) vb = 0, vp ^= 1; };
+    auto next_k = [&] { if (++kb == S) kb = 0, kp ^= 1; };
+    auto step = [&](int x, int by, int n) { return x + by >= n ? x + by - n : x + by; };
     if (dual) {
       // stream b = j & 1: O += P V of key tile j, then S of key tile j + 2
+      constexpr int n = S + kMore;
+      int sv = stage_of(v_at(0)), sk = 0;
       ok = wait(&q_ready[0], 0);
       for (int j = -2; ok && j < nt; ++j) {
-        const int b = j & 1, sv = stage_of(max(0, v_at(j))), tk = k_at(j + 2), sk = stage_of(tk);
+        const int b = j & 1;
         const bool next = j + 2 < nt;
         if (j >= 0) {
-          if (!(ok = wait(&v_ok[j % S], j / S))) break;
+          if (!(ok = wait(&v_ok[vb], vp))) break;
+          next_v();
 #pragma unroll
           for (int hf = 0; hf < C::kHands; ++hf) {
             if (!(ok = ok && wait(&p_full[b][hf], j >> 1))) break;
@@ -364,29 +380,33 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
           if (!ok) break;
           pg_commit(leader, &kv_empty[sv]);
           pg_commit(leader, &o_done[b]);
+          sv = step(sv, j + 2 == nt ? 1 : 2, n);
         }
         if (next) {
-          if (!(ok = wait(&kv_full[sk], use_of(tk)))) break;
+          if (!(ok = wait(&k_full[kb], kp))) break;
+          next_k();
           qk(0, b, sk);
           pg_commit(leader, &s_full[b]);
           pg_commit(leader, &kv_empty[sk]);
+          sk = step(sk, j == -2 ? 1 : 2, n);
         }
       }
     } else {
-      ok = wait(&kv_full[0], 0);
+      ok = wait(&k_full[0], 0);
       for (int b = 0; ok && b < nq; ++b) {
         if (!(ok = wait(&q_ready[b], 0))) break;
         qk(b, NQ == 2 ? b : 0, 0);
         pg_commit(leader, &s_full[b]);
       }
       pg_commit(leader, &kv_empty[0]);
+      next_k();
     }
+    int sv = 1, sk = 2;
     for (int j = 0; ok && !dual && j < nt; ++j) {
-      const int tv = 2 * j + 1, tk = 2 * j + 2, sv = tv % S, sk = tk % S;
       if constexpr (NQ == 2) {
         // per Q tile: O += P V, then S of the next key tile.  MMAs run in the order of issue, so S may overwrite the P
         // that the product before it reads
-        if (!(ok = wait(&v_ok[j % S], j / S) && (j + 1 == nt || wait(&kv_full[sk], tk / S)))) break;
+        if (!(ok = wait(&v_ok[vb], vp) && (j + 1 == nt || wait(&k_full[kb], kp)))) break;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           if (b >= nq || !ok) break;
@@ -409,30 +429,37 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
       } else {
         // one Q tile, S in two places: S of the next key tile is issued ahead of this tile's O += P V
         if (j + 1 < nt) {
-          if (!(ok = wait(&kv_full[sk], tk / S))) break;
+          if (!(ok = wait(&k_full[kb], kp))) break;
           qk(0, (j + 1) & 1, sk);
           pg_commit(leader, &s_full[(j + 1) & 1]);
           pg_commit(leader, &kv_empty[sk]);
         }
-        if (!(ok = wait(&v_ok[j % S], j / S) && wait(&p_full[j & 1][0], j >> 1))) break;
+        if (!(ok = wait(&v_ok[vb], vp) && wait(&p_full[j & 1][0], j >> 1))) break;
         pv(0, j & 1, sv, 0, j > 0);
         pg_commit(leader, &kv_empty[sv]);
         pg_commit(leader, &o_done[j & 1]);
       }
+      next_v(), next_k();
+      sv = step(sv, 2, S), sk = step(sk, 2, S);
     }
     // every MMA has ended before tensor memory is released
     pg_commit(leader, &mma_idle);
     pg_wait(&mma_idle, 0, a.err);
-  } else {
-    // ---------------- warps 2, 3: V tiles that are not attended to entirely ----------------
-    bool ok = true;
-    for (int j = 0; ok && j < nt; ++j) {
-      const int t = v_at(j), s = stage_of(t);
-      ok = __all_sync(0xffffffffu, pg_wait(&kv_full[s], (uint32_t)(use_of(t) & 1), a.err));
+  }
+  if (warp >= 2) {
+    // ---------------- V tiles that are not attended to entirely ----------------
+    // Warp 2; the last three tiles, where most of them are, with warp 3, whose loads do not wait for those (four chunks of
+    // 2K tokens, 8B heads: 214.7 us with warp 2 alone, 210.6 with both).
+    const int both = max(0, nt - 3), j0 = warp == 2 ? 0 : both;
+    int vb = j0 % S, vp = j0 / S & 1;
+    bool ok = loaded;
+    for (int j = j0; ok && j < nt; ++j) {
+      ok = __all_sync(0xffffffffu, pg_wait(&v_full[vb], (uint32_t)vp, a.err));
       if (!ok) break;
-      const int key0 = (u.tile0 + j) * TN;
+      const int key0 = (u.tile0 + j) * TN, n_warps = j < both ? 1 : 2;
       if (key0 + TN - 1 > first_pos || key0 < lo_last) {
         bool bad = false;
+        const int s = stage_of(v_at(j));
         // keys [a, b) of the tile
         auto check = [&](int ka, int kb) {
           const int n = (kb - ka) * 8;  // 16-byte pieces of a 64-column block
@@ -440,7 +467,7 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
           for (int c = 0; c < HD / 64; ++c) {
             unsigned char* v = ring + s * C::kStage + c * (TN * 128) + (ka - key0) * 128;
 #pragma unroll 4
-            for (int x = (warp - 2) * 32 + lane; x < n; x += 64) {
+            for (int x = (j < both ? 0 : (warp - 2) * 32) + lane; x < n; x += 32 * n_warps) {
               const int key = ka + x / 8;
               uint4* p = reinterpret_cast<uint4*>(v + x * 16);
               uint4 w = *p;
@@ -460,7 +487,8 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
-      if (lane == 0) mbar_arrive(&v_ok[j % S]);  // by V tile: a stage holds K tiles in between
+      if (lane < 3 - n_warps) mbar_arrive(&v_ok[vb]);
+      if (++vb == S) vb = 0, vp ^= 1;
     }
   }
   } else {
