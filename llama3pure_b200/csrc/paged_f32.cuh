@@ -171,7 +171,13 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
   extern __shared__ unsigned char f32_smem_raw[];
   __shared__ uint32_t s_tmem;
   __shared__ float s_alpha[2][128], s_m[128], s_l[2][128], s_max[2][2][128];
-  __shared__ __align__(8) uint64_t bar_kv_full[S], bar_kv_empty[S], bar_kv_peer[S];
+  // Chunks in a CTA (full) and in the pair's other one (peer), by tile number modulo 3, not by stage: S and O have waiters
+  // of their own, which have not seen the other's chunk land in a stage before theirs, and a wait tells a phase from its
+  // neighbours only.  A chunk of tile t + 3 is loaded after a release that follows both waiters' use of tile t.
+  __shared__ __align__(8) uint64_t bar_kv_full[3 * Gm::kChunks], bar_kv_peer[3 * Gm::kChunks], bar_kv_empty[S];
+  auto k_bar = [](int t, int ch) { return t % 3 * Gm::kKChunks + ch; };
+  auto v_bar = [](int t, int ch) { return 3 * Gm::kKChunks + t % 3 * Gm::kVChunks + ch; };
+  static_assert(S < 3 * Gm::kChunks / 2, "the reach of the ring");
   __shared__ __align__(8) uint64_t bar_s_full, bar_s_free, bar_p_full[2], bar_p_free[2][2];
   __shared__ __align__(8) uint64_t bar_o_full, bar_o_free, bar_q_ready, bar_sm_done, bar_alpha[2], bar_mma_idle[2];
 
@@ -205,11 +211,11 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
     tc::tmem_relinquish_g<CG>();
   }
   if (tid == 32) {
-    for (int s = 0; s < S; ++s) {
+    for (int s = 0; s < 3 * Gm::kChunks; ++s) {
       mbar_init(&bar_kv_full[s], 1);
-      mbar_init(&bar_kv_empty[s], 1);
       mbar_init(&bar_kv_peer[s], 1);
     }
+    for (int s = 0; s < S; ++s) mbar_init(&bar_kv_empty[s], 1);
     mbar_init(&bar_s_full, 1);
     mbar_init(&bar_s_free, 8 * CG);
     for (int b = 0; b < 2; ++b) {
@@ -267,7 +273,7 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 || warp == 2) {
-      // ---------------- producers, chunks in turn ----------------
+      // ---------------- producers: every second stage each ----------------
       if (lane == 0) {
         const int me = warp >> 1;
         const unsigned char* img = reinterpret_cast<const unsigned char*>(a.img) + img_slot * Gm::kTileBytes + rank * C::kHalfTile;
@@ -279,8 +285,8 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
             if (t < 0 || t >= nt) continue;
             const int n_ch = part == 0 ? Gm::kKChunks : Gm::kVChunks;
             for (int ch = 0; ch < n_ch; ++ch, ++c) {
-              if (c % kProducers != me) continue;
               const int s = c % S, use = c / S;
+              if (s % kProducers != me) continue;  // a stage is always the same warp's, which has seen its last release
               if (use >= 1 && !wait(&bar_kv_empty[s], (uint32_t)((use - 1) & 1))) {
                 ok = false;
                 break;
@@ -288,24 +294,39 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
               const uint32_t bytes = part == 0 ? C::kKBytes : C::kVBytes;
               const long long off = part == 0 ? (long long)ch * C::kKBytes
                                               : (long long)Gm::kKChunks * C::kKBytes + (long long)ch * C::kVBytes;
-              mbar_arrive_expect_tx(&bar_kv_full[s], bytes);
+              uint64_t* full = &bar_kv_full[part == 0 ? k_bar(t, ch) : v_bar(t, ch)];
+              mbar_arrive_expect_tx(full, bytes);
               asm volatile(
                   "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                       smem_addr(ring + s * C::kStageBytes)),
-                  "l"(img + (long long)t * Gm::kTileBytes + off), "r"(bytes), "r"(smem_addr(&bar_kv_full[s]))
+                  "l"(img + (long long)t * Gm::kTileBytes + off), "r"(bytes), "r"(smem_addr(full))
                   : "memory");
             }
           }
         }
         // no copy of this thread may still be landing when the CTA ends
-        for (int i = c > S ? c - S : 0; i < c; ++i)
-          if (i % kProducers == me) wait(&bar_kv_full[i % S], (uint32_t)((i / S) & 1));
+        const int n0 = max(0, c - S) / Gm::kChunks;  // K of tile n0 and V of the tile before are not later than the last S loads
+        for (int n = n0, i = n0 == 0 ? 0 : n0 * Gm::kChunks - Gm::kVChunks; n <= nt && i < c; ++n)
+          for (int part = 0; part < 2; ++part) {
+            const int t = n - part, n_ch = part == 0 ? Gm::kKChunks : Gm::kVChunks;
+            if (t < 0 || t >= nt) continue;
+            for (int ch = 0; ch < n_ch; ++ch, ++i)
+              if (i >= c - S && i < c && i % S % kProducers == me)
+                wait(&bar_kv_full[part == 0 ? k_bar(t, ch) : v_bar(t, ch)], (uint32_t)((t / 3) & 1));
+          }
       }
     } else if (warp == 1 && rank == 1) {
       if (lane == 0)  // relay: chunk landed here -> issuers
-        for (int c = 0; c < Gm::kChunks * nt; ++c) {
-          if (!wait(&bar_kv_full[c % S], (uint32_t)((c / S) & 1))) break;
-          asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mapa_shared(smem_addr(&bar_kv_peer[c % S]), 0)) : "memory");
+        for (int n = 0; n < 2 * nt; ++n) {  // K0 K1 V0 K2 V1 ...
+          const bool v = n == 2 * nt - 1 || (n > 0 && (n & 1) == 0);
+          const int t = !v ? (n + 1) / 2 : n == 2 * nt - 1 ? nt - 1 : n / 2 - 1, n_ch = v ? Gm::kVChunks : Gm::kKChunks;
+          bool ok = true;
+          for (int ch = 0; ok && ch < n_ch; ++ch) {
+            const int b = v ? v_bar(t, ch) : k_bar(t, ch);
+            ok = wait(&bar_kv_full[b], (uint32_t)((t / 3) & 1));
+            if (ok) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mapa_shared(smem_addr(&bar_kv_peer[b]), 0)) : "memory");
+          }
+          if (!ok) break;
         }
     } else if (rank == 0) {
       // ---------------- MMA issuers: warp 1 S, warp 3 O ----------------
@@ -315,10 +336,9 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
       auto wait_all = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, wait(bar, parity)); };
       auto k_chunk0 = [&](int t) { return t == 0 ? 0 : nK + (t - 1) * nKV; };
       auto v_chunk0 = [&](int t) { return t + 1 < nt ? 2 * nK + t * nKV : nK + t * nKV; };
-      auto chunk_ready = [&](int c) -> bool {
-        const int s = c % S, use = c / S;
-        if (!wait_all(&bar_kv_full[s], (uint32_t)(use & 1))) return false;
-        if (CG == 2 && !wait_all(&bar_kv_peer[s], (uint32_t)(use & 1))) return false;
+      auto chunk_ready = [&](int b, int t) -> bool {
+        if (!wait_all(&bar_kv_full[b], (uint32_t)((t / 3) & 1))) return false;
+        if (CG == 2 && !wait_all(&bar_kv_peer[b], (uint32_t)((t / 3) & 1))) return false;
         tc::fence_after_sync();
         return true;
       };
@@ -337,7 +357,7 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
           }
 #pragma unroll 1
           for (int ch = 0; ch < nK; ++ch) {  // the small products
-            if (!(ok = chunk_ready(k_chunk0(t) + ch))) break;
+            if (!(ok = chunk_ready(k_bar(t, ch), t))) break;
             const uint64_t kh = desc_add(k_d, stage(k_chunk0(t) + ch)), kl = desc_add(kh, C::kStageBytes / 2);
             const uint64_t ql = desc_add(qlo_d, ch * 16384);
 #pragma unroll
@@ -365,7 +385,7 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
 #pragma unroll 1
           for (int qq = 0; ok && qq < Gm::kVChunks; ++qq) {
             const int c = v_chunk0(t) + qq, slot = qq & 1;
-            if (!(ok = chunk_ready(c))) break;
+            if (!(ok = chunk_ready(v_bar(t, qq), t))) break;
             // a new partial sum every 64 keys: the one before has been taken
             const int half = 2 * t + (qq >> 1);
             if (slot == 0 && half >= 1 && !(ok = wait_all(&bar_o_free, (uint32_t)((half - 1) & 1)))) break;
