@@ -573,7 +573,6 @@ int begin(Ctx* ctx, int n_seqs, const int* ids, const int* n_new, cudaStream_t s
   // shared last pages that a sequence grows into: the holder that finds others
   // beside it takes a copy; a page all of whose holders grow stays with the last one
   std::vector<std::pair<int, int>> cow;  // (index in the batch, page)
-  std::vector<int> left;                 // holders of cow[i].second after the copies before it
   for (int i = 0; i < n_seqs; ++i) {
     const auto& q = ctx->seqs[ids[i]];
     if (n_new[i] == 0 || (q.len & (ctx->cfg.page_size - 1)) == 0) continue;
@@ -582,7 +581,6 @@ int begin(Ctx* ctx, int n_seqs, const int* ids, const int* n_new, cudaStream_t s
   }
   {
     std::vector<std::pair<int, int>> take;
-    std::vector<int> gone;  // pages of the copies taken so far
     std::vector<int> count(cow.empty() ? 0 : ctx->cfg.n_pages, 0);
     for (const auto& x : cow)
       if (ctx->refs[x.second] - count[x.second] > 1) {
