@@ -17,7 +17,7 @@
 // What bounds it: for head_dim 128 the MMAs of a key tile and both Q tiles take
 // 2048 cycles, and so do its 32K exponentials at 16 a cycle; with the rest of
 // softmax and its hand-over to the tensor core it is 3.8K cycles (four chunks of
-// 2K tokens on up to 8K keys: 981 TFLOP/s).  Two Q tiles in turn keep the tensor core
+// 2K tokens on up to 8K keys: 960 TFLOP/s).  Two Q tiles in turn keep the tensor core
 // on one while the other's softmax runs.  Up to 128 rows: the loads, 4.8 TB/s.
 //
 // Tiles come from the pages by TMA, one box per page (or 128-key tile) and 64
