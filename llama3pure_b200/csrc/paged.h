@@ -214,8 +214,9 @@ inline bool windowed(const l3p_paged_ctx* ctx, int layer) {
 }
 
 // Launches a kernel that may start while the one before it on the stream ends:
-// every such kernel reads only the batch description (and cache rows of earlier
-// batches) ahead of its griddep_wait.
+// ahead of its griddep_wait every such kernel reads only the batch description,
+// which a copy brought.  (The row kernel beside a tensor-core kernel of the same
+// call starts behind that kernel's own wait, and waits for it at its end.)
 template <typename... P, typename... A>
 int launch(l3p_paged_ctx* ctx, void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t s, int cluster, A... args) {
   cudaLaunchConfig_t lc{};

@@ -182,10 +182,10 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
   // ---- loads: tiles in the order they are used, across segments ----------------
   int is = a.batch[l.row_first + blockIdx.x];  // segment of the next tile to load
   const int seg0 = is;
-  int it = 0, ie = 0, ilo = 0, ihi = 0, itbl = 0, ikvh = 0, ipos0 = 0, ipage = 0;
+  int it = 0, ie = 0, ilo = 0, ihi = 0, itbl = 0, ikvh = 0, ipage = 0;
   auto load_seg = [&]() {
     const PgSeg& s = segs[is];
-    it = s.tile0 + warp, ie = s.tile1, ilo = s.key_lo, ihi = s.key_hi, itbl = s.tbl, ikvh = s.kvh, ipos0 = s.pos0;
+    it = s.tile0 + warp, ie = s.tile1, ilo = s.key_lo, ihi = s.key_hi, itbl = s.tbl, ikvh = s.kvh;
   };
   auto settle = [&]() {  // to the next tile of this warp, and its page
     while (is < seg_end && it >= ie)
@@ -220,17 +220,12 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
   };
   if (is < seg_end) load_seg();
   settle();
-  // Rows of earlier batches are there already; the new tokens' rows, and q, come from the kernel before this one.
-  bool waited = a.late != 0;
+  // q and the new tokens' rows come from the kernel before this one, and older rows may: begin copies shared pages, callers
+  // write the storage with kernels of their own, and none of that is visible before the wait (tiles of older rows loaded
+  // ahead of it saved 0.2 to 1.2 us a layer: one token on 8K keys, 8B heads, with its rotation 14.0 us, now 15.2).
+  if (!a.late) griddep_wait();
 #pragma unroll
-  for (int i = 0; i < NP - 1; ++i) {
-    if (!waited && is < seg_end && (it + 1) * kPgTile > ipos0) {
-      griddep_wait();
-      waited = true;
-    }
-    issue();
-  }
-  if (!waited) griddep_wait();
+  for (int i = 0; i < NP - 1; ++i) issue();
 
   // the next place in the order of use, once it is there; the place used before it goes to the load after the last
   int cplace = 0;

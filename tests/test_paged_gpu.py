@@ -794,3 +794,77 @@ def test_create_without_memory(torch):
         _cache(n_layers=64, n_heads=8, n_kv_heads=8, head_dim=256, page_size=128, n_pages=16000)  # 537 GB
     assert e.value.code == -4
     assert torch.zeros(4, device="cuda").sum().item() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("page", [32, 128])
+@pytest.mark.parametrize("rotate", [False, True])
+def test_rows_copied_for_a_fork_are_read_after_the_copy(torch, dtype, page, rotate):
+    """begin, append and attention of many children of a prompt at once: whole tiles of each child's history are what begin
+    copies.  The pool holds garbage before, so that a row read too early shows."""
+    n, past, heads, kv, dim = 48, 3 * page + page - 1, 8, 2, 128
+    with _cache(n_heads=heads, n_kv_heads=kv, head_dim=dim, dtype=dtype, page_size=page, n_layers=2, n_pages=n + 8, max_seqs=n + 1,
+                max_tokens=past) as c:
+        c.set_rope(max_pos=past + 8)
+        b = Books(torch, c)
+        s = b.new()
+        b.step([s], [past], attend=False)
+        for _ in range(5):
+            kids = c.fork(s, n)
+            own = torch.arange(4, n + 4, device="cuda")  # the children's own last pages
+            c.storage()[own] = 1e30
+            qkv = b.randn(n, heads + 2 * kv, dim)
+            q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv], qkv[:, heads + kv:]
+            qr, outs = torch.empty(n, heads, dim, device="cuda", dtype=c.dtype), [torch.empty(n, heads, dim, device="cuda", dtype=c.dtype) for _ in range(2)]
+            torch.cuda.synchronize()
+            c.begin(kids, [1] * n)
+            for layer in range(2):
+                if rotate:
+                    c.rope_append_dev(layer, q, k, v, qr)
+                else:
+                    c.append_dev(layer, k, v)
+                c.attn_dev(layer, qr if rotate else q, outs[layer])
+            c.check()
+            last = c.tables(kids)[:, -1]
+            assert sorted(last.tolist()) == own.tolist()
+            for layer in range(2):
+                new = c.storage()[torch.from_numpy(last).cuda().long(), layer, :, :, past % page]  # [n, 2, kv, dim]: the rows as they were appended
+                for i in range(n):
+                    rows = torch.cat([b.rows[s][layer], new[i:i + 1]])
+                    want, tol = _want(torch, (qr if rotate else q)[i:i + 1], rows[:, 0], rows[:, 1], past)
+                    _near(outs[layer][i:i + 1], want, tol, f"child {i}, layer {layer}")
+            c.free(kids)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_that_the_caller_writes_ahead_of_attention(torch, dtype):
+    """Old rows replaced through storage() right before append and attention, and right before attention."""
+    with _cache(dtype=dtype, n_layers=1, page_size=64, n_pages=80, max_tokens=4000) as c:
+        b = Books(torch, c)
+        s = b.new()
+        b.step([s], [3990], attend=False)
+        table = torch.from_numpy(c.tables([s])[0]).cuda().long()
+        for when in ("append", "attention"):
+            past = c.length(s)
+            rows = b.randn(past, 2, 2, 128)
+            pages = torch.zeros(len(table) * 64, 2, 2, 128, device="cuda", dtype=c.dtype)
+            pages[:past] = rows
+            pages = pages.reshape(len(table), 64, 2, 2, 128).permute(0, 2, 3, 1, 4).contiguous()
+            q, k, v = b.randn(1, 8, 128), b.randn(1, 2, 128), b.randn(1, 2, 128)
+            out = torch.empty_like(q)
+            c.begin([s], [1])
+            torch.cuda.synchronize()
+            if when == "append":
+                c.storage()[table, 0] = pages
+                c.append_dev(0, k, v)
+            else:
+                c.append_dev(0, k, v)
+                new = c.storage()[table[-1], 0, :, :, past % 64].clone()
+                c.storage()[table, 0] = pages
+                c.storage()[table[-1], 0, :, :, past % 64] = new
+            c.attn_dev(0, q, out)
+            c.check()
+            kv = torch.cat([rows, torch.stack([k, v], 1)])
+            want, tol = _want(torch, q, kv[:, 0], kv[:, 1], past)
+            _near(out, want, tol, when)
+            b.rows[s] = [kv]
