@@ -38,6 +38,11 @@ void drop_page(Ctx* ctx, int p) {
   }
 }
 
+// Room for n pages in all, without a change; grown by doubling.
+void reserve_pages(std::vector<int>* pages, size_t n) {
+  if (pages->capacity() < n) pages->reserve(std::max(n, 2 * pages->capacity()));
+}
+
 int check_seq(Ctx* ctx, int seq) {
   if (seq < 0 || seq >= (int)ctx->seqs.size() || !ctx->seqs[seq].live)
     return fail(ctx, L3P_E_RANGE, "there is no sequence %d", seq);
@@ -88,7 +93,6 @@ int take_slot(Ctx* ctx, size_t words, Ctx::Slot** out) {
     }
     s.words = want;
   }
-  if (!s.done) PG_CUDA(ctx, cudaEventCreateWithFlags(&s.done, cudaEventDisableTiming));
   *out = &s;
   return L3P_OK;
 }
@@ -100,11 +104,9 @@ int upload(Ctx* ctx, Ctx::Slot* s, int* dev, size_t words, cudaStream_t st) {
   return L3P_OK;
 }
 
-// Enqueues the page copies `jobs` (source, destination, rows, 0).
-int copy_pages(Ctx* ctx, const std::vector<int4>& jobs, cudaStream_t st) {
+// Enqueues the page copies `jobs` (source, destination, rows, 0) from a slot that has room for them.
+int copy_pages(Ctx* ctx, const std::vector<int4>& jobs, Ctx::Slot* s, cudaStream_t st) {
   if (jobs.empty()) return L3P_OK;
-  Ctx::Slot* s;
-  if (int rc = take_slot(ctx, jobs.size() * 4, &s)) return rc;
   memcpy(s->host, jobs.data(), jobs.size() * sizeof(int4));
   if (int rc = upload(ctx, s, ctx->jobs, jobs.size() * 4, st)) return rc;
   return launch_page_copy(ctx, ctx->jobs, (int)jobs.size(), st);
@@ -372,19 +374,16 @@ void plan_tc(Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, std::vector<Pg
   });
 }
 
-// Lays the current batch out as the kernels read it, in a pinned slot, with the page copies behind it (*jobs_at: their
-// word offset).  The lists are the context's, so that a step allocates nothing.
-int build_batch(Ctx* ctx, const std::vector<BatchSeq>& bs, const int* seqs, int n_seqs, int n_tokens,
-                const std::vector<int4>& jobs, Ctx::Slot** out, size_t* words, size_t* jobs_at) {
+// Plans a batch: the lists of the kernels (the context's vectors, so that a step allocates nothing), the header, the words of
+// the description, and where in it the n_jobs page copies are.  Reads lengths and page counts from bs, not the books.
+int plan_batch(Ctx* ctx, const std::vector<BatchSeq>& bs, int n_tokens, size_t tbl_words, size_t n_jobs, PgHeader* out, size_t* words,
+               size_t* jobs_at) {
   PgHeader h{};
   h.n_tokens = n_tokens;
-  h.n_seqs = n_seqs;
+  h.n_seqs = (int)bs.size();
   int max_rows = 0;
-  size_t tbl_words = 0;
-  for (int i = 0; i < n_seqs; ++i) {
-    if (!bs[i].tc) max_rows = std::max(max_rows, bs[i].n_new * ctx->G);
-    tbl_words += ctx->seqs[seqs[i]].pages.size();
-  }
+  for (const auto& b : bs)
+    if (!b.tc) max_rows = std::max(max_rows, b.n_new * ctx->G);
   h.row_nt = std::min(max_rows <= 8 ? 1 : 2, row_max_nt(ctx));
   size_t at = kPgHdrWords;
   auto place = [&](size_t bytes) {
@@ -412,16 +411,22 @@ int build_batch(Ctx* ctx, const std::vector<BatchSeq>& bs, const int* seqs, int 
   }
   h.tok = (int)place((size_t)n_tokens * sizeof(int2));
   h.tbl = (int)place(tbl_words * 4);
-  *jobs_at = place(jobs.size() * sizeof(int4));
+  *jobs_at = place(n_jobs * sizeof(int4));
   if (at > ctx->batch_words) return fail(ctx, L3P_E_RANGE, "batch description of %zu words", at);
-  if (int rc = take_slot(ctx, at, out)) return rc;
-  int* w = (*out)->host;
+  *out = h;
+  *words = at;
+  return L3P_OK;
+}
+
+// Writes the planned batch to `w`, its tables and token rows from the books.
+void write_batch(const Ctx* ctx, const PgHeader& h, const std::vector<BatchSeq>& bs, const int* seqs, const std::vector<int4>& jobs,
+                 size_t jobs_at, int* w) {
   auto put = [&](size_t where, const void* p, size_t bytes) {
     if (bytes) memcpy(w + where, p, bytes);
   };
   memset(w, 0, kPgHdrWords * 4);
   memcpy(w, &h, sizeof h);
-  for (int v = 0; v < n_lists; ++v) {
+  for (int v = 0; v < (ctx->swa ? 2 : 1); ++v) {
     const auto& p = ctx->plan[v];
     const PgLists& l = h.lists[v];
     put(l.row_first, p.first.data(), p.first.size() * 4);
@@ -431,7 +436,7 @@ int build_batch(Ctx* ctx, const std::vector<BatchSeq>& bs, const int* seqs, int 
     put(l.prep, p.prep.data(), p.prep.size() * sizeof(PgPrep));
   }
   int* tbl = w + h.tbl;
-  for (int i = 0; i < n_seqs; ++i) {
+  for (size_t i = 0; i < bs.size(); ++i) {
     const auto& s = ctx->seqs[seqs[i]];
     const auto& b = bs[i];
     for (int t = 0; t < b.n_new; ++t) {
@@ -443,13 +448,10 @@ int build_batch(Ctx* ctx, const std::vector<BatchSeq>& bs, const int* seqs, int 
     put(tbl - w, s.pages.data(), s.pages.size() * 4);
     tbl += s.pages.size();
   }
-  put(*jobs_at, jobs.data(), jobs.size() * sizeof(int4));
-  ctx->hdr = h;
-  *words = at;
-  return L3P_OK;
+  put(jobs_at, jobs.data(), jobs.size() * sizeof(int4));
 }
 
-// Words of the largest batch block: bounds on what build_batch lays out.
+// Words of the largest batch block: bounds on what plan_batch lays out.
 size_t batch_capacity(const Ctx* ctx) {
   const auto& c = ctx->cfg;
   const size_t max_len = c.max_seq_len, rows = (size_t)c.max_tokens * ctx->G, kv = c.n_kv_heads, seqs = c.max_seqs;
@@ -544,6 +546,7 @@ int create(const l3p_paged_config& in, Ctx** out) {
   PG_CUDA(ctx, cudaHostAlloc(&ctx->err_host, sizeof(int), cudaHostAllocMapped));
   *ctx->err_host = 0;
   PG_CUDA(ctx, cudaHostGetDevicePointer(&ctx->err_dev, ctx->err_host, 0));
+  for (auto& s : ctx->slots) PG_CUDA(ctx, cudaEventCreateWithFlags(&s.done, cudaEventDisableTiming));
   ctx->seqs.resize(c.max_seqs);
   ctx->refs.assign(c.n_pages, 0);
   ctx->fill.assign(c.n_pages, 0);
@@ -594,13 +597,30 @@ int begin(Ctx* ctx, int n_seqs, const int* ids, const int* n_new, cudaStream_t s
     return fail(ctx, L3P_E_NOMEM, "the batch needs %lld pages, %zu are free", need, ctx->free_heap.size());
   if (int rc = refuse_capture(ctx, s, "begin")) return rc;
 
-  // all checks passed: give out pages.  In batch order, a sequence's copy first.
-  ctx->batch_valid = false;
+  // Everything that may find no memory comes before the books move: the plan, a slot for it, room in the lists.
   std::vector<int4> jobs;
+  jobs.reserve(cow.size());
   std::vector<BatchSeq> bs(n_seqs);
+  int row = 0, tbl = 0, max_pos = 0;
+  for (int i = 0; i < n_seqs; ++i) {
+    auto& q = ctx->seqs[ids[i]];
+    const int len = q.len + n_new[i], n_pages = pages_for(ctx, len);
+    reserve_pages(&q.pages, n_pages);
+    bs[i] = {row, n_new[i], len, tbl, false};
+    row += n_new[i];
+    if (n_new[i] > 0) max_pos = std::max(max_pos, len);
+    tbl += n_pages;
+  }
+  choose_paths(ctx, &bs);
+  PgHeader hdr;
+  size_t words, jobs_at;
+  if (int rc = plan_batch(ctx, bs, row, tbl, cow.size(), &hdr, &words, &jobs_at)) return rc;
+  Ctx::Slot* slot;
+  if (int rc = take_slot(ctx, words, &slot)) return rc;
+
+  // Give out pages, in batch order, a sequence's copy first.
+  ctx->batch_valid = false;
   size_t next = 0;
-  int row = 0, tbl = 0;
-  ctx->max_pos_in_batch = 0;
   for (int i = 0; i < n_seqs; ++i) {
     auto& q = ctx->seqs[ids[i]];
     if (next < cow.size() && cow[next].first == i) {
@@ -611,22 +631,17 @@ int begin(Ctx* ctx, int n_seqs, const int* ids, const int* n_new, cudaStream_t s
       q.pages.back() = dst;
       ++next;
     }
-    const int len = q.len + n_new[i], n_pages = pages_for(ctx, len);
+    const int len = bs[i].len, n_pages = pages_for(ctx, len);
     while ((int)q.pages.size() < n_pages) q.pages.push_back(take_page(ctx));
     for (int pos = q.len; pos < len; pos = (pos | (ctx->cfg.page_size - 1)) + 1) {
       const int p = q.pages[pos >> ctx->shift];
       ctx->fill[p] = std::max(ctx->fill[p], std::min(ctx->cfg.page_size, len - (pos & ~(ctx->cfg.page_size - 1))));
     }
     q.len = len;
-    bs[i] = {row, n_new[i], len, tbl, false};
-    row += n_new[i];
-    if (n_new[i] > 0) ctx->max_pos_in_batch = std::max(ctx->max_pos_in_batch, len);
-    tbl += (int)q.pages.size();
   }
-  choose_paths(ctx, &bs);
-  Ctx::Slot* slot;
-  size_t words, jobs_at;
-  if (int rc = build_batch(ctx, bs, ids, n_seqs, row, jobs, &slot, &words, &jobs_at)) return rc;
+  ctx->hdr = hdr;
+  ctx->max_pos_in_batch = max_pos;
+  write_batch(ctx, hdr, bs, ids, jobs, jobs_at, slot->host);
   if (int rc = upload(ctx, slot, ctx->batch, words, s)) return rc;
   if (!jobs.empty())
     if (int rc = launch_page_copy(ctx, ctx->batch + jobs_at, (int)jobs.size(), s)) return rc;
@@ -644,13 +659,20 @@ int copy_seqs(Ctx* ctx, int n, const int* ids, int* children, cudaStream_t s) {
   if (need > (long long)ctx->free_heap.size())
     return fail(ctx, L3P_E_NOMEM, "the copies need %lld pages, %zu are free", need, ctx->free_heap.size());
   if (int rc = refuse_capture(ctx, s, "copy")) return rc;
+  // everything that may find no memory comes before the books move
   std::vector<int4> jobs;
   jobs.reserve(need);
+  std::vector<std::vector<int>> pages(n);
+  for (int i = 0; i < n; ++i) pages[i].reserve(ctx->seqs[ids[i]].pages.size());
+  Ctx::Slot* slot = nullptr;
+  if (need > 0)
+    if (int rc = take_slot(ctx, need * 4, &slot)) return rc;
   for (int i = 0; i < n; ++i) {
     const int child = new_seq(ctx);
     auto& dst = ctx->seqs[child];
     const auto& src = ctx->seqs[ids[i]];
     dst.len = src.len;
+    dst.pages.swap(pages[i]);
     for (size_t k = 0; k < src.pages.size(); ++k) {
       const int p = take_page(ctx), rows = std::min(ctx->cfg.page_size, src.len - (int)k * ctx->cfg.page_size);
       ctx->fill[p] = rows;
@@ -659,13 +681,14 @@ int copy_seqs(Ctx* ctx, int n, const int* ids, int* children, cudaStream_t s) {
     }
     children[i] = child;
   }
-  return copy_pages(ctx, jobs, s);
+  return copy_pages(ctx, jobs, slot, s);
 }
 
 int compact(Ctx* ctx, int* n_used, cudaStream_t s) {
   if (int rc = refuse_capture(ctx, s, "compact")) return rc;
   const int k = ctx->cfg.n_pages - (int)ctx->free_heap.size();
   std::vector<int4> jobs;
+  jobs.reserve(ctx->cfg.n_pages - k);
   std::vector<int> moved(ctx->cfg.n_pages, -1);
   int dst = 0;
   for (int p = k; p < ctx->cfg.n_pages; ++p) {
@@ -676,8 +699,10 @@ int compact(Ctx* ctx, int* n_used, cudaStream_t s) {
     ++dst;
   }
   if (!jobs.empty()) {
+    Ctx::Slot* slot;
+    if (int rc = take_slot(ctx, jobs.size() * 4, &slot)) return rc;
     ctx->batch_valid = false;
-    if (int rc = copy_pages(ctx, jobs, s)) return rc;
+    if (int rc = copy_pages(ctx, jobs, slot, s)) return rc;
     for (const auto& j : jobs) {
       ctx->refs[j.y] = ctx->refs[j.x];
       ctx->fill[j.y] = ctx->fill[j.x];
@@ -762,12 +787,14 @@ L3P_API int l3p_paged_seq_fork(l3p_paged_ctx* ctx, int seq, int n_tokens, int n,
     if (n > free_seq_count(ctx))
       return fail(ctx, L3P_E_NOMEM, "%d sequences more than max_seqs = %d allows", n, ctx->cfg.max_seqs);
     const int n_pages = pages_for(ctx, len);
-    const std::vector<int> pages(ctx->seqs[seq].pages.begin(), ctx->seqs[seq].pages.begin() + n_pages);
+    const auto& shared = ctx->seqs[seq].pages;
+    std::vector<std::vector<int>> pages(n);  // before the books move
+    for (auto& p : pages) p.assign(shared.begin(), shared.begin() + n_pages);
     for (int i = 0; i < n; ++i) {
       const int id = new_seq(ctx);
-      ctx->seqs[id].pages = pages;
+      ctx->seqs[id].pages.swap(pages[i]);
       ctx->seqs[id].len = len;
-      for (int p : pages) ++ctx->refs[p];
+      for (int p : ctx->seqs[id].pages) ++ctx->refs[p];
       children[i] = id;
     }
     return L3P_OK;

@@ -1,0 +1,27 @@
+"""The paged cache's books without a GPU (tests/host/paged_books.cpp): calls that
+find no memory, pinned or ordinary, change nothing."""
+import os
+import subprocess
+
+import pytest
+
+from conftest import ROOT
+from llama3pure_b200.build import ARCH_FLAGS, CSRC, INCLUDE, nvcc
+
+
+@pytest.fixture(scope="module")
+def books(tmp_path_factory):
+    exe = str(tmp_path_factory.mktemp("books") / "paged_books")
+    subprocess.run([nvcc(), *ARCH_FLAGS, "-O1", "-std=c++17", "-cudart", "none", "-I", INCLUDE, "-I", CSRC, "-o", exe,
+                    os.path.join(ROOT, "tests", "host", "paged_books.cpp"), os.path.join(CSRC, "l3p_paged.cu")], check=True)
+
+    def run(*args):
+        r = subprocess.run([exe, *args], capture_output=True, text=True, timeout=120)
+        assert r.returncode == 0, r.stdout + r.stderr
+
+    return run
+
+
+@pytest.mark.parametrize("call", ["begin", "copy", "fork", "compact"])
+def test_a_call_without_memory_changes_nothing(books, call):
+    books(call)
