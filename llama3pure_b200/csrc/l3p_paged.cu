@@ -745,7 +745,7 @@ L3P_API void l3p_paged_destroy(l3p_paged_ctx* ctx) {
   delete ctx;
 }
 
-L3P_API const char* l3p_paged_last_error(const l3p_paged_ctx* ctx) { return ctx ? ctx->last_error.c_str() : ""; }
+L3P_API const char* l3p_paged_last_error(const l3p_paged_ctx* ctx) { return ctx ? ctx->last_error : ""; }
 
 L3P_API long long l3p_paged_launch_count(const l3p_paged_ctx* ctx) { return ctx ? ctx->launches : L3P_E_INVAL; }
 

@@ -7,7 +7,6 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
-#include <string>
 #include <vector>
 
 #include "llama3pure_paged.h"
@@ -159,7 +158,7 @@ struct l3p_paged_ctx {
   int* err_host = nullptr;
   int* err_dev = nullptr;
   long long launches = 0;
-  std::string last_error;
+  char last_error[512] = "";  // written without an allocation: a refusal may be for want of memory
 };
 
 namespace l3p_pg {
@@ -173,14 +172,12 @@ inline void retire(l3p_paged_ctx* ctx, void* p, bool captured) {
     cudaFree(p);
 }
 
-inline int fail(l3p_paged_ctx* ctx, int code, const char* fmt, ...) {
+inline int fail(l3p_paged_ctx* ctx, int code, const char* fmt, ...) noexcept {
   if (ctx) {
-    char buf[512];
     va_list ap;
     va_start(ap, fmt);
-    vsnprintf(buf, sizeof buf, fmt, ap);
+    vsnprintf(ctx->last_error, sizeof ctx->last_error, fmt, ap);
     va_end(ap);
-    ctx->last_error = buf;
   }
   return code;
 }

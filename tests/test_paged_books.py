@@ -25,3 +25,9 @@ def books(tmp_path_factory):
 @pytest.mark.parametrize("call", ["begin", "copy", "fork", "compact"])
 def test_a_call_without_memory_changes_nothing(books, call):
     books(call)
+
+
+@pytest.mark.parametrize("call", ["begin", "copy", "fork", "compact"])
+def test_no_exception_leaves_a_call_when_memory_is_exhausted(books, call):
+    """Every allocation after the failing one fails too."""
+    books(call, "rest")
