@@ -163,6 +163,18 @@ __device__ __forceinline__ void pg_commit_g(uint32_t leader, uint32_t bar_cluste
         : "memory");
 }
 
+// The two softmax warpgroups meet: whether `ok` holds in all of their threads.  A warp whose bounded wait gave up must not
+// leave a loop in which the others meet it at a barrier, which has no bound: all of them leave on the same tile.
+__device__ __forceinline__ bool pg_meet(bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"((uint32_t)ok)
+      : "memory");
+  return all != 0;
+}
+
 template <int CG, int HD>
 __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
   using C = PfCfg<CG, HD>;
@@ -461,12 +473,11 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
     float m = -INFINITY, lsum = 0.f;
     bool ok = true;
     for (int j = 0; j < nt; ++j) {
-      ok = __all_sync(0xffffffffu, wait(&bar_s_full, (uint32_t)(j & 1)));
+      ok = ok && __all_sync(0xffffffffu, wait(&bar_s_full, (uint32_t)(j & 1)));
       tc::fence_after_sync();
       if (!any_row) {  // lanes without a row: S, P and O as they come (MMA rows are independent)
-        if (lane == 0) arrive_issuer(&bar_s_free);
-        asm volatile("bar.sync 2, 256;" ::: "memory");
-        if (!ok) break;
+        if (lane == 0 && ok) arrive_issuer(&bar_s_free);
+        if (!(ok = pg_meet(ok))) break;
         if (half == 0 && lane == 0) mbar_arrive(&bar_alpha[j & 1]);
         for (int qq = 0; qq < 2; ++qq) {
           if (j >= 1 || half > 0) ok = ok && __all_sync(0xffffffffu, wait(&bar_p_free[half ^ 1][qq], (uint32_t)((half ? j : j - 1) & 1)));
@@ -485,7 +496,7 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
       tc::wait_ld();
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) arrive_issuer(&bar_s_free);
+      if (lane == 0 && ok) arrive_issuer(&bar_s_free);
       const int key0 = (u.tile0 + j) * kPfBN + half * 64;
       if (!__all_sync(0xffffffffu, key0 >= kmin && key0 + 63 <= qpos)) {
         const int last = qpos - key0, from = kmin - key0;
@@ -503,8 +514,7 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
       for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], sv[60 + i]);
       s_max[j & 1][half][row] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       // both halves of a row meet here once a tile, whether their waits succeeded or not
-      asm volatile("bar.sync 2, 256;" ::: "memory");
-      if (!ok) break;
+      if (!(ok = pg_meet(ok))) break;
       const float m_new = fmaxf(m, fmaxf(s_max[j & 1][0][row], s_max[j & 1][1][row]) * a.scale_log2);
       const float base = m_new == -INFINITY ? 0.f : m_new;
       const float alpha = fast_exp2(m - base);
@@ -529,7 +539,7 @@ __global__ void __launch_bounds__(512, 1) paged_f32_kernel(const PgF32Args a) {
         if (j >= 1 || half > 0) {
           // the slot's quarter before, the other half's, has been multiplied (a barrier for each half: of one that both
           // halves' quarters complete, a warpgroup could be two phases behind)
-          ok = __all_sync(0xffffffffu, wait(&bar_p_free[half ^ 1][qq], (uint32_t)((half ? j : j - 1) & 1)));
+          ok = ok && __all_sync(0xffffffffu, wait(&bar_p_free[half ^ 1][qq], (uint32_t)((half ? j : j - 1) & 1)));
           tc::fence_after_sync();
         }
         tc::st32(T_P + lb + qq * 64, ph);

@@ -1,10 +1,13 @@
 """The paged cache's C ABI without a GPU: bad configurations are refused
 before the device is touched, and null arguments are errors."""
 import ctypes as C
+import os
+import re
 
 import pytest
 
 from llama3pure_b200 import attn
+from llama3pure_b200.build import CSRC
 
 
 def _cfg(**kw):
@@ -63,3 +66,15 @@ def test_null_arguments_are_errors(lib):
     assert lib.l3p_paged_launch_count(None) == -1
     assert lib.l3p_paged_last_error(None) == b""
     lib.l3p_paged_destroy(None)
+
+
+def test_warps_meet_with_the_outcome_of_their_waits():
+    """The loop over key tiles of the fp32 chunk kernel has a barrier that some of a CTA's warps meet at.  A warp's bounded wait
+    may give up where another's does not, so the barrier has to tell all of them: one that only counts threads would be waited
+    for without a bound by the warps that go on."""
+    with open(os.path.join(CSRC, "paged_f32.cuh")) as f:
+        code = re.sub(r"//[^\n]*", "", f.read())
+    assert not re.findall(r"bar(?:rier)?(?:\.cta)?\.sync", code)
+    assert len(re.findall(r"bar\.red\.and\.pred", code)) == 1
+    meets = re.findall(r"[^\n]*pg_meet\(ok\)[^\n]*", code)
+    assert len(meets) == 2 and all(re.search(r"if \(!\(ok = pg_meet\(ok\)\)\) break;", m) for m in meets)
