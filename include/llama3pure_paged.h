@@ -73,6 +73,8 @@ typedef struct l3p_paged_config {
 typedef struct l3p_paged_ctx l3p_paged_ctx;
 
 int l3p_paged_create(const l3p_paged_config* cfg, l3p_paged_ctx** out);
+/* Why the last l3p_paged_create of the calling thread failed ("" after one that did not). */
+const char* l3p_paged_create_error(void);
 void l3p_paged_destroy(l3p_paged_ctx* ctx);
 const char* l3p_paged_last_error(const l3p_paged_ctx* ctx);
 /* Waits for `stream` and reports what its kernels recorded, clearing it:

@@ -75,6 +75,7 @@ EXPORTS = (
     "l3p_attn_decode_noalloc",
     "l3p_attn_noalloc_last_error",
     "l3p_paged_create",
+    "l3p_paged_create_error",
     "l3p_paged_destroy",
     "l3p_paged_last_error",
     "l3p_paged_check",
@@ -235,6 +236,7 @@ def load_library(path: str = LIB_PATH):
         "l3p_attn_decode_noalloc": (i, [C.POINTER(AttnConfig), i, i, fp, fp, fp, fp, vp]),
         "l3p_attn_noalloc_last_error": (C.c_char_p, []),
         "l3p_paged_create": (i, [C.POINTER(PagedConfig), C.POINTER(C.c_void_p)]),
+        "l3p_paged_create_error": (C.c_char_p, []),
         "l3p_paged_destroy": (None, [vp]),
         "l3p_paged_last_error": (C.c_char_p, [vp]),
         "l3p_paged_check": (i, [vp, vp]),

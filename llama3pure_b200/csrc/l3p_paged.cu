@@ -501,20 +501,35 @@ int guarded(Ctx* ctx, F f) {
   }
 }
 
+// Why the last create of this thread failed: its context is gone by then.
+thread_local char g_create_error[512] = "";
+
+int refuse(int code, const char* text) {
+  snprintf(g_create_error, sizeof g_create_error, "%s", text);
+  return code;
+}
+
 int create(const l3p_paged_config& in, Ctx** out) {
   l3p_paged_config c = in;
-  if (c.n_layers <= 0 || c.n_heads <= 0 || c.n_kv_heads <= 0 || c.n_heads % c.n_kv_heads != 0) return L3P_E_INVAL;
-  if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return L3P_E_UNSUPPORTED;
-  if (c.page_size != 16 && c.page_size != 32 && c.page_size != 64 && c.page_size != 128) return L3P_E_UNSUPPORTED;
-  if (c.n_pages <= 0 || c.max_seqs <= 0 || c.max_tokens <= 0 || c.max_seq_len < 0) return L3P_E_INVAL;
-  if (c.dtype != L3P_PAGED_F32 && c.dtype != L3P_PAGED_BF16) return L3P_E_INVAL;
-  if (!std::isfinite(c.scale) || c.scale < 0.f || c.swa_window < 0 || c.swa_pattern < 0 || c.device < 0) return L3P_E_INVAL;
+  if (c.n_layers <= 0 || c.n_heads <= 0 || c.n_kv_heads <= 0) return refuse(L3P_E_INVAL, "n_layers, n_heads and n_kv_heads are positive");
+  if (c.n_heads % c.n_kv_heads != 0) return refuse(L3P_E_INVAL, "n_heads is a multiple of n_kv_heads");
+  if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return refuse(L3P_E_UNSUPPORTED, "head_dim is 64, 128 or 256");
+  if (c.page_size != 16 && c.page_size != 32 && c.page_size != 64 && c.page_size != 128)
+    return refuse(L3P_E_UNSUPPORTED, "page_size is 16, 32, 64 or 128");
+  if (c.n_pages <= 0 || c.max_seqs <= 0 || c.max_tokens <= 0 || c.max_seq_len < 0)
+    return refuse(L3P_E_INVAL, "n_pages, max_seqs and max_tokens are positive, max_seq_len is not negative");
+  if (c.dtype != L3P_PAGED_F32 && c.dtype != L3P_PAGED_BF16) return refuse(L3P_E_INVAL, "dtype is L3P_PAGED_F32 or L3P_PAGED_BF16");
+  if (!std::isfinite(c.scale) || c.scale < 0.f) return refuse(L3P_E_INVAL, "scale is finite and not negative");
+  if (c.swa_window < 0 || c.swa_pattern < 0 || c.device < 0)
+    return refuse(L3P_E_INVAL, "swa_window, swa_pattern and device are not negative");
   // positions, storage rows and query rows are counted in 32 bits
   const long long pool_pos = (long long)c.n_pages * c.page_size;
-  if (pool_pos > INT_MAX / 2 || c.max_seqs > 65536) return L3P_E_RANGE;
+  if (pool_pos > INT_MAX / 2) return refuse(L3P_E_RANGE, "the pool has more than 2^30 positions");
+  if (c.max_seqs > 65536) return refuse(L3P_E_RANGE, "max_seqs is above 65536");
   if (c.max_seq_len == 0 || c.max_seq_len > pool_pos) c.max_seq_len = (int)pool_pos;
-  if ((long long)c.max_tokens * c.n_heads > INT_MAX / 2) return L3P_E_RANGE;
-  if (pool_pos * c.n_layers * 2 * c.n_kv_heads > INT_MAX) return L3P_E_RANGE;  // rows of the tensor map
+  if ((long long)c.max_tokens * c.n_heads > INT_MAX / 2) return refuse(L3P_E_RANGE, "max_tokens * n_heads is above 2^30");
+  if (pool_pos * c.n_layers * 2 * c.n_kv_heads > INT_MAX)  // rows of the tensor map
+    return refuse(L3P_E_RANGE, "the pool has more than 2^31 rows");
   Ctx* ctx = new Ctx;
   ctx->cfg = c;
   ctx->hd = c.head_dim;
@@ -720,12 +735,17 @@ int compact(Ctx* ctx, int* n_used, cudaStream_t s) {
 
 }  // namespace
 
+L3P_API const char* l3p_paged_create_error(void) { return g_create_error; }
+
 L3P_API int l3p_paged_create(const l3p_paged_config* cfg, l3p_paged_ctx** out) {
-  if (!cfg || !out) return L3P_E_INVAL;
+  if (!cfg || !out) return refuse(L3P_E_INVAL, "null pointer");
   *out = nullptr;
+  g_create_error[0] = 0;
   Ctx* ctx = nullptr;
   const int rc = guarded(nullptr, [&] { return create(*cfg, &ctx); });
   if (rc != L3P_OK) {
+    if (ctx && ctx->last_error[0]) refuse(rc, ctx->last_error);
+    if (!g_create_error[0]) refuse(rc, "host memory is exhausted");
     if (ctx) {
       DeviceScope dev(ctx->cfg.device);
       release(ctx);

@@ -59,7 +59,7 @@ class PagedCache:
         h = C.c_void_p()
         rc = self.lib.l3p_paged_create(C.byref(self.cfg), C.byref(h))
         if rc != L3P_OK:
-            raise AttnError(rc, "l3p_paged_create failed")
+            raise AttnError(rc, f"create: {self.lib.l3p_paged_create_error().decode()}")
         self.h = h
 
     @classmethod

@@ -215,11 +215,34 @@ static int compact_call(l3p_paged_ctx* ctx, const int*) {
   return l3p_paged_compact(ctx, &used, nullptr);
 }
 
+// Every allocation of create fails in turn: it returns L3P_E_NOMEM, says why, and leaves no context.
+static void create_everywhere(int dtype) {
+  l3p_paged_config c{};
+  c.n_layers = 1, c.n_heads = 8, c.n_kv_heads = 2, c.head_dim = 64, c.page_size = 16, c.n_pages = kPages;
+  c.max_seqs = kSeqs, c.max_tokens = 4000, c.dtype = dtype;
+  int refused = 0;
+  for (long at = 0, reached = 1; reached; ++at) {
+    l3p_paged_ctx* ctx = nullptr;
+    g_watch = true, g_fail_in = at;
+    const int rc = l3p_paged_create(&c, &ctx);
+    g_watch = false;
+    reached = g_fail_in < 0;
+    g_fail_in = -1;
+    EXPECT((rc == L3P_OK) == (l3p_paged_create_error()[0] == 0) && (rc == L3P_OK) == (ctx != nullptr));
+    EXPECT(reached ? rc == L3P_E_NOMEM || rc == L3P_E_CUDA : rc == L3P_OK);
+    refused += rc != L3P_OK;
+    l3p_paged_destroy(ctx);
+  }
+  EXPECT(refused > 5);
+}
+
 int main(int argc, char** argv) {
   const std::string test = argc > 1 ? argv[1] : "";
   g_fail_rest = argc > 2 && std::string(argv[2]) == "rest";
   for (int dtype : {L3P_PAGED_F32, L3P_PAGED_BF16}) {
-    if (test == "begin") {
+    if (test == "create") {
+      create_everywhere(dtype);
+    } else if (test == "begin") {
       fail_everywhere("begin", dtype, begin_call);
     } else if (test == "copy") {
       fail_everywhere("copy", dtype, copy_call);

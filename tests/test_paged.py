@@ -78,3 +78,26 @@ def test_warps_meet_with_the_outcome_of_their_waits():
     assert len(re.findall(r"bar\.red\.and\.pred", code)) == 1
     meets = re.findall(r"[^\n]*pg_meet\(ok\)[^\n]*", code)
     assert len(meets) == 2 and all(re.search(r"if \(!\(ok = pg_meet\(ok\)\)\) break;", m) for m in meets)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(n_heads=6, n_kv_heads=4), "n_heads"),
+    (dict(head_dim=96), "head_dim"),
+    (dict(page_size=24), "page_size"),
+    (dict(dtype=2), "dtype"),
+    (dict(scale=-0.1), "scale"),
+    (dict(n_pages=2**30), "positions"),
+    (dict(max_seqs=2**20), "max_seqs"),
+    (dict(max_tokens=2**30), "max_tokens"),
+    (dict(n_pages=2**20, n_layers=2**10), "rows"),
+])
+def test_a_refused_create_says_why(lib, kw, text):
+    from llama3pure_b200.paged import PagedCache
+
+    h = C.c_void_p()
+    assert lib.l3p_paged_create(C.byref(_cfg(**kw)), C.byref(h)) < 0
+    assert text in lib.l3p_paged_create_error().decode()
+    base = dict(n_layers=2, n_heads=8, n_kv_heads=2, head_dim=128, page_size=16, n_pages=8, max_seqs=4, max_tokens=64) | kw
+    if base.get("dtype", "f32") == "f32":  # the binding refuses names of types by itself
+        with pytest.raises(attn.AttnError, match=text):
+            PagedCache(**base, lib=lib)

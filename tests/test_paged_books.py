@@ -31,3 +31,8 @@ def test_a_call_without_memory_changes_nothing(books, call):
 def test_no_exception_leaves_a_call_when_memory_is_exhausted(books, call):
     """Every allocation after the failing one fails too."""
     books(call, "rest")
+
+
+def test_create_without_memory_says_why(books):
+    books("create")
+    books("create", "rest")
