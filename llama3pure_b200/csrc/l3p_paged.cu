@@ -528,7 +528,8 @@ int create(const l3p_paged_config& in, Ctx** out) {
   if (c.max_seqs > 65536) return refuse(L3P_E_RANGE, "max_seqs is above 65536");
   if (c.max_seq_len == 0 || c.max_seq_len > pool_pos) c.max_seq_len = (int)pool_pos;
   if ((long long)c.max_tokens * c.n_heads > INT_MAX / 2) return refuse(L3P_E_RANGE, "max_tokens * n_heads is above 2^30");
-  if (pool_pos * c.n_layers * 2 * c.n_kv_heads > INT_MAX)  // rows of the tensor map
+  // rows of the tensor map; by division, since the product may pass 64 bits
+  if (c.n_layers > INT_MAX / pool_pos || c.n_kv_heads > INT_MAX / (2 * pool_pos * c.n_layers))
     return refuse(L3P_E_RANGE, "the pool has more than 2^31 rows");
   Ctx* ctx = new Ctx;
   ctx->cfg = c;

@@ -101,3 +101,14 @@ def test_a_refused_create_says_why(lib, kw, text):
     if base.get("dtype", "f32") == "f32":  # the binding refuses names of types by itself
         with pytest.raises(attn.AttnError, match=text):
             PagedCache(**base, lib=lib)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(n_pages=2**20, n_layers=2**30, n_heads=2**9, n_kv_heads=2**9, max_tokens=1),  # 2^64 rows: 0 in 64 bits
+    dict(n_pages=2**26, n_layers=2**22, n_heads=2**12, n_kv_heads=2**12, max_tokens=1),  # 2^65
+    dict(n_pages=2**22, n_layers=2**30 + 1, n_heads=2**12, n_kv_heads=2**12, max_tokens=1),
+])
+def test_sizes_whose_product_passes_64_bits_are_refused(lib, kw):
+    h = C.c_void_p()
+    assert lib.l3p_paged_create(C.byref(_cfg(**kw)), C.byref(h)) == -2
+    assert not h.value
