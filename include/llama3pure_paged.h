@@ -169,8 +169,7 @@ int l3p_paged_append_dev(l3p_paged_ctx* ctx, int layer, const void* k, long long
  * with n_new * n_heads / n_kv_heads query rows per KV head, the largest count
  * of a batch of few tokens is at most 8, or 9 to 16 (F32 pools: 9 to 64, with
  * head_dim 256 9 and more).  A replay on a batch that does not fit writes
- * nothing for it and l3p_paged_check reports L3P_E_INVAL.  An F32 chunk may need a workspace that
- * cannot grow during capture: make one call of the size before. */
+ * nothing for it and l3p_paged_check reports L3P_E_INVAL. */
 int l3p_paged_attn_dev(l3p_paged_ctx* ctx, int layer, const void* q, long long q_stride, void* out,
                        long long out_stride, void* stream);
 

@@ -633,6 +633,7 @@ int begin(Ctx* ctx, int n_seqs, const int* ids, const int* n_new, cudaStream_t s
   if (int rc = plan_batch(ctx, bs, row, tbl, cow.size(), &hdr, &words, &jobs_at)) return rc;
   Ctx::Slot* slot;
   if (int rc = take_slot(ctx, words, &slot)) return rc;
+  if (int rc = prepare_f32(ctx, hdr)) return rc;
 
   // Give out pages, in batch order, a sequence's copy first.
   ctx->batch_valid = false;

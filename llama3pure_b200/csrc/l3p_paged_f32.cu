@@ -9,7 +9,7 @@ using namespace l3p;
 
 namespace l3p_pg {
 
-// Images of more than this are made for some KV heads at a time.
+// Images of more than this are made for some KV heads at a time, at least one: its images are twice its K and V.
 static constexpr size_t kImageBytes = 1ull << 30;
 
 int f32_rows(const l3p_paged_ctx* ctx) { return ctx->hd == 64 ? 128 : 256; }
@@ -29,37 +29,48 @@ int init_f32(l3p_paged_ctx* ctx) {
   return L3P_OK;
 }
 
-// Makes the image buffer hold `floats` and the flags `n`.
-static int ensure_images(l3p_paged_ctx* ctx, size_t floats, size_t n, cudaStream_t s) {
-  if (floats <= ctx->img_floats && n <= ctx->v_flags_n) return L3P_OK;
-  if (capturing(s))
-    return fail(ctx, L3P_E_INVAL, "the fp32 chunk's workspace must grow to %zu bytes, which cannot happen during stream capture: "
-                "make one call of this size before capturing", floats * sizeof(float));
-  PG_CUDA(ctx, cudaStreamSynchronize(s));
+static size_t tile_floats(const l3p_paged_ctx* ctx) { return ctx->hd == 64 ? PfGeom<64>::kTileFloats : PfGeom<128>::kTileFloats; }
+
+// KV heads whose images of n_prep tiles are made at a time.
+static int image_heads(const l3p_paged_ctx* ctx, int n_prep) {
+  const size_t fit = std::max<size_t>(1, kImageBytes / (tile_floats(ctx) * sizeof(float) * n_prep));
+  return (int)std::min<size_t>(fit, ctx->cfg.n_kv_heads);
+}
+
+// The image buffer for a batch, as part of begin: attention then has nothing to allocate, in a capture or out of it.  It grows
+// by half at least, since a prompt fed in chunks needs a little more at every step.
+int prepare_f32(l3p_paged_ctx* ctx, const PgHeader& h) {
+  size_t tiles = 0;  // of all heads at a time
+  for (const PgLists& l : h.lists)
+    if (l.n_prep > 0) tiles = std::max(tiles, (size_t)l.n_prep * image_heads(ctx, l.n_prep));
+  if (tiles <= ctx->img_tiles) return L3P_OK;
+  const size_t tile = tile_floats(ctx) * sizeof(float);
+  ctx->retired.reserve(ctx->retired.size() + 2);
+  float* img = nullptr;
+  int* flags = nullptr;
+  size_t want = std::max(tiles, ctx->img_tiles + ctx->img_tiles / 2);
+  auto get = [&] {
+    if (cudaMalloc(&img, want * tile) == cudaSuccess && cudaMalloc(&flags, want * 4 * sizeof(int)) == cudaSuccess) return true;
+    cudaGetLastError();
+    cudaFree(img);
+    img = nullptr;
+    return false;
+  };
+  if (!get() && (want == tiles || (want = tiles, !get())))
+    return fail(ctx, L3P_E_NOMEM, "the fp32 chunks' workspace of %zu bytes does not fit on the device", want * tile);
+  if (ctx->img) PG_CUDA(ctx, cudaDeviceSynchronize());  // earlier calls' kernels read the old ones
   retire(ctx, ctx->img, ctx->img_captured);
   retire(ctx, ctx->v_flags, ctx->img_captured);
   ctx->img_captured = false;
-  ctx->img = nullptr;
-  ctx->v_flags = nullptr;
-  ctx->img_floats = ctx->v_flags_n = 0;
-  if (cudaMalloc(&ctx->img, floats * sizeof(float)) != cudaSuccess || cudaMalloc(&ctx->v_flags, n * sizeof(int)) != cudaSuccess) {
-    cudaGetLastError();
-    cudaFree(ctx->img);
-    ctx->img = nullptr;
-    return fail(ctx, L3P_E_NOMEM, "the fp32 chunk's workspace of %zu bytes does not fit on the device", floats * sizeof(float));
-  }
-  ctx->img_floats = floats;
-  ctx->v_flags_n = n;
+  ctx->img = img;
+  ctx->v_flags = flags;
+  ctx->img_tiles = want;
   return L3P_OK;
 }
 
 template <int CG, int HD>
 static int chunks(l3p_paged_ctx* ctx, PgF32Args a, const PgLists& l, cudaStream_t s) {
-  const size_t tile = PfGeom<HD>::kTileFloats;
-  const int n_kv = ctx->cfg.n_kv_heads;
-  const size_t fit = std::max<size_t>(1, kImageBytes / (tile * sizeof(float) * l.n_prep));
-  const int group = (int)std::min<size_t>(fit, n_kv);
-  if (int rc = ensure_images(ctx, tile * l.n_prep * group, 4 * (size_t)l.n_prep * group, s)) return rc;
+  const int n_kv = ctx->cfg.n_kv_heads, group = image_heads(ctx, l.n_prep);
   ctx->img_captured |= capturing(s);
   a.img = ctx->img;
   a.flags = ctx->v_flags;

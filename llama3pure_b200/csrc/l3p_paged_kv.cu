@@ -154,6 +154,7 @@ int set_rope(l3p_paged_ctx* ctx, const l3p_paged_rope_config& in) {
   }
 
   // everything new is built before anything old goes
+  ctx->retired.reserve(ctx->retired.size() + 3);
   const size_t n = (size_t)r.max_pos * half;
   float2 *tab = nullptr, *tab_swa = nullptr;
   float* norm = nullptr;
@@ -302,15 +303,11 @@ L3P_API int l3p_paged_attn_dev(l3p_paged_ctx* ctx, int layer, const void* q, lon
   DeviceScope dev(ctx->cfg.device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const PgLists& l = ctx->hdr.lists[windowed(ctx, layer) ? 1 : 0];
-  try {
-    if (l.n_tc > 0)
-      if (int rc = ctx->bf16 ? launch_tc(ctx, layer, q, q_stride, out, out_stride, s)
-                             : launch_f32(ctx, layer, q, q_stride, out, out_stride, s))
-        return rc;
-    if (l.row_ctas > 0)
-      if (int rc = launch_rows(ctx, layer, q, q_stride, out, out_stride, s)) return rc;
-    return launch_merge(ctx, l, windowed(ctx, layer), out, out_stride, s);
-  } catch (...) {
-    return fail(ctx, L3P_E_NOMEM, "host memory is exhausted");
-  }
+  if (l.n_tc > 0)
+    if (int rc = ctx->bf16 ? launch_tc(ctx, layer, q, q_stride, out, out_stride, s)
+                           : launch_f32(ctx, layer, q, q_stride, out, out_stride, s))
+      return rc;
+  if (l.row_ctas > 0)
+    if (int rc = launch_rows(ctx, layer, q, q_stride, out, out_stride, s)) return rc;
+  return launch_merge(ctx, l, windowed(ctx, layer), out, out_stride, s);
 }

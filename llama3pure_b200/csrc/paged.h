@@ -138,11 +138,10 @@ struct l3p_paged_ctx {
   unsigned* tickets = nullptr;
   float* tc_o = nullptr;
   float* tc_ml = nullptr;
-  // fp32 pools on the tensor cores: K/V tile images, flags of tiles with values that are not finite
+  // fp32 pools on the tensor cores: K/V tile images, flags of tiles with values that are not finite (l3p_paged_f32.cu)
   float* img = nullptr;
-  size_t img_floats = 0;
   int* v_flags = nullptr;
-  size_t v_flags_n = 0;
+  size_t img_tiles = 0;
   alignas(64) unsigned char tmap[128] = {};  // bf16 pools: the storage as rows of head_dim values (CUtensorMap)
 
   float2* rope_tab = nullptr;      // (cos, sin) [max_pos][rotary_dim/2]
@@ -253,6 +252,9 @@ int init_kv(l3p_paged_ctx* ctx);
 int init_rows(l3p_paged_ctx* ctx);
 int init_tc(l3p_paged_ctx* ctx);
 int init_f32(l3p_paged_ctx* ctx);
+
+// Part of begin, before the books move: the workspace of a planned batch's fp32 chunks.
+int prepare_f32(l3p_paged_ctx* ctx, const l3p::PgHeader& h);
 
 int launch_rows(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void* out, long long os, cudaStream_t s);
 int launch_tc(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void* out, long long os, cudaStream_t s);

@@ -82,6 +82,9 @@ int init_kv(l3p_paged_ctx*) { return L3P_OK; }
 int init_rows(l3p_paged_ctx*) { return L3P_OK; }
 int init_tc(l3p_paged_ctx*) { return L3P_OK; }
 int init_f32(l3p_paged_ctx*) { return L3P_OK; }
+int prepare_f32(l3p_paged_ctx* ctx, const l3p::PgHeader&) {
+  return g_watch && fails() ? fail(ctx, L3P_E_NOMEM, "planted") : (int)L3P_OK;
+}
 int row_limit(const l3p_paged_ctx* ctx) { return ctx->bf16 ? 16 : 64; }
 int row_max_nt(const l3p_paged_ctx*) { return 2; }
 int row_warps(const l3p_paged_ctx*) { return 8; }

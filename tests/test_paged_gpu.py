@@ -868,3 +868,38 @@ def test_rows_that_the_caller_writes_ahead_of_attention(torch, dtype):
             want, tol = _want(torch, q, kv[:, 0], kv[:, 1], past)
             _near(out, want, tol, when)
             b.rows[s] = [kv]
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_begin_makes_the_workspace_of_fp32_chunks(torch, dim):
+    """A chunk whose workspace is larger than any before is captured without a call ahead of it, and a graph captured with
+    smaller images keeps working when later batches need larger ones."""
+    with _cache(n_heads=8, n_kv_heads=2, head_dim=dim, n_layers=1, n_pages=700, max_tokens=6000, max_seqs=3) as c:
+        b = Books(torch, c, dim)
+        s, t = b.new(), b.new()
+        b.step([s], [300])  # loads the kernels
+        graphs = []
+        stream = torch.cuda.Stream()
+        for x, past, n in ((t, 0, 2000), (s, 300, 4000)):
+            q, out = b.randn(n, 8, dim), torch.empty(n, 8, dim, device="cuda")
+            kv = [b.randn(n, 2, dim) for _ in range(2)]
+            c.begin([x], [n])
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                c.append_dev(0, *kv)
+                c.attn_dev(0, q, out)
+            graphs.append((graph, x, past, n, q, out, kv))
+            b.rows[x] = [torch.cat([b.rows[x][0], torch.stack(kv, 1)])]
+            for graph, x, past, n, q, out, kv in graphs:  # the earlier graph too, on a batch of its own
+                c.truncate(x, past)
+                c.begin([x], [n])
+                out.fill_(9.0)
+                torch.cuda.synchronize()
+                graph.replay()
+                torch.cuda.synchronize()
+                c.check()
+                rows = b.rows[x][0]
+                want, tol = _want(torch, q, rows[:, 0], rows[:, 1], past)
+                _near(out, want, tol, f"{n} tokens on {past}")
+        del graph, graphs
