@@ -144,10 +144,11 @@ int set_rope(l3p_paged_ctx* ctx, const l3p_paged_rope_config& in) {
   if (r.scaling == L3P_ROPE_SCALE_YARN) {
     // pair at which a head turns n times over original_len
     auto pair_of = [&](double n) { return dim * log(r.original_len / (n * 2 * pi)) / (2 * log((double)r.theta)); };
-    const double lo = std::max(floor(pair_of(r.beta_fast)), 0.0);
-    const double hi = std::min(ceil(pair_of(r.beta_slow)), dim - 1.0);
+    const double from = floor(pair_of(r.beta_fast)), to = ceil(pair_of(r.beta_slow));
+    const double lo = std::max(from, 0.0), hi = std::min(to, dim - 1.0);
     for (int i = 0; i < half; ++i) {
-      const double ramp = std::min(1.0, std::max(0.0, (i - lo) / (hi == lo ? 0.001 : hi - lo)));
+      // the ramp's ends are moved to the head's values; where all of it lies before the first or behind the last, its side counts
+      const double ramp = to <= 0 ? 1.0 : from > dim - 1.0 ? 0.0 : std::min(1.0, std::max(0.0, (i - lo) / (hi == lo ? 0.001 : hi - lo)));
       freq[i] = freq[i] * (1.0 - ramp) + freq[i] / r.factor * ramp;
     }
     mult = r.attn_factor > 0.f ? r.attn_factor : 0.1 * log((double)r.factor) + 1.0;

@@ -903,3 +903,25 @@ def test_begin_makes_the_workspace_of_fp32_chunks(torch, dim):
                 want, tol = _want(torch, q, rows[:, 0], rows[:, 1], past)
                 _near(out, want, tol, f"{n} tokens on {past}")
         del graph, graphs
+
+
+@pytest.mark.parametrize("original,theta,beta_slow,beta_fast,scaled", [
+    (4, 10000.0, 1.0, 32.0, True), (6, 10000.0, 1.0, 32.0, True), (256, 500000.0, 64.0, 128.0, True),  # every pair turns less than beta_slow times
+    (2**30, 50.0, 1.0, 32.0, False),                                    # every pair turns more than beta_fast times
+])
+def test_yarn_where_no_pair_is_on_the_ramp(torch, original, theta, beta_slow, beta_fast, scaled):
+    turns = [original * theta ** (-2 * i / 128) / (2 * math.pi) for i in range(64)]
+    assert max(turns) < beta_slow if scaled else min(turns) > beta_fast
+    with _cache(n_layers=1) as c:
+        b = Books(torch, c)
+        c.set_rope(max_pos=600, layout="half", scaling="yarn", factor=8.0, original_len=original, theta=theta, beta_slow=beta_slow,
+                   beta_fast=beta_fast, attn_factor=1.25)
+        s = b.new()
+        c.begin([s], [500])
+        q, k, v = b.randn(500, 8, 128), b.randn(500, 2, 128), b.randn(500, 2, 128)
+        out = torch.empty_like(q)
+        c.rope_append_dev(0, q, k, v, out)
+        c.check()
+        pos = torch.arange(500, device="cuda")
+        want = 1.25 * _turned(torch, q, pos, 128, "half", 0, "linear" if scaled else "none", 8.0, 0.0, theta, 0)
+        _rope_near(torch, out, want, "f32", "q")
