@@ -925,3 +925,134 @@ def test_yarn_where_no_pair_is_on_the_ramp(torch, original, theta, beta_slow, be
         pos = torch.arange(500, device="cuda")
         want = 1.25 * _turned(torch, q, pos, 128, "half", 0, "linear" if scaled else "none", 8.0, 0.0, theta, 0)
         _rope_near(torch, out, want, "f32", "q")
+
+
+LONG = [("f32", 32, 8, 128, 9000, 64), ("f32", 16, 8, 128, 66100, 64), ("f32", 8, 1, 64, 20011, 16), ("f32", 8, 1, 256, 5000, 32),
+        ("bf16", 32, 8, 128, 20000, 64), ("bf16", 8, 1, 64, 33000, 16), ("bf16", 8, 1, 256, 7000, 128), ("bf16", 16, 8, 128, 6000, 32)]
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim,past,page", LONG)
+def test_long_histories_by_the_norm_of_the_error(torch, dtype, heads, kv, dim, past, page):
+    """The error of every output row by its norm, relative to the row's own.
+
+    q, k and v are independent and normal, so that errors of the weights meet values of either sign: with a relative error e_j
+    of weight j, an output's error is sum p_j e_j v_j, whose size is at most max |e| of the output's, sum p_j v_j.  bf16: a
+    weight is rounded once (2^-8) and so is the output (2^-8): 2^-7 together; scores are exact products summed in fp32.
+    fp32: scores are about 1 in size and their sums of head_dim products pass through at most 16 roundings and 48 truncations
+    (2^-23 of a partial sum of that size each), mostly 6: 2^-18 with the split's rest (2^-21) and the exponential (2^-22);
+    the second product's partial sums of 16 to 64 keys are cut off likewise (2^-20) and then added in fp32: 2^-17 together.
+    A tile of 16 keys left out moves a row by sqrt(16 / past) of its norm, three times the tolerance and more."""
+    tol = 2**-7 if dtype == "bf16" else 2**-17
+    with _cache(n_heads=heads, n_kv_heads=kv, head_dim=dim, dtype=dtype, n_layers=1, n_pages=(past + 200) // page + 1, page_size=page,
+                max_tokens=past) as c:
+        b = Books(torch, c, past)
+        s = b.new()
+        b.step([s], [past], attend=False)
+        rows = b.rows[s][0]
+        for n in (1, 3, 8, 70, 200):
+            c.begin([s], [n])
+            q, k, v = b.randn(n, heads, dim), b.randn(n, kv, dim), b.randn(n, kv, dim)
+            out = torch.empty_like(q)
+            c.append_dev(0, k, v)
+            c.attn_dev(0, q, out)
+            c.check()
+            full = torch.cat([rows, torch.stack([k, v], 1)])
+            want, _ = _want(torch, q, full[:, 0], full[:, 1], past)
+            size = want.norm(dim=-1)
+            worst = float(((out.double() - want).norm(dim=-1) / size).max())
+            assert worst <= tol, f"{n} tokens: {worst:.3g}, at most {tol:.3g}"
+            if n == 1:  # the tolerance sees a lost tile, wherever it is
+                for at in range(0, past - 16, past // 7):
+                    less = torch.cat([full[:at], full[at + 16:]])
+                    w, _ = _want(torch, q, less[:, 0], less[:, 1], past - 16)
+                    assert float(((w - want).norm(dim=-1) / size).min()) > tol, at
+            c.truncate(s, past)
+
+
+@pytest.mark.parametrize("dtype,dim", [("f32", 64), ("f32", 128), ("f32", 256), ("bf16", 64), ("bf16", 128), ("bf16", 256)])
+def test_strided_outputs(torch, dtype, dim):
+    """Output rows further apart than a token's heads, by every kernel: single tokens, few, chunks with parts that are joined;
+    the values between them stay."""
+    heads, kv = 8, 2
+    with _cache(n_heads=heads, n_kv_heads=kv, head_dim=dim, dtype=dtype, n_layers=1, n_pages=700, max_tokens=9000) as c:
+        b = Books(torch, c, dim)
+        seqs = [b.new() for _ in range(3)]
+        b.step(seqs, [8000, 30, 77], attend=False)
+        for new in ([1, 1, 1], [4, 2, 1], [100, 1, 3], [0, 0, 130]):
+            past, n = [c.length(s) for s in seqs], sum(new)
+            wide = torch.full((n, heads + 3, dim), 7.0, device="cuda", dtype=c.dtype)
+            q = b.randn(n, heads + 1, dim)[:, 1:]
+            k, v = b.randn(n, kv, dim), b.randn(n, kv, dim)
+            c.begin(seqs, new)
+            c.append_dev(0, k, v)
+            c.attn_dev(0, q, wide[:, 2:2 + heads])
+            c.check()
+            assert bool((wide[:, :2] == 7.0).all()) and bool((wide[:, 2 + heads:] == 7.0).all())
+            at = 0
+            for s, p, m in zip(seqs, past, new):
+                b.rows[s][0] = torch.cat([b.rows[s][0], torch.stack([k[at:at + m], v[at:at + m]], 1)])
+                if m:
+                    want, tol = _want(torch, q[at:at + m], b.rows[s][0][:, 0], b.rows[s][0][:, 1], p)
+                    _near(wide[at:at + m, 2:2 + heads], want, tol, f"sequence {s}, {m} tokens")
+                at += m
+
+
+def test_for_shape(torch):
+    """A cache of a model's geometry: heads, and sliding windows where the model has them."""
+    from llama3pure_b200.paged import PagedCache
+    from llama3pure_b200 import synth
+
+    for shape in synth.CONFIGS.values():
+        with PagedCache.for_shape(shape, n_layers=2, page_size=16, n_pages=40, max_seqs=2, max_tokens=600) as c:
+            assert (c.n_heads, c.n_kv_heads, c.head_dim) == (shape.n_heads, shape.n_kv_heads, shape.head_dim)
+            window = shape.swa_window if shape.is_gemma3 else 0
+            assert (c.cfg.is_gemma3, c.cfg.swa_window, c.cfg.swa_pattern) == (shape.is_gemma3, shape.swa_window, shape.swa_pattern)
+            b = Books(torch, c)
+            s = b.new()
+            win = lambda layer: window if window and layer % shape.swa_pattern < shape.swa_pattern - 1 else 0  # noqa: E731
+            b.step([s], [560], window=win)
+            b.step([s], [1], window=win)
+
+
+@pytest.mark.parametrize("dtype,dim", [("f32", 64), ("f32", 128), ("bf16", 64), ("bf16", 128), ("bf16", 256)])
+def test_a_replay_that_does_not_fit_writes_nothing(torch, dtype, dim):
+    """A graph of chunks beside single tokens meets single tokens alone, and a graph of single tokens meets a chunk."""
+    with _cache(n_heads=8, n_kv_heads=2, head_dim=dim, dtype=dtype, n_layers=1, n_pages=800, max_tokens=6000, page_size=16) as c:
+        b = Books(torch, c)
+        seqs = [b.new() for _ in range(3)]
+        b.step(seqs, [5000, 900, 17], attend=False)
+        kinds = {"chunks": [200, 130, 1], "single": [1, 1, 1], "few": [4, 3, 4] if dtype == "bf16" else [9, 4, 5]}
+        q, out = b.randn(400, 8, dim), torch.empty(400, 8, dim, device="cuda", dtype=c.dtype)
+        s = torch.cuda.Stream()
+        graphs = {}
+
+        def begin(new):
+            for x, m in zip(seqs, (5000, 900, 17)):
+                c.truncate(x, m)
+            c.begin(seqs, new)
+
+        for kind, new in kinds.items():
+            begin(new)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(s):
+                c.attn_dev(0, q, out)
+            s.synchronize()
+            graphs[kind] = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graphs[kind], stream=s):
+                c.attn_dev(0, q, out)
+        for kind, new in kinds.items():
+            for other, graph in graphs.items():
+                begin(new)
+                out.fill_(9.0)
+                torch.cuda.synchronize()
+                graph.replay()
+                torch.cuda.synchronize()
+                if other == kind:
+                    c.check()
+                    assert bool((out[:sum(new)] != 9.0).any(-1).all()) and bool((out[sum(new):] == 9.0).all())
+                else:
+                    with pytest.raises(AttnError) as e:
+                        c.check()
+                    assert e.value.code == -1
+                    assert bool((out == 9.0).all()), f"a graph of {other} on {kind}"
+        del graph, graphs
