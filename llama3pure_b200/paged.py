@@ -34,6 +34,11 @@ def _ints(x) -> tuple[int, int, array]:
     return *a.buffer_info(), a
 
 
+def _int(x) -> int:
+    """A whole number of 32 bits (others raise; ctypes would cut them off)."""
+    return array("i", (x,))[0]
+
+
 class PagedCache:
     """One l3p_paged_ctx."""
 
@@ -46,8 +51,8 @@ class PagedCache:
         self.lib = lib or load_library()
         if dtype not in DTYPES:
             raise ValueError(f"dtype {dtype!r}: one of {sorted(DTYPES)}")
-        self.cfg = PagedConfig(n_layers, n_heads, n_kv_heads, head_dim, page_size, n_pages, max_seqs, max_tokens,
-                               max_seq_len, DTYPES[dtype], scale, is_gemma3, swa_window, swa_pattern, device)
+        self.cfg = PagedConfig(*map(_int, (n_layers, n_heads, n_kv_heads, head_dim, page_size, n_pages, max_seqs, max_tokens,
+                                           max_seq_len, DTYPES[dtype])), scale, *map(_int, (is_gemma3, swa_window, swa_pattern, device)))
         self.dtype = torch.bfloat16 if dtype == "bf16" else torch.float32
         self.n_layers, self.n_heads, self.n_kv_heads, self.head_dim = n_layers, n_heads, n_kv_heads, head_dim
         self.device = device
@@ -128,6 +133,7 @@ class PagedCache:
 
     def fork(self, seq: int, n: int = 1, n_tokens: int = -1) -> list[int]:
         """n sequences that share the first n_tokens positions of `seq` (default: all of them)."""
+        seq, n, n_tokens = map(_int, (seq, n, n_tokens))
         out = array("i", bytes(4 * max(n, 1)))
         self._ok(self.lib.l3p_paged_seq_fork(self.h, seq, n_tokens, n, out.buffer_info()[0]), "fork")
         return out.tolist()[:n]
@@ -140,7 +146,7 @@ class PagedCache:
         return out.tolist()
 
     def truncate(self, seq: int, n_tokens: int) -> None:
-        self._ok(self.lib.l3p_paged_seq_truncate(self.h, seq, n_tokens), "truncate")
+        self._ok(self.lib.l3p_paged_seq_truncate(self.h, _int(seq), _int(n_tokens)), "truncate")
 
     def free(self, seqs) -> None:
         p, n, ids = _ints(seqs)
@@ -148,7 +154,7 @@ class PagedCache:
 
     def length(self, seq: int) -> int:
         n = C.c_int()
-        self._ok(self.lib.l3p_paged_seq_length(self.h, seq, C.byref(n)), "length")
+        self._ok(self.lib.l3p_paged_seq_length(self.h, _int(seq), C.byref(n)), "length")
         return n.value
 
     def tables(self, seqs) -> np.ndarray:

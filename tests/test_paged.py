@@ -112,3 +112,26 @@ def test_sizes_whose_product_passes_64_bits_are_refused(lib, kw):
     h = C.c_void_p()
     assert lib.l3p_paged_create(C.byref(_cfg(**kw)), C.byref(h)) == -2
     assert not h.value
+
+
+def test_the_binding_refuses_numbers_beyond_32_bits():
+    """ctypes would cut them off: a cut at 2^32 positions would empty the sequence, a pool of 2^32 + 8 pages have 8."""
+    from llama3pure_b200.paged import PagedCache
+
+    class Lib:  # nothing may be called
+        def __getattr__(self, name):
+            def call(*args):
+                raise AssertionError(f"{name}{args} was called")
+
+            return call
+
+    base = dict(n_layers=2, n_heads=8, n_kv_heads=2, head_dim=128, page_size=16, n_pages=8, max_seqs=4, max_tokens=64)
+    for k in (*base, "max_seq_len", "swa_window", "device"):
+        with pytest.raises(OverflowError):
+            PagedCache(**(base | {k: 2**32 + 8}), lib=Lib())
+    c = PagedCache.__new__(PagedCache)
+    c.lib, c.h = Lib(), None
+    for call in (lambda: c.truncate(0, 2**32), lambda: c.truncate(2**32, 0), lambda: c.fork(0, 1, 2**32), lambda: c.fork(2**32), lambda: c.fork(0, 2**32),
+                 lambda: c.length(2**32), lambda: c.free([2**32]), lambda: c.begin([0], [2**32])):
+        with pytest.raises(OverflowError):
+            call()
