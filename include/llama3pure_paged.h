@@ -17,7 +17,9 @@
  *
  * Conventions (beside those of llama3pure_attn.h, whose codes are used)
  *   - Rows are of the pool's type: float with L3P_PAGED_F32, bfloat16 with
- *     L3P_PAGED_BF16.  Scores, softmax statistics and sums are fp32 in both.
+ *     L3P_PAGED_BF16.  Scores, softmax statistics and sums are fp32 in both;
+ *     with BF16 rows a weight is rounded to bfloat16 ahead of its product with
+ *     V, and so is the output; fp32 products are right to 2^-21 of themselves.
  *   - Token rows of a batch are stacked in the order of l3p_paged_begin's
  *     sequences: q, out [n_tok][n_heads][head_dim], k, v
  *     [n_tok][n_kv_heads][head_dim].  Strides are elements from one token to
@@ -61,7 +63,9 @@ typedef struct l3p_paged_config {
     int n_pages;      /* pages of the pool */
     int max_seqs;     /* sequences that may exist at once */
     int max_tokens;   /* new tokens of one batch at most */
-    int max_seq_len;  /* positions of one sequence at most; 0 => n_pages * page_size */
+    int max_seq_len;  /* positions of one sequence at most; 0 => n_pages * page_size.  The device block of a step's
+                         description has room for max_seqs tables of that many positions (a word a page; F32 pools: and
+                         four words per 128 positions): 64 sequences in a pool of 64K pages: 17 MB */
     int dtype;        /* L3P_PAGED_F32 or L3P_PAGED_BF16 */
     float scale;      /* multiplies q.k, not negative; 0 => 1/sqrt(head_dim) */
     int is_gemma3;    /* sliding-window layers as in l3p_attn_config: with is_gemma3, */
@@ -161,7 +165,10 @@ int l3p_paged_append_dev(l3p_paged_ctx* ctx, int layer, const void* k, long long
  * t attends to positions [max(0, t - window + 1), t] (windowed layers) or
  * [0, t].  The new tokens' K/V rows must have been appended.  Rows of out
  * behind the batch's last token are left as they were.  Positions that a token
- * does not attend to never reach its output, whatever they hold.
+ * does not attend to never reach its output, whatever they hold.  A value that
+ * is not finite at a position that it does attend to leaves values that are not
+ * finite (F32 pools: NaN also where the formula has an infinity or, for a key,
+ * a weight of 0).
  *
  * Capture: a captured launch reads the batch's description when it is
  * replayed, so one graph of a decoding step serves every later step whose
@@ -169,7 +176,8 @@ int l3p_paged_append_dev(l3p_paged_ctx* ctx, int layer, const void* k, long long
  * with n_new * n_heads / n_kv_heads query rows per KV head, the largest count
  * of a batch of few tokens is at most 8, or 9 to 16 (F32 pools: 9 to 64, with
  * head_dim 256 9 and more).  A replay on a batch that does not fit writes
- * nothing for it and l3p_paged_check reports L3P_E_INVAL. */
+ * nothing for it and l3p_paged_check reports L3P_E_INVAL.  A graph of chunks
+ * serves batches whose plan has no more parts, which goes by the lengths too. */
 int l3p_paged_attn_dev(l3p_paged_ctx* ctx, int layer, const void* q, long long q_stride, void* out,
                        long long out_stride, void* stream);
 

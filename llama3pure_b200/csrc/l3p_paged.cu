@@ -128,7 +128,7 @@ struct BatchSeq {
 
 // Which kernels a sequence takes: the row kernel up to row_limit rows per KV head.  In bf16, sequences of 9 to row_limit
 // rows go with the longer ones where there are some: two kernels, each with part of the batch, fill the GPU less than one
-// (16 drafts of 12 to 24 rows, 8B heads: 58.6 us, by two kernels 72.5).
+// (16 drafts of 12 to 24 rows on 3000 keys, 8B heads, layers in turn: 44.2 us, by two kernels 62.5).
 void choose_paths(const Ctx* ctx, std::vector<BatchSeq>* bs) {
   const int limit = row_limit(ctx);
   bool any = false;
@@ -147,8 +147,9 @@ int first_key(const Ctx* ctx, bool win, int pos) { return win ? std::max(0, pos 
 //     CTAs): one segment per CTA, the longest part sets the time.
 // A run or part is a multiple of the CTA's warps, which take its tiles in turn,
 // so both are counted in rounds of one tile per warp.  A further segment of a CTA
-// costs about kSegRounds rounds that its prefetched tiles do not hide (16
-// sequences x 4 tokens x 3000 keys, 8B heads: 46.8 us end to end, 38.5 us by units).
+// costs about kSegRounds rounds that its prefetched tiles do not hide (8B heads:
+// one token on 8K keys 17.3 us end to end, 12.4 by units; 4 sequences x 3000 keys
+// 18.0 and 14.3; with 128 units, 16 sequences x 4 tokens, 43 either way).
 constexpr double kSegRounds = 1.5;
 void plan_rows(Ctx* ctx, bool win, const std::vector<BatchSeq>& bs, int nt, std::vector<int>* first,
                std::vector<PgSeg>* segs) {

@@ -261,7 +261,7 @@ L3P_API int l3p_paged_rope_append_dev(l3p_paged_ctx* ctx, int layer, const void*
   a.rotary = ctx->rotary_dim;
   a.interleaved = ctx->rope_layout == L3P_ROPE_INTERLEAVED;
   // Tokens stream through shared memory where two of them fit a CTA's ring and a table row is whole 16-byte pieces (8B
-  // heads, bf16: 64 tokens 2.9 us, 8192 tokens 43.8 us; by the kernel below 3.9 and 109 us).
+  // heads, bf16, call after call: 64 tokens 2.7 us, 8192 tokens 39.3 us; by the kernel below 3.6 and 103 us).
   const int token_bytes = (c.n_heads + 2 * c.n_kv_heads) * ctx->hd * ctx->es + ctx->rotary_dim * 4 + 128;
   if (2 * token_bytes <= kRingBytes && ctx->rotary_dim % 4 == 0)
     return ctx->bf16 ? launch_rope_ring<__nv_bfloat16>(ctx, a, static_cast<cudaStream_t>(stream))

@@ -9,10 +9,10 @@ using namespace l3p;
 
 namespace l3p_pg {
 
-// Sequences with more query rows per KV head take the tensor-core kernels.  16 sequences of 3000 keys, 8B heads, by the
-// row kernel and by the tensor-core kernel: bf16 16 rows 38.3 and 40.4 us (one such sequence 10.7 and 18.5), 32 rows 75.6
-// (blocks of 32 rows, since dropped) and 42.6; fp32, whose tensor-core kernel first splits every key tile, 64 rows 391 and
-// 459 us, 128 rows 751 and 465.  fp32 with head_dim 256 has none: Q and O alone would fill tensor memory.
+// Sequences with more query rows per KV head take the tensor-core kernels.  16 sequences of 3000 keys, 8B heads, layers in
+// turn, by the row kernel and by the tensor-core kernel: bf16 16 rows 43.8 and 44.0 us (one such sequence 12.4 and 18.4), 32
+// rows, blocks of 16, 77.6 and 45.2; fp32, whose tensor-core kernel first splits every key tile, 64 rows 397 and 472 us (34.1
+// and 65.0), 128 rows 778 and 489.  fp32 with head_dim 256 has none: Q and O of a key tile of 128 would fill tensor memory.
 int row_limit(const l3p_paged_ctx* ctx) {
   return ctx->bf16 ? 16 : ctx->hd == 256 ? INT_MAX : 64;
 }

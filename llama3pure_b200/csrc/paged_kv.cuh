@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kPgRingThreads) paged_rope_ring_kernel(const P
   }
   __syncthreads();
   griddep_wait();  // the rows come from the kernel before this one
-  griddep_launch();  // not earlier: attention's CTAs would only wait, on SMs that turn rows (8 fp32 sequences: 25.0 us, 25.7)
+  griddep_launch();  // not earlier: the next kernel's CTAs would only wait (64 tokens, 8B heads, call after call: 2.7 us, 2.9)
   if (n_tok > a.n_tokens) {
     if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
     return;

@@ -62,8 +62,9 @@ struct PgRowCfg {
   static constexpr int kTileBytes = kPgTile * kRow;  // a tile's K or V
   // 192 KB of rings per CTA, at least three places per warp: the one that it computes on and those in flight.  A place
   // holds K and V of a tile; for fp32, whose split products keep a warp on a tile for 2.5K cycles, K or V, which makes room
-  // for twice the warps (one token on 128K keys, 8B heads: 175 -> 157 us; Gemma heads, 64 sequences: 264 -> 152; bf16 loses
-  // 5 % to the second wait a tile).  Four warps for head_dim 256, whose merge buffer is twice as large.
+  // for twice the warps (one token on 128K keys, 8B heads, the same 1.07 GB call after call, of which L2 keeps a tenth: 181 ->
+  // 163 us; on caches in turn 182 us = 5.9 TB/s.  64 sequences of 4095, Gemma heads: 250 -> 142 us.  bf16 loses 5 % to the
+  // second wait a tile).  Four warps for head_dim 256, whose merge buffer is twice as large.
   static constexpr bool kPair = kEs == 2;
   static constexpr int kPlaceBytes = kPair ? 2 * kTileBytes : kTileBytes;
   static constexpr int kWarps = HD == 256 ? 4 : 8;

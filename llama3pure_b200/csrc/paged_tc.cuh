@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
     // Few instructions a load: the softmax warps want the issue slots, and at 16 or 32 positions a page these loads bound
     // the kernel (16 sequences x 9 tokens x 3000 keys, 8B heads, pages of 16: 49.5 us with stages and tiles found by
     // division from the load's number, 44.0 us with running counters and a page looked up a tile ahead, 41.1 us with a warp
-    // for K and one for V).  A load waits for the release one ring earlier, and the warp's load before it has waited for a
+    // for K and one for V, 42.5 us since barriers go by the tile's number).  A load waits for the release one ring earlier, and the warp's load before it has waited for a
     // later release than the one two rings earlier: one phase.
     const bool is_v = warp == 3;
     const int box = min(1 << a.shift, TN), n_box = TN / box;  // keys of a box, boxes down a tile
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(PgTcCfg<HD>::kThreads, 1)
       return r;
     };
     bool ok = true;
-    // running numbers instead of divisions (16 sequences x 9 tokens x 3000 keys, head_dim 64: 29.3 -> 26.8 us): V tile j's and
+    // running numbers instead of divisions (16 sequences x 9 tokens x 3000 keys, head_dim 64: 29.3 -> 26.8 us; now 27.9): V tile j's and
     // the next K tile's barriers, phases and stages
     int vb = 0, vp = 0, kb = 0, kp = 0;
     auto next_v = [&] { if (++vb == S) vb = 0, vp ^= 1; };
