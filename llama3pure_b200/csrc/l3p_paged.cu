@@ -706,7 +706,7 @@ int compact(Ctx* ctx, int* n_used, cudaStream_t s) {
   if (int rc = refuse_capture(ctx, s, "compact")) return rc;
   const int k = ctx->cfg.n_pages - (int)ctx->free_heap.size();
   std::vector<int4> jobs;
-  jobs.reserve(ctx->cfg.n_pages - k);
+  jobs.reserve(std::min(k, ctx->cfg.n_pages - k));
   std::vector<int> moved(ctx->cfg.n_pages, -1);
   int dst = 0;
   for (int p = k; p < ctx->cfg.n_pages; ++p) {

@@ -85,7 +85,7 @@ int launch_rows(l3p_paged_ctx* ctx, int layer, const void* q, long long qs, void
   a.ws_ml = ctx->ws_ml;
   a.tickets = ctx->tickets;
   a.err = ctx->err_dev;
-  // a captured launch may meet a batch that uses more CTAs
+  // a captured launch may meet a batch that uses more CTAs, of which plan_rows makes no more than SMs
   const int grid = capturing(s) ? ctx->num_sms : l.row_ctas;
   return with_kernel(ctx, ctx->hdr.row_nt,
                      [&](auto kernel, int threads, int smem) { return launch(ctx, kernel, dim3(grid), threads, smem, s, 1, a); });

@@ -67,15 +67,17 @@ struct __align__(16) PgPart {
 };
 static_assert(sizeof(PgPart) == 64, "part");
 
-// What a launch was made for: a batch that it meets when it is replayed must
-// not exceed it (fits), else nothing is written and the error word is set.
+// What a call's launches were made for: a batch that they meet when they are
+// replayed must not exceed it (fits), else nothing is written and the error word
+// is set.  All launches of a call decide alike.
 struct PgLimits {
-  int n_tokens, n_tc, n_merge, n_prep, with_rows, with_tc;
+  int n_tokens, n_tc, n_merge, n_prep, with_tc;
+  int with_rows;  // blocks of 8 rows that the row kernel's instance takes; 0: no row kernel
 };
 #ifdef __CUDACC__
 __device__ __forceinline__ bool pg_fits(const PgHeader* h, const PgLists& l, const PgLimits& m) {
   return h->n_tokens <= m.n_tokens && l.n_tc <= m.n_tc && l.n_merge <= m.n_merge && l.n_prep <= m.n_prep &&
-         (l.row_ctas != 0) == (m.with_rows != 0) && (l.n_tc != 0) == (m.with_tc != 0);
+         (l.row_ctas != 0 ? h->row_nt : 0) == m.with_rows && (l.n_tc != 0) == (m.with_tc != 0);
 }
 #endif
 
@@ -235,7 +237,7 @@ int launch(l3p_paged_ctx* ctx, void (*kernel)(P...), dim3 grid, int threads, int
 }
 
 inline l3p::PgLimits limits(const l3p_paged_ctx* ctx, const l3p::PgLists& l) {
-  return {ctx->hdr.n_tokens, l.n_tc, l.n_merge, l.n_prep, l.row_ctas > 0, l.n_tc > 0};
+  return {ctx->hdr.n_tokens, l.n_tc, l.n_merge, l.n_prep, l.n_tc > 0, l.row_ctas > 0 ? ctx->hdr.row_nt : 0};
 }
 
 // Rows per KV head up to which a sequence takes the row kernel, and the key

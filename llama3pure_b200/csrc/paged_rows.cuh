@@ -167,9 +167,10 @@ __global__ void __launch_bounds__(PgRowCfg<T, HD>::kWarps * 32, 1) paged_rows_ke
   // In a batch with chunks this kernel follows a tensor-core kernel, which lets it start once all of its CTAs have seen the
   // kernel before them complete.  The two read the same rows and write others, so they run side by side; this one's CTAs
   // wait at their end, so that what follows this kernel follows both.
-  if (!pg_fits(h, l, a.lim) || h->row_nt != NT || l.row_ctas > (int)gridDim.x || (int)blockIdx.x >= l.row_ctas) {
+  const bool fits = pg_fits(h, l, a.lim);
+  if (!fits || (int)blockIdx.x >= l.row_ctas) {
     griddep_wait();
-    if ((int)blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
+    if (!fits && blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = kErrBadArg;
     return;
   }
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;

@@ -1056,3 +1056,46 @@ def test_a_replay_that_does_not_fit_writes_nothing(torch, dtype, dim):
                     assert e.value.code == -1
                     assert bool((out == 9.0).all()), f"a graph of {other} on {kind}"
         del graph, graphs
+
+
+@pytest.mark.parametrize("dtype,dim", [("f32", 64), ("f32", 128), ("bf16", 64), ("bf16", 128)])
+def test_a_replay_whose_row_part_does_not_fit_writes_nothing(torch, dtype, dim):
+    """A graph of a chunk beside single tokens, of another row path than the batch that it meets: both parts stay out."""
+    with _cache(n_heads=8, n_kv_heads=2, head_dim=dim, dtype=dtype, n_layers=1, n_pages=300, max_tokens=3000) as c:
+        b = Books(torch, c)
+        seqs = [b.new() for _ in range(3)]
+        q, out = b.randn(600, 8, dim), torch.empty(600, 8, dim, device="cuda", dtype=c.dtype)
+        kinds = [[300, 1, 1], [300, 4, 1] if dtype == "f32" else [300, 0, 2]]  # fp32: 16 rows per KV head, another kernel
+        s = torch.cuda.Stream()
+        graphs = []
+
+        def begin(new):
+            for x in seqs:
+                c.truncate(x, 0)
+            c.begin(seqs, new)
+
+        for new in kinds:
+            begin(new)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(s):
+                c.attn_dev(0, q, out)
+            s.synchronize()
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=s):
+                c.attn_dev(0, q, out)
+        for i, new in enumerate(kinds):
+            for j, graph in enumerate(graphs):
+                begin(new)
+                c.attn_dev(0, q, out)
+                want = out.clone()
+                out.fill_(9.0)
+                torch.cuda.synchronize()
+                graph.replay()
+                torch.cuda.synchronize()
+                try:
+                    c.check()
+                    assert bool((out[:sum(new)] == want[:sum(new)]).all()) and bool((out[sum(new):] == 9.0).all())
+                except AttnError as e:
+                    assert e.code == -1 and i != j
+                    assert bool((out == 9.0).all()), f"a graph of {kinds[j]} on {new}"
+        del graph, graphs
