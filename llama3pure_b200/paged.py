@@ -39,6 +39,15 @@ def _int(x) -> int:
     return array("i", (x,))[0]
 
 
+class _Memory:
+    """A cache's storage for torch, which holds this object by its tensor: the cache lives as long as that.  No class of its own
+    for every tensor: a class is part of a reference cycle, and the pool would stay until a garbage collection."""
+
+    def __init__(self, owner, interface: dict):
+        self.owner = owner
+        self.__cuda_array_interface__ = interface
+
+
 class PagedCache:
     """One l3p_paged_ctx."""
 
@@ -114,15 +123,11 @@ class PagedCache:
         base, size = C.c_void_p(), C.c_size_t()
         self._ok(self.lib.l3p_paged_storage(self.h, C.byref(base), C.byref(size)), "storage")
         c = self.cfg
-
-        class _Memory:  # bfloat16 has no array-interface type: 16-bit integers, viewed below
-            owner = self  # the tensor holds this object, and so the cache
-            __cuda_array_interface__ = {
-                "shape": (c.n_pages, c.n_layers, 2, c.n_kv_heads, c.page_size, c.head_dim),
-                "typestr": "<f4" if c.dtype == 0 else "<i2", "data": (base.value, False), "version": 3, "stream": None,
-            }
-
-        t = self.torch.as_tensor(_Memory(), device=f"cuda:{self.device}")
+        memory = _Memory(self, {  # bfloat16 has no array-interface type: 16-bit integers, viewed below
+            "shape": (c.n_pages, c.n_layers, 2, c.n_kv_heads, c.page_size, c.head_dim),
+            "typestr": "<f4" if c.dtype == 0 else "<i2", "data": (base.value, False), "version": 3, "stream": None,
+        })
+        t = self.torch.as_tensor(memory, device=f"cuda:{self.device}")
         return t if c.dtype == 0 else t.view(self.torch.bfloat16)
 
     # -- sequences and pages -----------------------------------------------------

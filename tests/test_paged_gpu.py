@@ -1099,3 +1099,25 @@ def test_a_replay_whose_row_part_does_not_fit_writes_nothing(torch, dtype, dim):
                     assert e.code == -1 and i != j
                     assert bool((out == 9.0).all()), f"a graph of {kinds[j]} on {new}"
         del graph, graphs
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_dropped_cache_is_gone_at_once(torch, dtype):
+    """Not when the garbage collector comes: a pool is large, and freeing one in the middle of another's capture would end that."""
+    import gc
+    import weakref
+
+    gc.collect()
+    gc.disable()
+    try:
+        c = _cache(n_layers=1, dtype=dtype)
+        gone = weakref.ref(c)
+        st = c.storage()
+        c.storage().zero_()
+        view = st[1:2]
+        del c, st
+        assert gone() is not None and not bool(view.any())
+        del view
+        assert gone() is None
+    finally:
+        gc.enable()
