@@ -202,9 +202,12 @@ struct DeviceScope {
   }
 };
 
+// Whether `s` captures; of the null stream: or a stream that work on it would wait for.
 inline bool capturing(cudaStream_t s) {
   cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-  return cudaStreamIsCapturing(s, &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
+  const cudaError_t e = cudaStreamIsCapturing(s, &st);
+  if (e != cudaSuccess) cudaGetLastError();
+  return e == cudaErrorStreamCaptureImplicit || (e == cudaSuccess && st != cudaStreamCaptureStatusNone);
 }
 
 inline bool windowed(const l3p_paged_ctx* ctx, int layer) {

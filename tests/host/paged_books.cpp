@@ -38,9 +38,8 @@ static cudaError_t give(void** p, size_t n) {
   *p = calloc(n ? n : 1, 1);
   return *p ? cudaSuccess : cudaErrorMemoryAllocation;
 }
-static bool g_capturing = false;
-static std::string g_device_error;  // name of the call that fails
-static cudaError_t result(const char* name) { return g_watch && g_device_error == name ? cudaErrorUnknown : cudaSuccess; }
+static bool g_capturing = false;  // the stream
+static bool g_implicit = false;   // another stream, which work on the null stream would wait for
 extern "C" {
 cudaError_t cudaGetDevice(int* d) { return *d = 0, cudaSuccess; }
 cudaError_t cudaSetDevice(int) { return cudaSuccess; }
@@ -56,7 +55,7 @@ cudaError_t cudaFreeHost(void* p) { return free(p), cudaSuccess; }
 cudaError_t cudaHostGetDevicePointer(void** d, void* h, unsigned) { return *d = h, cudaSuccess; }
 cudaError_t cudaMemset(void* p, int v, size_t n) { return memset(p, v, n), cudaSuccess; }
 cudaError_t cudaMemcpyAsync(void* d, const void* s, size_t n, cudaMemcpyKind, cudaStream_t) {
-  if (cudaError_t e = result("cudaMemcpyAsync")) return e;
+  if (g_capturing || g_implicit) return cudaErrorStreamCaptureImplicit;
   return memcpy(d, s, n), cudaSuccess;
 }
 cudaError_t cudaEventCreateWithFlags(cudaEvent_t* e, unsigned) { return give(reinterpret_cast<void**>(e), 1); }
@@ -66,7 +65,8 @@ cudaError_t cudaEventDestroy(cudaEvent_t e) { return free(e), cudaSuccess; }
 cudaError_t cudaDeviceSynchronize() { return cudaSuccess; }
 cudaError_t cudaStreamSynchronize(cudaStream_t) { return cudaSuccess; }
 cudaError_t cudaStreamIsCapturing(cudaStream_t, cudaStreamCaptureStatus* s) {
-  return *s = g_capturing ? cudaStreamCaptureStatusActive : cudaStreamCaptureStatusNone, cudaSuccess;
+  *s = g_capturing ? cudaStreamCaptureStatusActive : cudaStreamCaptureStatusNone;
+  return g_implicit ? cudaErrorStreamCaptureImplicit : cudaSuccess;
 }
 cudaError_t cudaGetLastError() { return cudaSuccess; }
 const char* cudaGetErrorString(cudaError_t) { return "planted"; }
@@ -92,7 +92,6 @@ int tc_tile(const l3p_paged_ctx*) { return 128; }
 int tc_rows(const l3p_paged_ctx*) { return 256; }
 int f32_rows(const l3p_paged_ctx*) { return 256; }
 int launch_page_copy(l3p_paged_ctx* ctx, const int* jobs, int n, cudaStream_t) {
-  if (result("page copy") != cudaSuccess) return fail(ctx, L3P_E_CUDA, "planted");
   char* base = static_cast<char*>(ctx->storage);
   for (int i = 0; i < n; ++i, jobs += 4)
     for (size_t b = 0; b < ctx->page_bytes; b += ctx->block_bytes)
@@ -239,11 +238,35 @@ static void create_everywhere(int dtype) {
   EXPECT(refused > 5);
 }
 
+// Calls that move host data, on a stream that captures and on the null stream while another one does.
+static void refused_in_capture(int dtype) {
+  int ids[8], free_id[1];
+  l3p_paged_ctx* ctx = make(dtype);
+  fill(ctx, ids);
+  free_id[0] = ids[1];
+  EXPECT(l3p_paged_seq_free(ctx, 1, free_id) == L3P_OK);  // holes for compact
+  const int one[1] = {1};
+  EXPECT(l3p_paged_begin(ctx, 1, ids + 2, one, nullptr) == L3P_OK);
+  const Seen before = look(ctx);
+  for (bool* how : {&g_capturing, &g_implicit}) {
+    *how = true;
+    int children[1], used;
+    EXPECT(l3p_paged_begin(ctx, 1, ids, one, nullptr) == L3P_E_INVAL);
+    EXPECT(l3p_paged_seq_copy(ctx, 1, ids, children, nullptr) == L3P_E_INVAL);
+    EXPECT(l3p_paged_compact(ctx, &used, nullptr) == L3P_E_INVAL);
+    *how = false;
+    EXPECT(look(ctx) == before);
+  }
+  l3p_paged_destroy(ctx);
+}
+
 int main(int argc, char** argv) {
   const std::string test = argc > 1 ? argv[1] : "";
   g_fail_rest = argc > 2 && std::string(argv[2]) == "rest";
   for (int dtype : {L3P_PAGED_F32, L3P_PAGED_BF16}) {
-    if (test == "create") {
+    if (test == "capture") {
+      refused_in_capture(dtype);
+    } else if (test == "create") {
       create_everywhere(dtype);
     } else if (test == "begin") {
       fail_everywhere("begin", dtype, begin_call);

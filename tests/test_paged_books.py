@@ -1,5 +1,6 @@
 """The paged cache's books without a GPU (tests/host/paged_books.cpp): calls that
-find no memory, pinned or ordinary, change nothing."""
+find no memory, pinned or ordinary, and calls that a capture does not allow change
+nothing."""
 import os
 import subprocess
 
@@ -36,3 +37,7 @@ def test_no_exception_leaves_a_call_when_memory_is_exhausted(books, call):
 def test_create_without_memory_says_why(books):
     books("create")
     books("create", "rest")
+
+
+def test_capture_of_the_stream_or_of_one_that_the_null_stream_waits_for(books):
+    books("capture")
