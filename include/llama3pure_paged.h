@@ -83,7 +83,8 @@ void l3p_paged_destroy(l3p_paged_ctx* ctx);
 const char* l3p_paged_last_error(const l3p_paged_ctx* ctx);
 /* Waits for `stream` and reports what its kernels recorded, clearing it:
  * L3P_E_TIMEOUT after a bounded wait gave up, L3P_E_INVAL when a captured
- * launch met a batch that it cannot serve (see l3p_paged_attn_dev). */
+ * launch met a batch that it cannot serve (see l3p_paged_attn_dev).  Not during
+ * stream capture. */
 int l3p_paged_check(l3p_paged_ctx* ctx, void* stream);
 /* Kernels launched since the context was created. */
 long long l3p_paged_launch_count(const l3p_paged_ctx* ctx);

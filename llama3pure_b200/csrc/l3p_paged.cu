@@ -775,6 +775,7 @@ L3P_API long long l3p_paged_launch_count(const l3p_paged_ctx* ctx) { return ctx 
 L3P_API int l3p_paged_check(l3p_paged_ctx* ctx, void* stream) {
   if (!ctx) return L3P_E_INVAL;
   DeviceScope dev(ctx->cfg.device);
+  if (capturing(as_stream(stream))) return fail(ctx, L3P_E_INVAL, "check waits for the stream: not during stream capture");
   PG_CUDA(ctx, cudaStreamSynchronize(as_stream(stream)));
   const int e = *ctx->err_host;
   *ctx->err_host = 0;

@@ -254,6 +254,7 @@ static void refused_in_capture(int dtype) {
     EXPECT(l3p_paged_begin(ctx, 1, ids, one, nullptr) == L3P_E_INVAL);
     EXPECT(l3p_paged_seq_copy(ctx, 1, ids, children, nullptr) == L3P_E_INVAL);
     EXPECT(l3p_paged_compact(ctx, &used, nullptr) == L3P_E_INVAL);
+    EXPECT(l3p_paged_check(ctx, nullptr) == L3P_E_INVAL);  // a wait would end the capture
     *how = false;
     EXPECT(look(ctx) == before);
   }

@@ -1121,3 +1121,28 @@ def test_a_dropped_cache_is_gone_at_once(torch, dtype):
         assert gone() is None
     finally:
         gc.enable()
+
+
+def test_check_during_capture_leaves_the_capture(torch):
+    with _cache(n_layers=1) as c:
+        b = Books(torch, c)
+        s = b.new()
+        b.step([s], [20], attend=False)
+        c.begin([s], [1])
+        q, out = b.randn(1, 8, 128), torch.full((1, 8, 128), 9.0, device="cuda")
+        k, v = b.randn(1, 2, 128), b.randn(1, 2, 128)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            c.append_dev(0, k, v)
+            with pytest.raises(AttnError) as e:
+                c.check()
+            c.attn_dev(0, q, out)
+        assert e.value.code == -1
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check()
+        rows = torch.cat([b.rows[s][0], torch.stack([k, v], 1)])
+        want, tol = _want(torch, q, rows[:, 0], rows[:, 1], 20)
+        _near(out, want, tol)
+        del graph
