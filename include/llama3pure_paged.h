@@ -34,9 +34,9 @@
  *     or copy; work on it that is already enqueued comes first when the stream
  *     is the same.
  *   - new, fork, begin, truncate, free, copy and compact check everything
- *     first: a call that they refuse changes nothing, also for want of host or
- *     pinned memory (L3P_E_NOMEM).  L3P_E_CUDA is a failure of the device, after
- *     which the pool's rows are not defined.
+ *     first: a call that they refuse changes nothing, also for want of host,
+ *     pinned or device memory (L3P_E_NOMEM).  L3P_E_CUDA is a failure of the
+ *     device, after which the pool's rows are not defined.
  *   - Freeing, truncating or compacting ends the current batch: append and
  *     attention are refused until the next begin.
  */

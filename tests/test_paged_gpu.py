@@ -1146,3 +1146,62 @@ def test_check_during_capture_leaves_the_capture(torch):
         want, tol = _want(torch, q, rows[:, 0], rows[:, 1], 20)
         _near(out, want, tol)
         del graph
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_pools_of_more_values_than_32_bits_count(torch, dtype):
+    """Pages behind the 2^32nd value of a pool: rotation, append, copies, compaction, and every attention kernel."""
+    with _cache(n_heads=8, n_kv_heads=8, head_dim=128, dtype=dtype, n_layers=32, page_size=128, n_pages=620, max_tokens=80000, max_seqs=4) as c:
+        assert c.storage()[590].storage_offset() > 2**32
+        c.set_rope(max_pos=600)
+        b = Books(torch, c)
+        full = c.new_seq()
+        c.begin([full], [595 * 128])  # the pages before, without rows
+        ids, rows = [c.new_seq() for _ in range(2)], [[], []]
+        layer = 31
+
+        def step(seqs, new):
+            c.begin([ids[i] for i in seqs], new)
+            n = sum(new)
+            q, k, v = b.randn(n, 8, 128), b.randn(n, 8, 128), b.randn(n, 8, 128)
+            qr, out = torch.empty_like(q), torch.empty_like(q)
+            c.rope_append_dev(layer, q, k, v, qr)
+            c.attn_dev(layer, qr, out)
+            c.check()
+            at = 0
+            for i, m in zip(seqs, new):
+                past = sum(len(x) for x in rows[i])
+                t = torch.from_numpy(c.tables([ids[i]])[0]).cuda().long()
+                pos = torch.arange(past, past + m, device="cuda")
+                got = c.storage()[t[pos // 128], layer, :, :, pos % 128]
+                kr = _turned(torch, k[at:at + m], pos, 128, "interleaved", 0, "none", 1.0, 0.0, 500000.0, 0)
+                _rope_near(torch, got[:, 0], kr, dtype, "k")
+                assert bool((got[:, 1] == v[at:at + m]).all())
+                rows[i].append(got.clone())
+                h = torch.cat(rows[i])
+                want, tol = _want(torch, qr[at:at + m], h[:, 0], h[:, 1], past)
+                _near(out[at:at + m], want, tol, f"{m} tokens on {past}")
+                at += m
+
+        step([0, 1], [300, 40])
+        assert all(int(c.tables([i]).min()) >= 595 for i in ids)
+        step([0, 1], [1, 1])
+        step([0, 1], [3, 2])
+        k, v = b.randn(1, 8, 128), b.randn(1, 8, 128)
+        c.begin([ids[1]], [1])
+        c.append_dev(layer, k, v)
+        c.check()
+        rows[1].append(torch.stack([k, v], 1))
+        t = c.tables([ids[1]])[0]
+        assert bool((c.storage()[int(t[-1]), layer, :, :, (c.length(ids[1]) - 1) % 128] == rows[1][-1][0]).all())
+        kid = c.copy([ids[0]])[0]
+        h = torch.cat(rows[0])
+        for s in (kid, None):
+            if s is None:  # moved to the front
+                c.truncate(full, 0)
+                assert c.compact() <= 10
+                s = ids[0]
+            t = torch.from_numpy(c.tables([s])[0]).cuda().long()
+            pos = torch.arange(len(h), device="cuda")
+            assert bool((c.storage()[t[pos // 128], layer, :, :, pos % 128] == h).all())
+        step([0, 1], [1, 1])
